@@ -31,6 +31,11 @@ extern "C" {
 #define NERF_EINVAL (-22) /* bad argument (shape, null pointer, unsupported size) */
 #define NERF_ELAUNCH (-5) /* the HIP runtime rejected a launch                    */
 
+/* Element types of the operators that take more than float32 (the `*_type` arguments). */
+#define NERF_F32 0
+#define NERF_BF16 1
+#define NERF_F16 2
+
 int nerf_abi_version(void);
 const char* nerf_last_error(void);
 
@@ -196,6 +201,33 @@ int nerf_gather_kept(const float* d_rgb, const float* d_sigma, const int32_t* ke
  * (entries behind the count stay untouched). */
 int nerf_gather_kept_by_slot(const float* d_rgb, const float* d_sigma, const int32_t* slot, int64_t P,
                              float* d_rgb_kept, float* d_sigma_kept, void* stream);
+
+/* Gated linear recurrence along a sequence or a ray, no counterpart in the reference beyond its
+ * compositing loop (src/Camera.py:143-183), whose back-to-front form it generalises:
+ *   h_t = a_t h_{t-1} + x_t,   or with blend  h_t = a_t h_{t-1} + (1 - a_t) x_t,
+ * over t = 0..T-1 (reverse: T-1..0), h before the first step = state (NULL: zeros).
+ * x, h [B,T,C] of x_type; gate [B,T,G], of x_type or float32, G dividing C: channel c takes gate
+ * c / (C/G) (G = C: one per channel, G = 1: one per step); state, last [B,C] float32; last (may be
+ * NULL) receives the state after the last step.  The state is held in float32; h is rounded once.
+ * Made for |gate| <= 1; larger gates are right as long as float32 holds their products over
+ * stretches of the sequence.  Infinities and NaN propagate as in the formula.
+ * carry: nerf_linear_scan_carry_floats(B,T,C,G) floats that the backward pass needs (NULL: not
+ * kept).  workspace: nerf_linear_scan_workspace_floats(B,T,C,G,backward) floats, NULL where that is
+ * 0.  T >= 1; B = 0 or C = 0 is nothing to do.  Every pointer 16-byte aligned.
+ * bwd: d_h [B,T,C] of x_type and d_last [B,C] (either may be NULL: zeros) -> d_gate (gate's type and
+ * shape; the sum over the channels of a gate), d_x, d_state, all WRITTEN (any may be NULL); sums
+ * have a fixed order.  h is recomputed from x, so h itself is not needed. */
+size_t nerf_linear_scan_carry_floats(int64_t B, int64_t T, int C, int G);
+size_t nerf_linear_scan_workspace_floats(int64_t B, int64_t T, int C, int G, int backward);
+int nerf_linear_scan_fwd(const void* gate, int gate_type, const void* x, int x_type,
+                         const float* state, int64_t B, int64_t T, int C, int G, int reverse,
+                         int blend, void* h, float* last, float* carry, float* workspace,
+                         void* stream);
+int nerf_linear_scan_bwd(const void* gate, int gate_type, const void* x, int x_type,
+                         const float* state, const float* carry, const void* d_h,
+                         const float* d_last, int64_t B, int64_t T, int C, int G, int reverse,
+                         int blend, void* d_gate, void* d_x, float* d_state, float* workspace,
+                         void* stream);
 
 /* ---------------------------------------------------------- fused MLPs ---- */
 

@@ -41,6 +41,10 @@ SIGNATURES = {
     "nerf_expand_kept": (_I, [_P, _P, _P, _L, _P, _P, _P]),
     "nerf_gather_kept": (_I, [_P, _P, _P, _L, _P, _P, _P]),
     "nerf_gather_kept_by_slot": (_I, [_P, _P, _P, _L, _P, _P, _P]),
+    "nerf_linear_scan_carry_floats": (C.c_size_t, [_L, _L, _I, _I]),
+    "nerf_linear_scan_workspace_floats": (C.c_size_t, [_L, _L, _I, _I, _I]),
+    "nerf_linear_scan_fwd": (_I, [_P, _I, _P, _I, _P, _L, _L, _I, _I, _I, _I, _P, _P, _P, _P, _P]),
+    "nerf_linear_scan_bwd": (_I, [_P, _I, _P, _I, _P, _P, _P, _P, _L, _L, _I, _I, _I, _I, _P, _P, _P, _P, _P]),
     "nerf_mlp_vanilla_pack_floats": (C.c_size_t, []),
     "nerf_mlp_vanilla_pack": (_I, [_P, _I, _P, _P]),
     "nerf_mlp_vanilla_ws_floats_per_point": (C.c_size_t, []),
@@ -129,6 +133,43 @@ def f32c(t: torch.Tensor) -> torch.Tensor:
     if t.dtype != torch.float32:
         t = t.float()
     return t.contiguous()
+
+
+# the element types of the operators that take more than float32 (NERF_F32, NERF_BF16, NERF_F16)
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def type_code(t: torch.Tensor, what: str) -> int:
+    code = TYPES.get(t.dtype)
+    if code is None:
+        raise NerfHipError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def dense(t: torch.Tensor) -> torch.Tensor:
+    """Dense view/copy that starts on a 16-byte boundary, of the tensor's own type."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def launch(name: str, t: torch.Tensor, *args) -> None:
+    """Call an entry point on the current stream of ``t``'s device, which need not be the current device."""
+    index = t.device.index
+    fn = getattr(lib(), name)
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    if rc != 0:
+        check(rc, name)
+
+
+def same_device(*tensors: torch.Tensor) -> None:
+    need_gpu(*tensors)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise NerfHipError("the tensors of one call must be on one device, got " + ", ".join(sorted(map(str, devices))))
 
 
 def ptr_array(tensors):

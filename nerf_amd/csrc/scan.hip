@@ -1,0 +1,553 @@
+// Gated linear recurrence along a sequence or a ray, and its gradient, for gfx950.
+//
+//   h_i = a_i h_{i-1} + w_i x_i,   w_i = 1, or 1 - a_i ("blend": with the samples taken last to first this is
+//   back-to-front alpha compositing of any number of channels, a_i = 1 - alpha_i).
+//
+// A stretch of steps acts on the state it is entered with as h -> A h + X (A the product of its gates), and two
+// stretches compose, (A2 A1, A2 X1 + X2).  So every thread takes K consecutive steps of VEC channels into registers and
+// forms (A, X) of them; a scan over the time slices of the group (lanes, then waves) gives each thread the state it
+// starts from; and the thread replays its steps from there -- every output comes from the recurrence itself, only the
+// states between slices from the composed form.  The state is held in float whatever the types of gate and x are.
+//
+// Gradient, with r_i what reaches h_i from the steps behind it: g_i = dh_i + r_i, r_{i-1} = a_i g_i, d x_i = w_i g_i,
+// d a_i = g_i h_{i-1} (blend: g_i (h_{i-1} - x_i)), summed over the channels that share the gate.  r is the same kind of
+// recurrence from the other end, with the same products A.  h is recomputed from x and the state the tile was entered
+// with (kept in float by the forward pass): x costs the bytes that a saved h would, and h is not rounded on the way.
+//
+// Layout: x [B,T,C], gate [B,T,G]; the C/G = P channels of a gate are neighbours.  G = C: one "unit" of C columns per
+// batch entry; G < C: one unit of P columns per (batch entry, gate).  A workgroup of 256 threads is cut into groups of
+// CL x S threads: CL lanes side by side on the columns of a unit (VEC each), S slices of K steps.  Both passes are
+// bound by memory: the forward pass moves gate + x + h once, the backward pass gate, x, dh in and d_gate, d_x out.
+#include <algorithm>
+
+#include "typed.h"
+
+namespace nerf {
+
+constexpr int SCAN_K = 8;          // steps per thread
+constexpr int SCAN_THREADS = 256;
+constexpr int SCAN_COLS = 64;      // most columns of a unit that one workgroup takes side by side
+constexpr int SCAN_WANT_BLOCKS = 1024;
+
+struct ScanShape {
+    int64_t B, T;
+    int C, G, P;            // channels, gates, channels per unit
+    int units_per_b;        // 1 (a gate per channel) or G
+    int vec, lcl, ls;       // elements per lane, log2 of CL and of S
+    int col_tiles;          // column tiles of a unit
+    int64_t unit_tiles;     // B * units_per_b * col_tiles
+    int64_t blocks;         // workgroups that hold them
+    int tile_steps;         // S * K
+    int64_t tiles;          // time tiles
+    int64_t segments, seg_tiles;   // the time axis is cut into segments of seg_tiles tiles when there are few workgroups
+};
+
+static int log2_up(int64_t n) {
+    int l = 0;
+    while ((1ll << l) < n) ++l;
+    return l;
+}
+
+// A function of the sizes alone: the backward pass finds the forward pass's tiles again.
+static ScanShape scan_shape(int64_t B, int64_t T, int C, int G) {
+    ScanShape s;
+    s.B = B; s.T = T; s.C = C; s.G = G;
+    s.units_per_b = G == C ? 1 : G;
+    s.P = C / s.units_per_b;
+    s.vec = s.P % 4 == 0 ? 4 : 1;
+    s.lcl = log2_up(std::min<int64_t>(ceil_div(s.P, s.vec), SCAN_COLS / s.vec));
+    s.ls = std::min(log2_up(ceil_div(T, SCAN_K)), 8 - s.lcl);
+    s.col_tiles = (int)ceil_div(s.P, (int64_t)s.vec << s.lcl);
+    s.unit_tiles = B * s.units_per_b * s.col_tiles;
+    const int per_block = SCAN_THREADS >> (s.lcl + s.ls);
+    s.blocks = ceil_div(s.unit_tiles, per_block);
+    s.tile_steps = SCAN_K << s.ls;
+    s.tiles = ceil_div(T, s.tile_steps);
+    // few workgroups: cut the time axis (a second pass over gate and x, or gate and dh, finds the states between segments)
+    const int64_t want = std::min<int64_t>(s.tiles, ceil_div(SCAN_WANT_BLOCKS, s.blocks));
+    s.seg_tiles = ceil_div(s.tiles, std::max<int64_t>(1, want));
+    s.segments = ceil_div(s.tiles, s.seg_tiles);
+    return s;
+}
+
+struct ScanArgs {
+    ScanShape s;
+    const void* gate;
+    const void* x;
+    const float* state;    // [B,C] or null (zeros)
+    int reverse, blend;
+    void* h;
+    float* last;           // [B,C] or null
+    float* carry;          // [tiles - 1][B,C]: the state every tile but the first is entered with; null: not kept
+    float* agg;            // [2][segments][B,C]: A and X (backward: A and R) of the segments
+    // backward
+    const void* d_h;       // null: zeros
+    const float* d_last;   // null: zeros
+    void* d_gate;
+    void* d_x;
+    float* d_state;
+    float* d_gate_part;    // [col_tiles][B,T,G] where a gate's channels take more than one column tile
+};
+
+// A h + X.  A state of exactly zero stays without effect however large the product of the gates has become.
+__device__ __forceinline__ float scan_apply(float A, float h, float X) { return h == 0.0f ? X : fmaf(A, h, X); }
+
+// Where a thread stands: its columns and its slice.
+template <int VEC>
+struct ScanPlace {
+    int CL, S, SW, NW;          // lanes on columns, slices, slices of the group in one wave, waves of the group
+    int c, sl, slw, lane, first_wave;
+    bool on;                    // has columns
+    int64_t b;
+    int j;                      // first column, in [0, C)
+    int64_t g;                  // gate of a shared unit
+    int64_t bc;                 // b * C + j
+    int col_tile;
+
+    __device__ __forceinline__ explicit ScanPlace(const ScanShape& s, int64_t block) {
+        const int tid = threadIdx.x;
+        CL = 1 << s.lcl;
+        S = 1 << s.ls;
+        SW = min(S, 64 >> s.lcl);
+        NW = S / SW;
+        lane = tid & 63;
+        c = tid & (CL - 1);
+        sl = (tid >> s.lcl) & (S - 1);
+        slw = sl & (SW - 1);
+        const int q = tid >> (s.lcl + s.ls);
+        first_wave = NW > 1 ? (tid >> 6) & ~(NW - 1) : 0;
+        const int64_t ut = block * (SCAN_THREADS >> (s.lcl + s.ls)) + q;
+        const int64_t u = ut / s.col_tiles;
+        col_tile = (int)(ut - u * s.col_tiles);
+        b = u / s.units_per_b;
+        g = u - b * s.units_per_b;
+        const int in_unit = (col_tile * CL + c) * VEC;
+        on = ut < s.unit_tiles && in_unit < s.P;
+        j = (int)g * s.P + in_unit;
+        bc = b * s.C + j;
+    }
+    // place of step i (in the order of the recurrence) of this thread's columns in a [B,T,C] array / of its gate
+    __device__ __forceinline__ int64_t at(const ScanShape& s, int64_t i, int reverse) const {
+        return (b * s.T + (reverse ? s.T - 1 - i : i)) * s.C + j;
+    }
+    __device__ __forceinline__ int64_t gate_at(const ScanShape& s, int64_t i, int reverse) const {
+        return (b * s.T + (reverse ? s.T - 1 - i : i)) * s.G + g;
+    }
+};
+
+// K steps of the thread's columns; steps behind the end and columns that do not exist read `fill`.
+template <int VEC, class T>
+__device__ __forceinline__ void scan_load(const ScanArgs& p, const ScanPlace<VEC>& w, const void* base, int64_t i0, float fill,
+                                          float (&out)[SCAN_K][VEC]) {
+    const T* __restrict__ src = static_cast<const T*>(base);
+#pragma unroll
+    for (int k = 0; k < SCAN_K; ++k) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) out[k][v] = fill;
+        if (w.on && i0 + k < p.s.T) load_run<VEC>(src + w.at(p.s, i0 + k, p.reverse), out[k]);
+    }
+}
+template <int VEC, int GV, class T>
+__device__ __forceinline__ void scan_load_gate(const ScanArgs& p, const ScanPlace<VEC>& w, int64_t i0, float (&a)[SCAN_K][GV]) {
+    if constexpr (GV == VEC && GV > 1) {
+        scan_load<VEC, T>(p, w, p.gate, i0, 1.0f, a);
+    } else {
+        const T* __restrict__ src = static_cast<const T*>(p.gate);
+#pragma unroll
+        for (int k = 0; k < SCAN_K; ++k) {
+            a[k][0] = 1.0f;
+            // one gate for the unit, or (G = C, VEC = 1) the column's own
+            if (w.on && i0 + k < p.s.T) a[k][0] = (float)src[p.s.units_per_b == 1 && p.s.G == p.s.C ? w.at(p.s, i0 + k, p.reverse) : w.gate_at(p.s, i0 + k, p.reverse)];
+        }
+    }
+}
+
+// Inclusive scan of (A, X) over the slices that the wave holds of the group; UP: from the first slice, else from the last.
+template <int VEC, bool UP>
+__device__ __forceinline__ void scan_wave(const ScanPlace<VEC>& w, float (&A)[VEC], float (&X)[VEC]) {
+    for (int d = 1; d < w.SW; d <<= 1) {
+        const bool take = UP ? w.slw >= d : w.slw + d < w.SW;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            const float pa = UP ? __shfl_up(A[v], d * w.CL, 64) : __shfl_down(A[v], d * w.CL, 64);
+            const float px = UP ? __shfl_up(X[v], d * w.CL, 64) : __shfl_down(X[v], d * w.CL, 64);
+            if (take) {
+                X[v] = scan_apply(A[v], px, X[v]);
+                A[v] *= pa;
+            }
+        }
+    }
+}
+
+// From the inclusive wave scan (A, X) and the state `carry` that the tile is entered with (the same in all slices of a
+// column): `in` = the state this slice is entered with, `carry` = the state the tile is left with.
+// s_a, s_x: [waves][SCAN_COLS] of this exchange's own, written here and read behind one barrier.
+template <int VEC, bool UP>
+__device__ __forceinline__ void scan_carry(const ScanPlace<VEC>& w, const float (&A)[VEC], const float (&X)[VEC], float (&carry)[VEC], float (&in)[VEC],
+                                           float (*s_a)[SCAN_COLS], float (*s_x)[SCAN_COLS]) {
+    const bool edge = UP ? w.slw == w.SW - 1 : w.slw == 0;   // its inclusive value is the wave's
+    float from[VEC];
+    if (w.NW > 1) {
+        const int wave = threadIdx.x >> 6;
+        if (edge) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                s_a[wave][w.c * VEC + v] = A[v];
+                s_x[wave][w.c * VEC + v] = X[v];
+            }
+        }
+        __syncthreads();
+        const int mine = wave - w.first_wave;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) from[v] = carry[v];
+        for (int n = 0; n < w.NW; ++n) {
+            const int k = UP ? n : w.NW - 1 - n;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                if (k == mine) from[v] = carry[v];
+                carry[v] = scan_apply(s_a[w.first_wave + k][w.c * VEC + v], carry[v], s_x[w.first_wave + k][w.c * VEC + v]);
+            }
+        }
+    } else {
+        const int last = (w.lane & ~(w.CL * w.SW - 1)) + (UP ? (w.SW - 1) * w.CL : 0) + w.c;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            from[v] = carry[v];
+            carry[v] = scan_apply(__shfl(A[v], last, 64), carry[v], __shfl(X[v], last, 64));
+        }
+    }
+    const bool first = UP ? w.slw == 0 : w.slw == w.SW - 1;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        const float pa = UP ? __shfl_up(A[v], w.CL, 64) : __shfl_down(A[v], w.CL, 64);
+        const float px = UP ? __shfl_up(X[v], w.CL, 64) : __shfl_down(X[v], w.CL, 64);
+        in[v] = first ? from[v] : scan_apply(pa, from[v], px);
+    }
+}
+
+// (A, X) of the thread's K steps; x is multiplied by its weight first if the recurrence blends.
+template <int VEC, int GV>
+__device__ __forceinline__ void scan_local(const float (&a)[SCAN_K][GV], const float (&x)[SCAN_K][VEC], int blend, float (&A)[VEC], float (&X)[VEC]) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) { A[v] = 1.0f; X[v] = 0.0f; }
+#pragma unroll
+    for (int k = 0; k < SCAN_K; ++k)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            const float ak = a[k][GV == 1 ? 0 : v];
+            X[v] = fmaf(ak, X[v], blend ? (1.0f - ak) * x[k][v] : x[k][v]);
+            A[v] *= ak;
+        }
+}
+// (A, R) of the same steps from the other end: r_{i-1} = a_i (dh_i + r_i)
+template <int VEC, int GV>
+__device__ __forceinline__ void scan_local_back(const float (&a)[SCAN_K][GV], const float (&dh)[SCAN_K][VEC], float (&A)[VEC], float (&R)[VEC]) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) { A[v] = 1.0f; R[v] = 0.0f; }
+#pragma unroll
+    for (int k = SCAN_K - 1; k >= 0; --k)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            const float ak = a[k][GV == 1 ? 0 : v];
+            R[v] = ak * (dh[k][v] + R[v]);
+            A[v] *= ak;
+        }
+}
+
+// (A, X) of whole segments -- all but the last one -- or, BACK, (A, R) of all but the first.
+template <class GT, class XT, int VEC, int GV, bool BACK>
+__global__ __launch_bounds__(SCAN_THREADS) void scan_segments_kernel(ScanArgs p) {
+    __shared__ float s_a[2][4][SCAN_COLS], s_x[2][4][SCAN_COLS];
+    const ScanShape& s = p.s;
+    const int64_t seg = blockIdx.x / s.blocks + (BACK ? 1 : 0);
+    const ScanPlace<VEC> w(s, blockIdx.x % s.blocks);
+    const int64_t t_begin = seg * s.seg_tiles, t_end = min(t_begin + s.seg_tiles, s.tiles);
+    float A_all[VEC], X_all[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) { A_all[v] = 1.0f; X_all[v] = 0.0f; }
+    for (int64_t n = 0; n < t_end - t_begin; ++n) {
+        const int64_t tile = BACK ? t_end - 1 - n : t_begin + n;
+        const int64_t i0 = tile * s.tile_steps + w.sl * SCAN_K;
+        float a[SCAN_K][GV], x[SCAN_K][VEC], A[VEC], X[VEC], in[VEC];
+        scan_load_gate<VEC, GV, GT>(p, w, i0, a);
+        if (BACK && !p.d_h) {
+#pragma unroll
+            for (int k = 0; k < SCAN_K; ++k)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) x[k][v] = 0.0f;
+        } else {
+            scan_load<VEC, XT>(p, w, BACK ? p.d_h : p.x, i0, 0.0f, x);
+        }
+        if (BACK) scan_local_back<VEC, GV>(a, x, A, X);
+        else scan_local<VEC, GV>(a, x, p.blend, A, X);
+        scan_wave<VEC, !BACK>(w, A, X);
+        float prod[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) prod[v] = A_all[v];
+        scan_carry<VEC, !BACK>(w, A, X, X_all, in, s_a[n & 1], s_x[n & 1]);
+        if (w.NW > 1) {
+            for (int k = 0; k < w.NW; ++k)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) prod[v] *= s_a[n & 1][w.first_wave + k][w.c * VEC + v];
+        } else {
+            const int last = (w.lane & ~(w.CL * w.SW - 1)) + (BACK ? 0 : (w.SW - 1) * w.CL) + w.c;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) prod[v] *= __shfl(A[v], last, 64);
+        }
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) A_all[v] = prod[v];
+    }
+    if (w.on && w.sl == 0) {
+        const int64_t BC = s.B * s.C;
+        store_run<VEC>(p.agg + seg * BC + w.bc, A_all);
+        store_run<VEC>(p.agg + (s.segments + seg) * BC + w.bc, X_all);
+    }
+}
+
+template <class GT, class XT, int VEC, int GV>
+__global__ __launch_bounds__(SCAN_THREADS) void scan_fwd_kernel(ScanArgs p) {
+    __shared__ float s_a[2][4][SCAN_COLS], s_x[2][4][SCAN_COLS];
+    const ScanShape& s = p.s;
+    const int64_t seg = blockIdx.x / s.blocks, BC = s.B * s.C;
+    const ScanPlace<VEC> w(s, blockIdx.x % s.blocks);
+    const int64_t t_begin = seg * s.seg_tiles, t_end = min(t_begin + s.seg_tiles, s.tiles);
+    float carry[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) carry[v] = 0.0f;
+    if (w.on) {
+        if (p.state) load_run<VEC>(p.state + w.bc, carry);
+        for (int64_t k = 0; k < seg; ++k) {
+            float A[VEC], X[VEC];
+            load_run<VEC>(p.agg + k * BC + w.bc, A);
+            load_run<VEC>(p.agg + (s.segments + k) * BC + w.bc, X);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) carry[v] = scan_apply(A[v], carry[v], X[v]);
+        }
+    }
+    XT* __restrict__ h_out = static_cast<XT*>(p.h);
+    for (int64_t tile = t_begin; tile < t_end; ++tile) {
+        const int64_t i0 = tile * s.tile_steps + w.sl * SCAN_K;
+        if (p.carry && tile > 0 && w.on && w.sl == 0) store_run<VEC>(p.carry + (tile - 1) * BC + w.bc, carry);
+        float a[SCAN_K][GV], x[SCAN_K][VEC], A[VEC], X[VEC], h[VEC];
+        scan_load_gate<VEC, GV, GT>(p, w, i0, a);
+        scan_load<VEC, XT>(p, w, p.x, i0, 0.0f, x);
+        scan_local<VEC, GV>(a, x, p.blend, A, X);
+        scan_wave<VEC, true>(w, A, X);
+        scan_carry<VEC, true>(w, A, X, carry, h, s_a[tile & 1], s_x[tile & 1]);
+#pragma unroll
+        for (int k = 0; k < SCAN_K; ++k) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const float ak = a[k][GV == 1 ? 0 : v];
+                h[v] = fmaf(ak, h[v], p.blend ? (1.0f - ak) * x[k][v] : x[k][v]);
+            }
+            if (w.on && i0 + k < s.T) store_run<VEC>(h_out + w.at(s, i0 + k, p.reverse), h);
+        }
+    }
+    if (p.last && t_end == s.tiles && w.on && w.sl == 0) store_run<VEC>(p.last + w.bc, carry);
+}
+
+template <class GT, class XT, int VEC, int GV>
+__global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
+    __shared__ float s_a[2][4][SCAN_COLS], s_x[2][4][SCAN_COLS], s_b[2][4][SCAN_COLS], s_r[2][4][SCAN_COLS];
+    const ScanShape& s = p.s;
+    const int64_t seg = blockIdx.x / s.blocks, BC = s.B * s.C;
+    const ScanPlace<VEC> w(s, blockIdx.x % s.blocks);
+    const int64_t t_begin = seg * s.seg_tiles, t_end = min(t_begin + s.seg_tiles, s.tiles);
+    const bool shared_gate = s.G != s.C;
+    float r_carry[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) r_carry[v] = 0.0f;
+    if (w.on) {
+        if (p.d_last) load_run<VEC>(p.d_last + w.bc, r_carry);
+        for (int64_t k = s.segments - 1; k > seg; --k) {
+            float A[VEC], R[VEC];
+            load_run<VEC>(p.agg + k * BC + w.bc, A);
+            load_run<VEC>(p.agg + (s.segments + k) * BC + w.bc, R);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) r_carry[v] = scan_apply(A[v], r_carry[v], R[v]);
+        }
+    }
+    XT* __restrict__ dx_out = static_cast<XT*>(p.d_x);
+    GT* __restrict__ da_out = static_cast<GT*>(p.d_gate);
+    for (int64_t tile = t_end - 1; tile >= t_begin; --tile) {
+        const int64_t i0 = tile * s.tile_steps + w.sl * SCAN_K;
+        float a[SCAN_K][GV], x[SCAN_K][VEC], dh[SCAN_K][VEC], A[VEC], X[VEC], h[VEC], r[VEC], carry[VEC];
+        scan_load_gate<VEC, GV, GT>(p, w, i0, a);
+        scan_load<VEC, XT>(p, w, p.x, i0, 0.0f, x);
+        if (p.d_h) {
+            scan_load<VEC, XT>(p, w, p.d_h, i0, 0.0f, dh);
+        } else {
+#pragma unroll
+            for (int k = 0; k < SCAN_K; ++k)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) dh[k][v] = 0.0f;
+        }
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) carry[v] = 0.0f;
+        if (w.on) {
+            if (tile > 0) load_run<VEC>(p.carry + (tile - 1) * BC + w.bc, carry);
+            else if (p.state) load_run<VEC>(p.state + w.bc, carry);
+        }
+        scan_local<VEC, GV>(a, x, p.blend, A, X);
+        scan_wave<VEC, true>(w, A, X);
+        scan_carry<VEC, true>(w, A, X, carry, h, s_a[tile & 1], s_x[tile & 1]);
+        scan_local_back<VEC, GV>(a, dh, A, X);
+        scan_wave<VEC, false>(w, A, X);
+        scan_carry<VEC, false>(w, A, X, r_carry, r, s_b[tile & 1], s_r[tile & 1]);
+        // x becomes what multiplies g in the gradient of the gate
+#pragma unroll
+        for (int k = 0; k < SCAN_K; ++k)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const float ak = a[k][GV == 1 ? 0 : v], xk = x[k][v];
+                x[k][v] = p.blend ? h[v] - xk : h[v];
+                h[v] = fmaf(ak, h[v], p.blend ? (1.0f - ak) * xk : xk);
+            }
+#pragma unroll
+        for (int k = SCAN_K - 1; k >= 0; --k) {
+            float da[VEC], dx[VEC];
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const float ak = a[k][GV == 1 ? 0 : v], g = dh[k][v] + r[v];
+                da[v] = g * x[k][v];
+                dx[v] = p.blend ? (1.0f - ak) * g : g;
+                r[v] = ak * g;
+            }
+            const bool here = w.on && i0 + k < s.T;
+            if (here && dx_out) store_run<VEC>(dx_out + w.at(s, i0 + k, p.reverse), dx);
+            if (!da_out) continue;
+            if (!shared_gate) {
+                if (here) store_run<VEC>(da_out + w.at(s, i0 + k, p.reverse), da);
+            } else {
+                float sum = da[0];
+#pragma unroll
+                for (int v = 1; v < VEC; ++v) sum += da[v];
+                if (!here) sum = 0.0f;
+                for (int d = 1; d < w.CL; d <<= 1) sum += __shfl_xor(sum, d, 64);
+                if (here && w.c == 0) {
+                    const int64_t at = w.gate_at(s, i0 + k, p.reverse);
+                    if (s.col_tiles == 1) da_out[at] = (GT)sum;
+                    else p.d_gate_part[(int64_t)w.col_tile * s.B * s.T * s.G + at] = sum;
+                }
+            }
+        }
+    }
+    if (p.d_state && seg == 0 && w.on && w.sl == 0) store_run<VEC>(p.d_state + w.bc, r_carry);
+}
+
+// d_gate = the sum over the column tiles, in their order
+template <class GT>
+__global__ __launch_bounds__(256) void scan_gate_sum_kernel(const float* __restrict__ part, int col_tiles, int64_t n, GT* __restrict__ out) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    float sum = 0.0f;
+    for (int k = 0; k < col_tiles; ++k) sum += part[(int64_t)k * n + i];
+    out[i] = (GT)sum;
+}
+
+enum { SCAN_FWD, SCAN_BWD };
+
+template <class GT, class XT, int VEC, int GV>
+static int scan_launch(const ScanArgs& p, int dir, const char* who, hipStream_t stream) {
+    const ScanShape& s = p.s;
+    if (s.segments > 1) {
+        const dim3 grid((unsigned)(s.blocks * (s.segments - 1)));
+        if (dir == SCAN_FWD) hipLaunchKernelGGL((scan_segments_kernel<GT, XT, VEC, GV, false>), grid, dim3(SCAN_THREADS), 0, stream, p);
+        else hipLaunchKernelGGL((scan_segments_kernel<GT, XT, VEC, GV, true>), grid, dim3(SCAN_THREADS), 0, stream, p);
+        if (int rc = check_launch(who)) return rc;
+    }
+    const dim3 grid((unsigned)(s.blocks * s.segments));
+    if (dir == SCAN_FWD) hipLaunchKernelGGL((scan_fwd_kernel<GT, XT, VEC, GV>), grid, dim3(SCAN_THREADS), 0, stream, p);
+    else hipLaunchKernelGGL((scan_bwd_kernel<GT, XT, VEC, GV>), grid, dim3(SCAN_THREADS), 0, stream, p);
+    if (int rc = check_launch(who)) return rc;
+    if (dir == SCAN_BWD && p.d_gate && s.G != s.C && s.col_tiles > 1) {
+        const int64_t n = s.B * s.T * s.G;
+        hipLaunchKernelGGL((scan_gate_sum_kernel<GT>), dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, stream, p.d_gate_part, s.col_tiles, n,
+                           static_cast<GT*>(p.d_gate));
+        return check_launch(who);
+    }
+    return NERF_OK;
+}
+
+template <class GT, class XT>
+static int scan_run_typed(const ScanArgs& p, int dir, const char* who, hipStream_t stream) {
+    if (p.s.vec == 1) return scan_launch<GT, XT, 1, 1>(p, dir, who, stream);
+    return p.s.G == p.s.C ? scan_launch<GT, XT, 4, 4>(p, dir, who, stream) : scan_launch<GT, XT, 4, 1>(p, dir, who, stream);
+}
+
+static int scan_run(const ScanArgs& p, int gate_type, int x_type, int dir, const char* who, hipStream_t stream) {
+    return with_type(x_type, [&](auto xt) {
+        using XT = decltype(xt);
+        return gate_type == NERF_F32 ? scan_run_typed<float, XT>(p, dir, who, stream) : scan_run_typed<XT, XT>(p, dir, who, stream);
+    });
+}
+
+static int scan_check(const char* who, int64_t B, int64_t T, int C, int G, int gate_type, int x_type) {
+    NERF_REQUIRE(B >= 0 && T >= 0 && C >= 0 && G >= 0, "%s: B=%lld T=%lld C=%d G=%d", who, (long long)B, (long long)T, C, G);
+    NERF_REQUIRE(C == 0 || (G > 0 && C % G == 0), "%s: %d gates do not divide %d channels", who, G, C);
+    NERF_REQUIRE(known_type(x_type) && (gate_type == NERF_F32 || gate_type == x_type), "%s: gate type %d with x type %d", who, gate_type, x_type);
+    if (B == 0 || T == 0 || C == 0) return NERF_OK;
+    NERF_REQUIRE(B <= (1ll << 40) && T <= (1ll << 40) && B * (double)T * C < 9e17, "%s: too large", who);
+    const ScanShape s = scan_shape(B, T, C, G);
+    NERF_REQUIRE(s.blocks * s.segments < (1ll << 31) && ceil_div(B * T * (double)G, 256) < (double)(1ll << 31), "%s: too many workgroups", who);
+    return NERF_OK;
+}
+
+}  // namespace nerf
+
+using namespace nerf;
+
+extern "C" size_t nerf_linear_scan_carry_floats(int64_t B, int64_t T, int C, int G) {
+    if (B <= 0 || T <= 0 || C <= 0 || G <= 0 || C % G) return 0;
+    return (size_t)((scan_shape(B, T, C, G).tiles - 1) * B * C);
+}
+
+extern "C" size_t nerf_linear_scan_workspace_floats(int64_t B, int64_t T, int C, int G, int backward) {
+    if (B <= 0 || T <= 0 || C <= 0 || G <= 0 || C % G) return 0;
+    const ScanShape s = scan_shape(B, T, C, G);
+    size_t n = s.segments > 1 ? (size_t)(2 * s.segments * B * C) : 0;
+    if (backward && G != C && s.col_tiles > 1) n += (size_t)s.col_tiles * (size_t)(B * T * G);
+    return n;
+}
+
+extern "C" int nerf_linear_scan_fwd(const void* gate, int gate_type, const void* x, int x_type, const float* state, int64_t B,
+                                    int64_t T, int C, int G, int reverse, int blend, void* h, float* last, float* carry,
+                                    float* workspace, void* stream) {
+    const char* who = "nerf_linear_scan_fwd";
+    if (int rc = scan_check(who, B, T, C, G, gate_type, x_type)) return rc;
+    if (B == 0 || C == 0) return NERF_OK;
+    NERF_REQUIRE(T > 0, "%s: a sequence of no steps", who);
+    NERF_REQUIRE(gate && x && h, "%s: null pointer", who);
+    NERF_REQUIRE(aligned16(gate) && aligned16(x) && aligned16(state) && aligned16(h) && aligned16(last) && aligned16(carry) && aligned16(workspace),
+                 "%s: pointers must be 16-byte aligned", who);
+    ScanArgs p{};
+    p.s = scan_shape(B, T, C, G);
+    NERF_REQUIRE(workspace || nerf_linear_scan_workspace_floats(B, T, C, G, 0) == 0, "%s: null workspace", who);
+    p.gate = gate; p.x = x; p.state = state; p.reverse = reverse != 0; p.blend = blend != 0;
+    p.h = h; p.last = last; p.carry = carry; p.agg = workspace;
+    return scan_run(p, gate_type, x_type, SCAN_FWD, who, (hipStream_t)stream);
+}
+
+extern "C" int nerf_linear_scan_bwd(const void* gate, int gate_type, const void* x, int x_type, const float* state, const float* carry,
+                                    const void* d_h, const float* d_last, int64_t B, int64_t T, int C, int G, int reverse, int blend,
+                                    void* d_gate, void* d_x, float* d_state, float* workspace, void* stream) {
+    const char* who = "nerf_linear_scan_bwd";
+    if (int rc = scan_check(who, B, T, C, G, gate_type, x_type)) return rc;
+    if (B == 0 || C == 0) return NERF_OK;
+    NERF_REQUIRE(T > 0, "%s: a sequence of no steps", who);
+    NERF_REQUIRE(gate && x, "%s: null pointer", who);
+    NERF_REQUIRE(aligned16(gate) && aligned16(x) && aligned16(state) && aligned16(carry) && aligned16(d_h) && aligned16(d_last) && aligned16(d_gate) &&
+                     aligned16(d_x) && aligned16(d_state) && aligned16(workspace),
+                 "%s: pointers must be 16-byte aligned", who);
+    ScanArgs p{};
+    p.s = scan_shape(B, T, C, G);
+    NERF_REQUIRE(carry || p.s.tiles == 1, "%s: null carry (the forward pass keeps it)", who);
+    NERF_REQUIRE(workspace || nerf_linear_scan_workspace_floats(B, T, C, G, 1) == 0, "%s: null workspace", who);
+    p.gate = gate; p.x = x; p.state = state; p.reverse = reverse != 0; p.blend = blend != 0;
+    p.carry = const_cast<float*>(carry);
+    p.d_h = d_h; p.d_last = d_last; p.d_gate = d_gate; p.d_x = d_x; p.d_state = d_state;
+    p.agg = workspace;
+    p.d_gate_part = workspace ? workspace + (p.s.segments > 1 ? 2 * p.s.segments * B * C : 0) : nullptr;
+    return scan_run(p, gate_type, x_type, SCAN_BWD, who, (hipStream_t)stream);
+}

@@ -8,6 +8,7 @@ from __future__ import annotations
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 
@@ -396,6 +397,98 @@ def render_loss(rgb, target, rgb_fine=None, weights=None, reg: float = 0.0) -> t
     plus ``mse_loss(rgb_fine, target)`` for a hierarchical render, plus ``reg * (1 - weights.sum(-1)).abs().mean()``
     (the hash-grid loop's regulariser, src/train_nerf_ngp.py:221-222, reg = 0.05).  The target receives no gradient."""
     return _RenderLoss.apply(rgb, target, rgb_fine, weights if reg != 0.0 else None, float(reg))
+
+
+# ---------------------------------------------------- linear recurrence ----
+def _scan_fwd(gate, x, state, reverse, blend, want_last, keep):
+    """Dense [B,T,G], [B,T,C], [B,C] | None -> h, last | None, carry | None (what the backward pass needs)."""
+    lib = L.lib()
+    B, T, C = x.shape
+    G = gate.shape[2]
+    h = torch.empty_like(x)
+    last = torch.empty(B, C, device=x.device) if want_last else None
+    n = lib.nerf_linear_scan_carry_floats(B, T, C, G) if keep else 0
+    carry = torch.empty(n, device=x.device) if n else None
+    n = lib.nerf_linear_scan_workspace_floats(B, T, C, G, 0)
+    work = torch.empty(n, device=x.device) if n else None
+    L.launch("nerf_linear_scan_fwd", x, L.ptr(gate), L.TYPES[gate.dtype], L.ptr(x), L.TYPES[x.dtype], L.ptr(state), B, T, C, G,
+             reverse, blend, L.ptr(h), L.ptr(last), L.ptr(carry), L.ptr(work))
+    return h, last, carry
+
+
+class _LinearScan(torch.autograd.Function):
+    """(gate [B,T,G], x [B,T,C], state [B,C] | None) -> (h [B,T,C], last [B,C] | None)."""
+
+    @staticmethod
+    def forward(ctx, gate, x, state, reverse, blend, want_last):
+        gate, x, state = (None if t is None else L.dense(t.detach()) for t in (gate, x, state))
+        h, last, carry = _scan_fwd(gate, x, state, reverse, blend, want_last, True)
+        ctx.save_for_backward(gate, x, state, carry)
+        ctx.meta = (reverse, blend)
+        ctx.set_materialize_grads(False)
+        return h, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_h, d_last):
+        gate, x, state, carry = ctx.saved_tensors
+        B, T, C = x.shape
+        G = gate.shape[2]
+        need_gate, need_x, need_state = ctx.needs_input_grad[:3]
+        d_h, d_last = (None if t is None else L.dense(t) for t in (d_h, d_last))
+        d_gate = torch.empty_like(gate) if need_gate else None
+        d_x = torch.empty_like(x) if need_x else None
+        d_state = torch.empty_like(state) if need_state else None
+        n = L.lib().nerf_linear_scan_workspace_floats(B, T, C, G, 1)
+        work = torch.empty(n, device=x.device) if n else None
+        L.launch("nerf_linear_scan_bwd", x, L.ptr(gate), L.TYPES[gate.dtype], L.ptr(x), L.TYPES[x.dtype], L.ptr(state), L.ptr(carry),
+                 L.ptr(d_h), L.ptr(d_last), B, T, C, G, *ctx.meta, L.ptr(d_gate), L.ptr(d_x), L.ptr(d_state), L.ptr(work))
+        return d_gate, d_x, d_state, None, None, None
+
+
+def linear_scan(gate: torch.Tensor, x: torch.Tensor, state: Optional[torch.Tensor] = None, reverse: bool = False, blend: bool = False,
+                return_state: bool = False):
+    """Gated linear recurrence over the second to last axis, ``h_t = a_t h_{t-1} + x_t``, or with ``blend``
+    ``h_t = a_t h_{t-1} + (1 - a_t) x_t`` -- with ``reverse`` (last step first) that is back-to-front alpha compositing of
+    any number of channels: ``linear_scan(1 - alpha, features, reverse=True, blend=True)[..., 0, :]``.
+
+    ``x`` [..., T, C]; ``gate`` [..., T, G] with G dividing C, channel c taking gate ``c // (C / G)``: G = C a gate per
+    channel, G = 1 one per step, anything between heads.  ``state`` [..., C]: h before the first step (zeros if None).
+    float32, bfloat16 or float16; a gate of another type than ``x`` is taken as float32.  The state is held in float32
+    and h rounded once to the type of ``x``.  A gate of zero starts a new sequence.  Gates are meant to lie in [-1, 1];
+    larger ones are right while float32 holds their products.
+    ``return_state``: ``(h, last)``, ``last`` [..., C] float32 the state after the last step, unrounded: what the next call
+    takes as ``state`` (a long sequence in parts, or one step at a time with T = 1).
+    Differentiable once in ``gate``, ``x`` and ``state``."""
+    L.require(x.dim() >= 2, f"x must be [..., T, C], got {tuple(x.shape)}")
+    lead, T, C = x.shape[:-2], x.shape[-2], x.shape[-1]
+    L.require(gate.dim() == x.dim() and gate.shape[:-1] == x.shape[:-1], f"gate must be {[*x.shape[:-1]]} + [G], got {tuple(gate.shape)}")
+    G = gate.shape[-1]
+    L.require(C == 0 or (G > 0 and C % G == 0), f"{G} gates do not divide {C} channels")
+    L.require(gate.is_floating_point(), f"gate must be floating point, got {gate.dtype}")
+    if gate.dtype != x.dtype and gate.dtype != torch.float32:
+        gate = gate.float()
+    if state is not None:
+        L.require(tuple(state.shape) == (*lead, C), f"state must be {[*lead, C]}, got {tuple(state.shape)}")
+        L.require(state.is_floating_point(), f"state must be floating point, got {state.dtype}")
+        state = state.float()
+    L.type_code(x, "x")
+    L.same_device(gate, x, state)
+    if T == 0:
+        h = x.clone()
+        if not return_state:
+            return h
+        return h, (state.clone() if state is not None else torch.zeros(*lead, C, device=x.device))
+    B = lead.numel()
+    gate3, x3 = gate.reshape(B, T, G), x.reshape(B, T, C)
+    state2 = state.reshape(B, C) if state is not None else None
+    if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or (state is not None and state.requires_grad)):
+        h, last = _LinearScan.apply(gate3, x3, state2, bool(reverse), bool(blend), bool(return_state))
+    else:
+        h, last, _ = _scan_fwd(L.dense(gate3.detach()), L.dense(x3.detach()), None if state is None else L.dense(state2.detach()), bool(reverse),
+                               bool(blend), bool(return_state), False)
+    h = h.view(x.shape)
+    return (h, last.view(*lead, C)) if return_state else h
 
 
 # ---------------------------------------------------------- fused MLPs ----
