@@ -126,6 +126,23 @@ int nerf_hashgrid_bwd(const float* x, int64_t P, const float* d_out, const int* 
                       const int* sizes, int levels, float* const* d_tables, void* workspace,
                       size_t workspace_bytes, void* stream);
 
+/* Rows of a learned table by integer id: out[n] = scale * table[ids[n]] (one code per image of the
+ * batch, a codebook, token embeddings; the reference's only tables are the hash grid's nn.Embedding,
+ * src/utils/hash_grid_encoder.py:31-37).  table [V,D] and out [N,D] of `type` (NERF_F32 / BF16 / F16),
+ * ids [N] of ids_bytes = 4 or 8 (int32, int64).  An id outside [0,V) reads nothing and yields a NaN row.
+ * bwd: d_table [V,D] of `type` is WRITTEN, untouched rows with zeros:
+ *   d_table[v] = scale * sum of d_out[n] over the n with ids[n] = v,
+ * ids outside [0,V) and padding_idx (-1: none) taking no gradient.  Sums are formed in float32 in an
+ * order that the ids alone decide, without atomics, and rounded once.  workspace:
+ * nerf_embedding_bwd_workspace_bytes(N,V,D) bytes, contents irrelevant.  V and N below 2^31 - 1; table,
+ * out, d_out, d_table and workspace 16-byte aligned. */
+int nerf_embedding_fwd(const void* table, int type, int64_t V, int D, const void* ids,
+                       int ids_bytes, int64_t N, float scale, void* out, void* stream);
+size_t nerf_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int D);
+int nerf_embedding_bwd(const void* d_out, int type, const void* ids, int ids_bytes, int64_t N,
+                       int64_t V, int D, float scale, int64_t padding_idx, void* d_table,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
 /* ----------------------------------------------------------- composite ---- */
 
 /* Camera.volume_render, src/Camera.py:143-183.  rgb [R,N,3], sigma [R,N],

@@ -33,6 +33,9 @@ SIGNATURES = {
     "nerf_hashgrid_fwd": (_I, [_P, _L, _P, _P, _P, _I, _P, _P, _P, _P]),
     "nerf_hashgrid_bwd_workspace_bytes": (C.c_size_t, [_L, _P, _I]),
     "nerf_hashgrid_bwd": (_I, [_P, _L, _P, _P, _P, _I, _P, _P, C.c_size_t, _P]),
+    "nerf_embedding_fwd": (_I, [_P, _I, _L, _I, _P, _I, _L, _F, _P, _P]),
+    "nerf_embedding_bwd_workspace_bytes": (C.c_size_t, [_L, _L, _I]),
+    "nerf_embedding_bwd": (_I, [_P, _I, _P, _I, _L, _L, _I, _F, _L, _P, _P, C.c_size_t, _P]),
     "nerf_composite_fwd": (_I, [_P, _P, _P, _L, _I, _I, _F, _P, _P, _P, _P]),
     "nerf_composite_bwd": (_I, [_P, _P, _P, _P, _P, _P, _L, _I, _I, _F, _P, _P, _P]),
     "nerf_occupancy_mask": (_I, [_P, _P, _L, _P, _L, _I, _P, _P]),

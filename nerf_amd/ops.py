@@ -192,6 +192,64 @@ def hashgrid_debug(x: torch.Tensor, tables: Sequence[torch.Tensor], res: Sequenc
     return out, idx, w
 
 
+# ----------------------------------------------------------- embedding ----
+def _embedding_fwd(ids, table, scale):
+    V, D = table.shape
+    out = torch.empty(*ids.shape, D, device=table.device, dtype=table.dtype)
+    L.launch("nerf_embedding_fwd", table, L.ptr(table), L.TYPES[table.dtype], V, D, L.ptr(ids), ids.element_size(), ids.numel(), scale, L.ptr(out))
+    return out
+
+
+class _Embedding(torch.autograd.Function):
+    """(table [V,D], ids [...]) -> [..., D]."""
+
+    @staticmethod
+    def forward(ctx, table, ids, scale, padding_idx):
+        out = _embedding_fwd(ids, L.dense(table.detach()), scale)
+        ctx.save_for_backward(ids)
+        ctx.meta = (tuple(table.shape), scale, padding_idx)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out):
+        (ids,) = ctx.saved_tensors
+        (V, D), scale, padding_idx = ctx.meta
+        d_out = L.dense(d_out)
+        N = ids.numel()
+        nbytes = L.lib().nerf_embedding_bwd_workspace_bytes(N, V, D)
+        work = torch.empty(nbytes, device=d_out.device, dtype=torch.uint8) if nbytes else None
+        d_table = torch.empty(V, D, device=d_out.device, dtype=d_out.dtype)
+        L.launch("nerf_embedding_bwd", d_out, L.ptr(d_out), L.TYPES[d_out.dtype], L.ptr(ids), ids.element_size(), N, V, D, scale, padding_idx,
+                 L.ptr(d_table), L.ptr(work), nbytes)
+        return d_table, None, None, None
+
+
+def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
+    """``scale * table[ids]``: ids [...] of any integer type, table [V, D] in float32, bfloat16 or float16 -> [..., D].
+
+    An id outside [0, V) gives a row of NaN and takes no gradient.  ``padding_idx``: that row of the table takes no
+    gradient (negative: counted from the end), as in ``torch.nn.functional.embedding``.  The gradient of the table is
+    dense, formed by sorting the ids -- the same bits for the same inputs, whatever ids repeat -- and summed in float32.
+    Differentiable once in ``table``."""
+    L.require(table.dim() == 2, f"table must be [V, D], got {tuple(table.shape)}")
+    L.require(not ids.is_floating_point() and not ids.is_complex() and ids.dtype != torch.bool, f"ids must be integers, got {ids.dtype}")
+    V = table.shape[0]
+    if padding_idx is None:
+        padding_idx = -1
+    else:
+        L.require(-V <= padding_idx < V, f"padding_idx {padding_idx} is outside the {V} rows")
+        padding_idx = int(padding_idx) % V
+    L.type_code(table, "table")
+    L.same_device(ids, table)
+    if ids.dtype not in (torch.int64, torch.int32):
+        ids = ids.long()
+    ids = ids.contiguous()
+    if torch.is_grad_enabled() and table.requires_grad:
+        return _Embedding.apply(table, ids, float(scale), padding_idx)
+    return _embedding_fwd(ids, L.dense(table.detach()), float(scale))
+
+
 # ----------------------------------------------------------- composite ----
 class _Composite(torch.autograd.Function):
     """(rgb [R,N,3], sigma [R,N], z [R,N]) -> (colour [R,3], weights [R,N], depth [R])."""
