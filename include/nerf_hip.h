@@ -395,6 +395,22 @@ size_t nerf_clip_grad_norm_workspace_floats(int count, const int64_t* numel);
 int nerf_clip_grad_norm(int count, float* const* grads, const int64_t* numel, float max_norm,
                         float* workspace, float* total_norm, void* stream);
 
+/* Clipping inside the optimiser's own pass: nerf_grad_norm leaves total = the 2-norm of all gradients
+ * together in norm_coef[0] and min(1, max_norm / (total + 1e-6)) in norm_coef[1] (2 device floats), the
+ * gradients untouched; squares and sums are double, so only a total beyond float32 is infinite.
+ * workspace: nerf_grad_norm_workspace_doubles(count, numel) doubles (0: may be NULL).
+ * nerf_adam_step_scaled is nerf_adam_step (step_state NULL) or nerf_adam_step_capturable (step_state
+ * given; step and lr are then ignored) on *grad_scale times the gradients, grad_scale one device float,
+ * e.g. norm_coef + 1; weight decay is added behind the scaling, as after clip_grad_norm_.  The betas are
+ * doubles: 1 - beta is formed from the value the caller has, not from its float32 rounding. */
+size_t nerf_grad_norm_workspace_doubles(int count, const int64_t* numel);
+int nerf_grad_norm(int count, const float* const* grads, const int64_t* numel, float max_norm,
+                   double* workspace, float* norm_coef, void* stream);
+int nerf_adam_step_scaled(int count, float* const* params, const float* const* grads,
+                          float* const* exp_avg, float* const* exp_avg_sq, const int64_t* numel,
+                          int64_t step, float* step_state, float lr, double beta1, double beta2,
+                          float eps, float weight_decay, const float* grad_scale, void* stream);
+
 /* nerf_clip_grad_norm without the workspace argument.  No counterpart in the reference: it is for
  * callers that cannot allocate device memory (code under HIP graph capture, tight serving or
  * training loops, harnesses that forbid allocation).  The scratch is a 256 KiB array built into the

@@ -71,6 +71,9 @@ SIGNATURES = {
     "nerf_adam_set_lr": (_I, [_P, _F, _P]),
     "nerf_clip_grad_norm_workspace_floats": (C.c_size_t, [_I, _P]),
     "nerf_clip_grad_norm": (_I, [_I, _P, _P, _F, _P, _P, _P]),
+    "nerf_grad_norm_workspace_doubles": (C.c_size_t, [_I, _P]),
+    "nerf_grad_norm": (_I, [_I, _P, _P, _F, _P, _P, _P]),
+    "nerf_adam_step_scaled": (_I, [_I, _P, _P, _P, _P, _P, _L, _P, _F, C.c_double, C.c_double, _F, _F, _P, _P]),
     "nerf_clip_grad_norm_static": (_I, [_I, _P, _P, _F, _P, _P]),
     "nerf_rccl_version": (_I, []),
     "nerf_comm_unique_id": (_I, [_P]),

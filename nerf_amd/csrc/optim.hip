@@ -39,12 +39,17 @@ __device__ __forceinline__ void adam_one(float& p, float g, float& m, float& v, 
 
 // dev_scalars: null, or the step state in device memory that adam_advance_kernel has just brought up to date
 // ([1] = sqrt(bias2), [2] = -lr / bias1), used in place of the two kernel arguments.
+// SCALED: the gradient is multiplied by *grad_scale (the clipping coefficient of all gradients together) as it is read.
+template <bool SCALED>
 __global__ __launch_bounds__(256) void adam_kernel(AdamTensors t, float b1m, float b2, float b2m, float bias2_sqrt,
-                                                   float eps, float neg_step, float wd, const float* __restrict__ dev_scalars) {
+                                                   float eps, float neg_step, float wd, const float* __restrict__ dev_scalars,
+                                                   const float* __restrict__ grad_scale) {
     if (dev_scalars) {
         bias2_sqrt = dev_scalars[1];
         neg_step = dev_scalars[2];
     }
+    const float gs = SCALED ? *grad_scale : 1.0f;
+    const auto scaled = [gs](float g) { return SCALED ? g * gs : g; };
     int k = 0;
     while (k + 1 < t.count && (int)blockIdx.x >= t.first_block[k + 1]) ++k;
     const long long base = (long long)(blockIdx.x - t.first_block[k]) * ADAM_CHUNK;
@@ -68,10 +73,10 @@ __global__ __launch_bounds__(256) void adam_kernel(AdamTensors t, float b1m, flo
 #pragma unroll
         for (int j = 0; j < ROUNDS; ++j) {
             const long long i = base + (long long)(j * 256 + threadIdx.x) * 4;
-            adam_one(pp[j].x, gg[j].x, mm[j].x, vv[j].x, b1m, b2, b2m, bias2_sqrt, eps, neg_step, wd);
-            adam_one(pp[j].y, gg[j].y, mm[j].y, vv[j].y, b1m, b2, b2m, bias2_sqrt, eps, neg_step, wd);
-            adam_one(pp[j].z, gg[j].z, mm[j].z, vv[j].z, b1m, b2, b2m, bias2_sqrt, eps, neg_step, wd);
-            adam_one(pp[j].w, gg[j].w, mm[j].w, vv[j].w, b1m, b2, b2m, bias2_sqrt, eps, neg_step, wd);
+            adam_one(pp[j].x, scaled(gg[j].x), mm[j].x, vv[j].x, b1m, b2, b2m, bias2_sqrt, eps, neg_step, wd);
+            adam_one(pp[j].y, scaled(gg[j].y), mm[j].y, vv[j].y, b1m, b2, b2m, bias2_sqrt, eps, neg_step, wd);
+            adam_one(pp[j].z, scaled(gg[j].z), mm[j].z, vv[j].z, b1m, b2, b2m, bias2_sqrt, eps, neg_step, wd);
+            adam_one(pp[j].w, scaled(gg[j].w), mm[j].w, vv[j].w, b1m, b2, b2m, bias2_sqrt, eps, neg_step, wd);
             *reinterpret_cast<float4*>(p + i) = pp[j];
             *reinterpret_cast<float4*>(m + i) = mm[j];
             *reinterpret_cast<float4*>(v + i) = vv[j];
@@ -84,15 +89,15 @@ __global__ __launch_bounds__(256) void adam_kernel(AdamTensors t, float b1m, flo
             float4 pp = *reinterpret_cast<float4*>(p + i), mm = *reinterpret_cast<float4*>(m + i),
                    vv = *reinterpret_cast<float4*>(v + i);
             const float4 gg = *reinterpret_cast<const float4*>(g + i);
-            adam_one(pp.x, gg.x, mm.x, vv.x, b1m, b2, b2m, bias2_sqrt, eps, neg_step, wd);
-            adam_one(pp.y, gg.y, mm.y, vv.y, b1m, b2, b2m, bias2_sqrt, eps, neg_step, wd);
-            adam_one(pp.z, gg.z, mm.z, vv.z, b1m, b2, b2m, bias2_sqrt, eps, neg_step, wd);
-            adam_one(pp.w, gg.w, mm.w, vv.w, b1m, b2, b2m, bias2_sqrt, eps, neg_step, wd);
+            adam_one(pp.x, scaled(gg.x), mm.x, vv.x, b1m, b2, b2m, bias2_sqrt, eps, neg_step, wd);
+            adam_one(pp.y, scaled(gg.y), mm.y, vv.y, b1m, b2, b2m, bias2_sqrt, eps, neg_step, wd);
+            adam_one(pp.z, scaled(gg.z), mm.z, vv.z, b1m, b2, b2m, bias2_sqrt, eps, neg_step, wd);
+            adam_one(pp.w, scaled(gg.w), mm.w, vv.w, b1m, b2, b2m, bias2_sqrt, eps, neg_step, wd);
             *reinterpret_cast<float4*>(p + i) = pp;
             *reinterpret_cast<float4*>(m + i) = mm;
             *reinterpret_cast<float4*>(v + i) = vv;
         } else {
-            for (long long e = i; e < i + 4 && e < n; ++e) adam_one(p[e], g[e], m[e], v[e], b1m, b2, b2m, bias2_sqrt, eps, neg_step, wd);
+            for (long long e = i; e < i + 4 && e < n; ++e) adam_one(p[e], scaled(g[e]), m[e], v[e], b1m, b2, b2m, bias2_sqrt, eps, neg_step, wd);
         }
     }
 }
@@ -102,7 +107,8 @@ __global__ __launch_bounds__(256) void adam_kernel(AdamTensors t, float b1m, flo
 // src/train_nerf.py:87,204, src/train_nerf_ngp.py:57-62,373-379): state[0] holds the count and state[3] the rate in
 // device memory.  One thread advances the count and derives the two step-dependent scalars the way the host does
 // for nerf_adam_step (in double, rounded to float).
-__global__ void adam_advance_kernel(float* __restrict__ state, float beta1, float beta2) {
+template <class R>
+__global__ void adam_advance_kernel(float* __restrict__ state, R beta1, R beta2) {
     if (threadIdx.x != 0 || blockIdx.x != 0) return;
     const double step = (double)state[0] + 1.0;
     const double bias1 = 1.0 - pow((double)beta1, step), bias2 = 1.0 - pow((double)beta2, step);
@@ -246,6 +252,108 @@ static int clip_run(int count, float* const* grads, const int64_t* numel, long l
 }
 
 // ---------------------------------------------------------------------------
+// The norm of all gradients and the clipping coefficient alone, for an optimiser that multiplies the gradients as it
+// reads them (adam_kernel<true>): clipping by itself reads them twice and writes them, and Adam reads them again --
+// 12 of the 40 bytes an element that the two move together; here the gradients are read twice and stay as they are.
+// Squares and sums in double: a gradient of 1e30 has a norm, and the result does not depend on how the tensors are cut.
+// One partial sum per workgroup, which takes a contiguous stretch of 4096-element chunks (the tensor of its first
+// chunk is searched for once); the partials are folded in a fixed order.
+// ---------------------------------------------------------------------------
+constexpr int NORM_MAX_TENSORS = 160;   // 20 bytes of kernel arguments each
+constexpr int NORM_BLOCKS = 2048;       // workgroups of a launch, at most
+struct NormTensors {
+    const float* g[NORM_MAX_TENSORS];
+    long long n[NORM_MAX_TENSORS];
+    int first_chunk[NORM_MAX_TENSORS + 1];
+    int count;
+};
+
+__global__ __launch_bounds__(256) void norm_sumsq_kernel(NormTensors t, int chunks, double* __restrict__ partials) {
+    __shared__ double s_wave[4];
+    const int begin = (int)((long long)chunks * blockIdx.x / gridDim.x), end = (int)((long long)chunks * (blockIdx.x + 1) / gridDim.x);
+    int k = 0;
+    for (int hi = t.count; k + 1 < hi;) {   // the last tensor that starts at or before the first chunk
+        const int mid = (k + hi) >> 1;
+        if (t.first_chunk[mid] <= begin) k = mid;
+        else hi = mid;
+    }
+    double s = 0.0;
+    for (int c = begin; c < end; ++c) {
+        while (k + 1 < t.count && c >= t.first_chunk[k + 1]) ++k;
+        const long long base = (long long)(c - t.first_chunk[k]) * CLIP_CHUNK, n = t.n[k];
+        const float* __restrict__ g = t.g[k];
+        if (((size_t)g & 15) == 0 && base + CLIP_CHUNK <= n) {
+            float4 v[CLIP_CHUNK / 1024];
+#pragma unroll
+            for (int j = 0; j < CLIP_CHUNK / 1024; ++j) v[j] = *reinterpret_cast<const float4*>(g + base + (j * 256 + (int)threadIdx.x) * 4);
+#pragma unroll
+            for (int j = 0; j < CLIP_CHUNK / 1024; ++j) {
+                s = fma((double)v[j].x, (double)v[j].x, s);
+                s = fma((double)v[j].y, (double)v[j].y, s);
+                s = fma((double)v[j].z, (double)v[j].z, s);
+                s = fma((double)v[j].w, (double)v[j].w, s);
+            }
+        } else {
+            const long long stop = base + CLIP_CHUNK < n ? base + CLIP_CHUNK : n;
+#pragma unroll 4
+            for (long long e = base + threadIdx.x; e < stop; e += 256) s = fma((double)g[e], (double)g[e], s);
+        }
+    }
+    for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d, 64);
+    if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) partials[blockIdx.x] = (s_wave[0] + s_wave[1]) + (s_wave[2] + s_wave[3]);
+}
+
+// out[0] = total, out[1] = min(1, max_norm / (total + 1e-6)); a NaN total stays one in both
+__global__ __launch_bounds__(256) void norm_coef_kernel(const double* __restrict__ partials, int n, float max_norm, float* __restrict__ out) {
+    __shared__ double s_wave[4];
+    double s = 0.0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += 256) s += partials[i];
+    for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d, 64);
+    if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const float total = (float)sqrt((s_wave[0] + s_wave[1]) + (s_wave[2] + s_wave[3]));
+        const float coef = max_norm / (total + 1e-6f);
+        out[0] = total;
+        out[1] = (coef < 1.0f || coef != coef) ? coef : 1.0f;
+    }
+}
+
+// Fills launches of up to NORM_MAX_TENSORS tensors; launch(tensors, chunks, workgroups, partials of earlier launches).
+// Returns the number of partials, or -1 for a bad list.
+template <class F>
+static long long norm_launches(int count, const float* const* grads, const int64_t* numel, F&& launch) {
+    long long partials = 0;
+    for (int k = 0; k < count;) {
+        NormTensors t;
+        t.count = 0;
+        long long chunks = 0;
+        for (; k < count && t.count < NORM_MAX_TENSORS; ++k) {
+            if (numel[k] < 0 || (grads && numel[k] > 0 && !grads[k])) return -1;
+            if (numel[k] == 0) continue;
+            const long long more = ceil_div(numel[k], CLIP_CHUNK);
+            if (chunks + more > 0x7fffffffll) {
+                if (t.count == 0) return -1;
+                break;
+            }
+            t.g[t.count] = grads ? grads[k] : nullptr;
+            t.n[t.count] = numel[k];
+            t.first_chunk[t.count++] = (int)chunks;
+            chunks += more;
+        }
+        if (t.count == 0) continue;
+        t.first_chunk[t.count] = (int)chunks;
+        const int blocks = (int)(chunks < NORM_BLOCKS ? chunks : NORM_BLOCKS);
+        if (!launch(t, (int)chunks, blocks, partials)) return partials;
+        partials += blocks;
+    }
+    return partials;
+}
+
+// ---------------------------------------------------------------------------
 // The same clipping for callers that cannot allocate (code under HIP graph capture, serving or
 // training loops with a fixed memory plan): the scratch floats live in this file-scope device
 // array instead of a caller workspace.  Each GPU holds its own copy of the array at its own
@@ -278,14 +386,16 @@ static int clip_static_scratch(float** out) {
 using namespace nerf;
 
 // step_state: null (the step count is `step`), or 4 floats in device memory whose first holds the count of steps taken.
+// R: the type the betas arrive in; 1 - beta is formed from it in double.  grad_scale: null, or one float in device memory.
+template <class R>
 static int adam_run(const char* who, int count, float* const* params, const float* const* grads, float* const* exp_avg,
-                    float* const* exp_avg_sq, const int64_t* numel, int64_t step, float* step_state, float lr, float beta1,
-                    float beta2, float eps, float weight_decay, hipStream_t stream) {
+                    float* const* exp_avg_sq, const int64_t* numel, int64_t step, float* step_state, float lr, R beta1,
+                    R beta2, float eps, float weight_decay, const float* grad_scale, hipStream_t stream) {
     // the scalars as torch computes them (Python floats = double), rounded to float where a tensor op consumes them
     const float b1m = (float)(1.0 - (double)beta1), b2m = (float)(1.0 - (double)beta2);
     float bias2_sqrt = 1.0f, neg_step = 0.0f;
     if (step_state) {
-        hipLaunchKernelGGL(adam_advance_kernel, dim3(1), dim3(64), 0, stream, step_state, beta1, beta2);
+        hipLaunchKernelGGL(adam_advance_kernel<R>, dim3(1), dim3(64), 0, stream, step_state, beta1, beta2);
         if (int rc = check_launch(who)) return rc;
     } else {
         const double bias1 = 1.0 - pow((double)beta1, (double)step), bias2 = 1.0 - pow((double)beta2, (double)step);
@@ -307,8 +417,12 @@ static int adam_run(const char* who, int count, float* const* params, const floa
         }
         if (t.count == 0) continue;
         t.first_block[t.count] = blocks;
-        hipLaunchKernelGGL(adam_kernel, dim3(blocks), dim3(256), 0, stream, t, b1m, beta2, b2m, bias2_sqrt, eps, neg_step,
-                           weight_decay, (const float*)step_state);
+        if (grad_scale)
+            hipLaunchKernelGGL(adam_kernel<true>, dim3(blocks), dim3(256), 0, stream, t, b1m, (float)beta2, b2m, bias2_sqrt, eps, neg_step,
+                               weight_decay, (const float*)step_state, grad_scale);
+        else
+            hipLaunchKernelGGL(adam_kernel<false>, dim3(blocks), dim3(256), 0, stream, t, b1m, (float)beta2, b2m, bias2_sqrt, eps, neg_step,
+                               weight_decay, (const float*)step_state, grad_scale);
         if (int rc = check_launch(who)) return rc;
     }
     return NERF_OK;
@@ -321,7 +435,7 @@ extern "C" int nerf_adam_step(int count, float* const* params, const float* cons
     NERF_REQUIRE(params && grads && exp_avg && exp_avg_sq && numel, "nerf_adam_step: null pointer");
     NERF_REQUIRE(count > 0 && step >= 1, "nerf_adam_step: count=%d step=%lld", count, (long long)step);
     return adam_run("nerf_adam_step", count, params, grads, exp_avg, exp_avg_sq, numel, step, nullptr, lr, beta1, beta2, eps,
-                    weight_decay, (hipStream_t)stream);
+                    weight_decay, nullptr, (hipStream_t)stream);
 }
 
 extern "C" int nerf_adam_step_capturable(int count, float* const* params, const float* const* grads, float* const* exp_avg,
@@ -331,7 +445,7 @@ extern "C" int nerf_adam_step_capturable(int count, float* const* params, const 
     NERF_REQUIRE(count >= 0 && (count == 0 || (params && grads && exp_avg && exp_avg_sq && numel)),
                  "nerf_adam_step_capturable: null pointer");
     return adam_run("nerf_adam_step_capturable", count, params, grads, exp_avg, exp_avg_sq, numel, 0, step_state, 0.0f, beta1,
-                    beta2, eps, weight_decay, (hipStream_t)stream);
+                    beta2, eps, weight_decay, nullptr, (hipStream_t)stream);
 }
 
 extern "C" int nerf_adam_set_lr(float* step_state, float lr, void* stream) {
@@ -368,4 +482,39 @@ extern "C" int nerf_clip_grad_norm_static(int count, float* const* grads, const 
     if (int rc = clip_static_scratch(&ptr)) return rc;
     // nothing in the scratch has to start at zero: every partial that is read is written first by this call
     return clip_run(count, grads, numel, chunks, max_norm, ptr, total_norm, (hipStream_t)stream);
+}
+
+extern "C" size_t nerf_grad_norm_workspace_doubles(int count, const int64_t* numel) {
+    if (count <= 0 || !numel) return 0;
+    const long long n = norm_launches(count, nullptr, numel, [](const NormTensors&, int, int, long long) { return true; });
+    return n > 0 ? (size_t)n : 0;
+}
+
+extern "C" int nerf_grad_norm(int count, const float* const* grads, const int64_t* numel, float max_norm, double* workspace, float* norm_coef,
+                              void* stream) {
+    NERF_REQUIRE(count >= 0 && (count == 0 || (grads && numel)) && norm_coef, "nerf_grad_norm: null pointer");
+    NERF_REQUIRE(max_norm >= 0.0f, "nerf_grad_norm: max_norm=%g", (double)max_norm);
+    const long long n = norm_launches(count, grads, numel, [](const NormTensors&, int, int, long long) { return true; });
+    NERF_REQUIRE(n >= 0 && n < (1ll << 31), "nerf_grad_norm: bad tensor list");
+    NERF_REQUIRE(n == 0 || workspace, "nerf_grad_norm: null workspace");
+    int rc = NERF_OK;
+    norm_launches(count, grads, numel, [&](const NormTensors& t, int chunks, int blocks, long long done) {
+        hipLaunchKernelGGL(norm_sumsq_kernel, dim3(blocks), dim3(256), 0, (hipStream_t)stream, t, chunks, workspace + done);
+        rc = check_launch("nerf_grad_norm");
+        return rc == NERF_OK;
+    });
+    if (rc) return rc;
+    hipLaunchKernelGGL(norm_coef_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, workspace, (int)n, max_norm, norm_coef);
+    return check_launch("nerf_grad_norm(coef)");
+}
+
+extern "C" int nerf_adam_step_scaled(int count, float* const* params, const float* const* grads, float* const* exp_avg, float* const* exp_avg_sq,
+                                     const int64_t* numel, int64_t step, float* step_state, float lr, double beta1, double beta2, float eps,
+                                     float weight_decay, const float* grad_scale, void* stream) {
+    const char* who = "nerf_adam_step_scaled";
+    NERF_REQUIRE(count >= 0 && (count == 0 || (params && grads && exp_avg && exp_avg_sq && numel)) && grad_scale, "%s: null pointer", who);
+    NERF_REQUIRE(step_state || step >= 1, "%s: step=%lld", who, (long long)step);
+    NERF_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "%s: betas %g %g", who, beta1, beta2);
+    return adam_run(who, count, params, grads, exp_avg, exp_avg_sq, numel, step, step_state, lr, beta1, beta2, eps, weight_decay, grad_scale,
+                    (hipStream_t)stream);
 }

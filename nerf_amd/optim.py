@@ -6,7 +6,11 @@ Drop-in for the way the reference's training loops use ``torch.optim.Adam``
 loops use, same update rule, and a ``state_dict`` with torch's keys
 (``step`` / ``exp_avg`` / ``exp_avg_sq``), so checkpoints move both ways.  ``weight_decay`` is torch's L2
 form (src/train_nerf_llff.py:82, src/train_nerf_skow.py:47 use 1e-6); amsgrad and maximize are
-not implemented and raise.  ``clip_grad_norm_`` (src/train_nerf.py:165) lives in ``nerf_amd.ops``.
+not implemented and raise.  ``clip_grad_norm_`` (src/train_nerf.py:165) lives in ``nerf_amd.ops``;
+``max_grad_norm`` does the same clipping inside ``step()``: the 2-norm of the gradients of all groups together, and
+Adam on the gradients times min(1, max_grad_norm / (norm + 1e-6)), formed as they are read -- the gradients themselves
+are left as they are.  ``grad_norm`` is then the norm of the last step, a 0-d tensor on the device (the same tensor for
+every step, also under a captured graph), NaN or infinite where a gradient is, as with ``clip_grad_norm_``.
 
 ``capturable=True`` (torch's name for it) keeps the step count AND the learning rate in device memory, so that a
 whole training step -- this optimiser's launch included -- can be captured into a HIP graph and replayed
@@ -27,11 +31,15 @@ from . import _lib as L
 
 class FusedAdam(torch.optim.Optimizer):
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0,
-                 amsgrad: bool = False, maximize: bool = False, capturable: bool = False):
+                 amsgrad: bool = False, maximize: bool = False, capturable: bool = False, max_grad_norm: float | None = None):
         if amsgrad or maximize:
             raise NotImplementedError("FusedAdam implements Adam without amsgrad or maximize")
         if lr < 0.0 or eps < 0.0 or weight_decay < 0.0 or not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0:
             raise ValueError("invalid Adam hyper-parameters")
+        if max_grad_norm is not None and not max_grad_norm >= 0.0:
+            raise ValueError("max_grad_norm must be at least 0")
+        self.max_grad_norm = max_grad_norm   # not part of the state dict, whose keys are torch's
+        self._norm = None                    # device floats: the norm of the last step, the coefficient it led to
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=False,
                                       maximize=False, capturable=bool(capturable)))
         self._dev_state = {}   # capturable groups: index -> 4 device floats, [0] = steps taken, [3] = learning rate
@@ -87,12 +95,74 @@ class FusedAdam(torch.optim.Optimizer):
         self._dev_state = {}   # rebuilt from the loaded step counts on the next step
         self._dev_lr = {}
 
+    @property
+    def grad_norm(self):
+        """The norm of all gradients in the last ``step()`` (0-d, on the device); None without ``max_grad_norm``
+        or before the first step."""
+        return None if self._norm is None else self._norm[0]
+
+    def _step_clipped(self) -> None:
+        lib = L.lib()
+        work = []   # per group: its index, the group, parameters, gradients, states
+        for gi, group in enumerate(self.param_groups):
+            ps = [p for p in group["params"] if p.grad is not None]
+            if not ps:
+                continue
+            grads = [p.grad for p in ps]
+            if any(g.is_sparse for g in grads):
+                raise L.NerfHipError("FusedAdam does not take sparse gradients")
+            if not all(p.dtype == torch.float32 and p.is_contiguous() for p in ps):
+                raise L.NerfHipError("FusedAdam needs contiguous float32 parameters")
+            work.append((gi, group, ps, [g if g.dtype == torch.float32 and g.is_contiguous() else L.f32c(g) for g in grads]))
+        if not work:
+            if self._norm is not None:
+                self._norm[0] = 0.0
+            return
+        every = [g for _, _, _, grads in work for g in grads]
+        L.same_device(*[p for _, _, ps, _ in work for p in ps], *every)
+        if self._norm is None or self._norm.device != every[0].device:
+            self._norm = torch.zeros(2, device=every[0].device)
+        n = len(every)
+        numel = (C.c_int64 * n)(*[g.numel() for g in every])
+        pointers = (C.c_void_p * n)(*[g.data_ptr() for g in every])
+        partials = torch.empty(lib.nerf_grad_norm_workspace_doubles(n, numel), device=every[0].device, dtype=torch.float64)
+        L.launch("nerf_grad_norm", every[0], n, pointers, numel, float(self.max_grad_norm), L.ptr(partials), L.ptr(self._norm))
+        coef = self._norm.data_ptr() + 4
+        for gi, group, ps, grads in work:
+            states = [self.state[p] for p in ps]
+            for p, st in zip(ps, states):
+                if not st:
+                    st["step"] = torch.tensor(0.0)
+                    st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                    st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+            parts = {None: range(len(ps))}
+            if group.get("capturable", False):
+                dev = self._capturable_state(gi, ps)
+                self.sync_lr()
+            else:
+                dev, parts = None, {}
+                # parameters of one group share the step count unless states were loaded piecemeal
+                for i, st in enumerate(states):
+                    parts.setdefault(int(st["step"].item()), []).append(i)
+            (beta1, beta2) = group["betas"]
+            for step0, part in parts.items():
+                m = len(part)
+                arrays = [(C.c_void_p * m)(*[x.data_ptr() for x in ts]) for ts in (
+                    [ps[i] for i in part], [grads[i] for i in part], [states[i]["exp_avg"] for i in part], [states[i]["exp_avg_sq"] for i in part])]
+                L.launch("nerf_adam_step_scaled", ps[0], m, *arrays, (C.c_int64 * m)(*[ps[i].numel() for i in part]),
+                         0 if step0 is None else step0 + 1, L.ptr(dev), group["lr"], beta1, beta2, group["eps"], group["weight_decay"], coef)
+                if step0 is not None:
+                    torch._foreach_add_([states[i]["step"] for i in part], 1.0)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        if self.max_grad_norm is not None:
+            self._step_clipped()
+            return loss
         for gi, group in enumerate(self.param_groups):
             ps = [p for p in group["params"] if p.grad is not None]
             if not ps:
