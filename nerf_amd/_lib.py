@@ -160,22 +160,23 @@ def dense(t: torch.Tensor) -> torch.Tensor:
 
 def launch(name: str, t: torch.Tensor, *args) -> None:
     """Call an entry point on the current stream of ``t``'s device, which need not be the current device."""
-    index = t.device.index
-    fn = getattr(lib(), name)
+    index = t.get_device()
+    fn = getattr(_lib or lib(), name)
+    # the stream's handle itself: a torch.cuda.Stream object costs a microsecond, a fifth of what a small call takes
     if index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc != 0:
         check(rc, name)
 
 
 def same_device(*tensors: torch.Tensor) -> None:
-    need_gpu(*tensors)
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise NerfHipError("the tensors of one call must be on one device, got " + ", ".join(sorted(map(str, devices))))
+    indices = {t.get_device() for t in tensors if t is not None}   # -1: on the CPU
+    if len(indices) > 1 or -1 in indices:
+        need_gpu(*tensors)
+        raise NerfHipError(f"the tensors of one call must be on one device, got cuda:{sorted(indices)}")
 
 
 def ptr_array(tensors):

@@ -205,7 +205,7 @@ class _Embedding(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, table, ids, scale, padding_idx):
-        out = _embedding_fwd(ids, L.dense(table.detach()), scale)
+        out = _embedding_fwd(ids, L.dense(table), scale)
         ctx.save_for_backward(ids)
         ctx.meta = (tuple(table.shape), scale, padding_idx)
         return out
@@ -232,14 +232,17 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, paddin
     gradient (negative: counted from the end), as in ``torch.nn.functional.embedding``.  The gradient of the table is
     dense, formed by sorting the ids -- the same bits for the same inputs, whatever ids repeat -- and summed in float32.
     Differentiable once in ``table``."""
-    L.require(table.dim() == 2, f"table must be [V, D], got {tuple(table.shape)}")
-    L.require(not ids.is_floating_point() and not ids.is_complex() and ids.dtype != torch.bool, f"ids must be integers, got {ids.dtype}")
+    if table.dim() != 2:
+        raise ValueError(f"table must be [V, D], got {tuple(table.shape)}")
+    if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
+        raise ValueError(f"ids must be integers, got {ids.dtype}")
     V = table.shape[0]
     if padding_idx is None:
         padding_idx = -1
-    else:
-        L.require(-V <= padding_idx < V, f"padding_idx {padding_idx} is outside the {V} rows")
+    elif -V <= padding_idx < V:
         padding_idx = int(padding_idx) % V
+    else:
+        raise ValueError(f"padding_idx {padding_idx} is outside the {V} rows")
     L.type_code(table, "table")
     L.same_device(ids, table)
     if ids.dtype not in (torch.int64, torch.int32):
@@ -479,7 +482,7 @@ class _LinearScan(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, gate, x, state, reverse, blend, want_last):
-        gate, x, state = (None if t is None else L.dense(t.detach()) for t in (gate, x, state))
+        gate, x, state = (None if t is None else L.dense(t) for t in (gate, x, state))
         h, last, carry = _scan_fwd(gate, x, state, reverse, blend, want_last, True)
         ctx.save_for_backward(gate, x, state, carry)
         ctx.meta = (reverse, blend)
@@ -518,17 +521,24 @@ def linear_scan(gate: torch.Tensor, x: torch.Tensor, state: Optional[torch.Tenso
     ``return_state``: ``(h, last)``, ``last`` [..., C] float32 the state after the last step, unrounded: what the next call
     takes as ``state`` (a long sequence in parts, or one step at a time with T = 1).
     Differentiable once in ``gate``, ``x`` and ``state``."""
-    L.require(x.dim() >= 2, f"x must be [..., T, C], got {tuple(x.shape)}")
+    # (the texts of these checks are only put together where one fails: a call may take a few microseconds in all)
+    if x.dim() < 2:
+        raise ValueError(f"x must be [..., T, C], got {tuple(x.shape)}")
     lead, T, C = x.shape[:-2], x.shape[-2], x.shape[-1]
-    L.require(gate.dim() == x.dim() and gate.shape[:-1] == x.shape[:-1], f"gate must be {[*x.shape[:-1]]} + [G], got {tuple(gate.shape)}")
+    if gate.shape[:-1] != x.shape[:-1]:
+        raise ValueError(f"gate must be {[*x.shape[:-1]]} + [G], got {tuple(gate.shape)}")
     G = gate.shape[-1]
-    L.require(C == 0 or (G > 0 and C % G == 0), f"{G} gates do not divide {C} channels")
-    L.require(gate.is_floating_point(), f"gate must be floating point, got {gate.dtype}")
+    if C != 0 and (G == 0 or C % G != 0):
+        raise ValueError(f"{G} gates do not divide {C} channels")
+    if not gate.is_floating_point():
+        raise ValueError(f"gate must be floating point, got {gate.dtype}")
     if gate.dtype != x.dtype and gate.dtype != torch.float32:
         gate = gate.float()
     if state is not None:
-        L.require(tuple(state.shape) == (*lead, C), f"state must be {[*lead, C]}, got {tuple(state.shape)}")
-        L.require(state.is_floating_point(), f"state must be floating point, got {state.dtype}")
+        if state.shape != (*lead, C):
+            raise ValueError(f"state must be {[*lead, C]}, got {tuple(state.shape)}")
+        if not state.is_floating_point():
+            raise ValueError(f"state must be floating point, got {state.dtype}")
         state = state.float()
     L.type_code(x, "x")
     L.same_device(gate, x, state)
@@ -537,16 +547,20 @@ def linear_scan(gate: torch.Tensor, x: torch.Tensor, state: Optional[torch.Tenso
         if not return_state:
             return h
         return h, (state.clone() if state is not None else torch.zeros(*lead, C, device=x.device))
-    B = lead.numel()
-    gate3, x3 = gate.reshape(B, T, G), x.reshape(B, T, C)
-    state2 = state.reshape(B, C) if state is not None else None
-    if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or (state is not None and state.requires_grad)):
-        h, last = _LinearScan.apply(gate3, x3, state2, bool(reverse), bool(blend), bool(return_state))
+    train = torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or (state is not None and state.requires_grad))
+    shape = x.shape
+    if len(shape) != 3:   # (a view of nothing new would still be a node of the graph)
+        B = lead.numel()
+        gate, x = gate.reshape(B, T, G), x.reshape(B, T, C)
+        state = state.reshape(B, C) if state is not None else None
+    if train:
+        h, last = _LinearScan.apply(gate, x, state, bool(reverse), bool(blend), bool(return_state))
     else:
-        h, last, _ = _scan_fwd(L.dense(gate3.detach()), L.dense(x3.detach()), None if state is None else L.dense(state2.detach()), bool(reverse),
+        h, last, _ = _scan_fwd(L.dense(gate.detach()), L.dense(x.detach()), None if state is None else L.dense(state.detach()), bool(reverse),
                                bool(blend), bool(return_state), False)
-    h = h.view(x.shape)
-    return (h, last.view(*lead, C)) if return_state else h
+    if len(shape) != 3:
+        h, last = h.view(shape), last.view(*lead, C) if return_state else None
+    return (h, last) if return_state else h
 
 
 # ---------------------------------------------------------- fused MLPs ----

@@ -118,8 +118,10 @@ class FusedAdam(torch.optim.Optimizer):
             if self._norm is not None:
                 self._norm[0] = 0.0
             return
-        every = [g for _, _, _, grads in work for g in grads]
-        L.same_device(*[p for _, _, ps, _ in work for p in ps], *every)
+        every = work[0][3] if len(work) == 1 else [g for _, _, _, grads in work for g in grads]
+        devices = {t.get_device() for _, _, ps, grads in work for ts in (ps, grads) for t in ts}
+        if len(devices) > 1 or -1 in devices:
+            L.same_device(*[p for _, _, ps, _ in work for p in ps], *every)
         if self._norm is None or self._norm.device != every[0].device:
             self._norm = torch.zeros(2, device=every[0].device)
         n = len(every)
@@ -135,24 +137,41 @@ class FusedAdam(torch.optim.Optimizer):
                     st["step"] = torch.tensor(0.0)
                     st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
                     st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-            parts = {None: range(len(ps))}
             if group.get("capturable", False):
                 dev = self._capturable_state(gi, ps)
                 self.sync_lr()
+                parts = [(0, None, range(len(ps)))]
             else:
-                dev, parts = None, {}
-                # parameters of one group share the step count unless states were loaded piecemeal
-                for i, st in enumerate(states):
-                    parts.setdefault(int(st["step"].item()), []).append(i)
-            (beta1, beta2) = group["betas"]
-            for step0, part in parts.items():
+                dev, parts = None, self._shared_steps(states)
+            beta1, beta2 = group["betas"]
+            for step0, step, part in parts:
                 m = len(part)
-                arrays = [(C.c_void_p * m)(*[x.data_ptr() for x in ts]) for ts in (
-                    [ps[i] for i in part], [grads[i] for i in part], [states[i]["exp_avg"] for i in part], [states[i]["exp_avg_sq"] for i in part])]
-                L.launch("nerf_adam_step_scaled", ps[0], m, *arrays, (C.c_int64 * m)(*[ps[i].numel() for i in part]),
-                         0 if step0 is None else step0 + 1, L.ptr(dev), group["lr"], beta1, beta2, group["eps"], group["weight_decay"], coef)
-                if step0 is not None:
-                    torch._foreach_add_([states[i]["step"] for i in part], 1.0)
+                ms, vs = [states[i]["exp_avg"].data_ptr() for i in part], [states[i]["exp_avg_sq"].data_ptr() for i in part]
+                if m == n:   # the one list of the one group: as the norm had it
+                    gp, counts, pp = pointers, numel, [p.data_ptr() for p in ps]
+                else:
+                    gp = (C.c_void_p * m)(*[grads[i].data_ptr() for i in part])
+                    counts, pp = (C.c_int64 * m)(*[ps[i].numel() for i in part]), [ps[i].data_ptr() for i in part]
+                L.launch("nerf_adam_step_scaled", ps[0], m, (C.c_void_p * m)(*pp), gp, (C.c_void_p * m)(*ms), (C.c_void_p * m)(*vs), counts,
+                         step0 + 1, L.ptr(dev), group["lr"], beta1, beta2, group["eps"], group["weight_decay"], coef)
+                if step is not None:
+                    step = step + 1   # a new tensor: a parameter without a gradient in this step keeps the old one
+                    for i in part:
+                        states[i]["step"] = step
+
+    @staticmethod
+    def _shared_steps(states):
+        """(steps taken, step tensor, members) of the states that have taken equally many: normally all of them, unless
+        states were loaded piecemeal or a parameter had no gradient in some step.  The members of a part are left with
+        one step tensor between them, which is never written, so that counting a step is one operation and not one per
+        parameter (``state_dict`` hands out a copy for each)."""
+        by_tensor = {}
+        for i, st in enumerate(states):
+            by_tensor.setdefault(id(st["step"]), []).append(i)
+        by_count = {}
+        for members in by_tensor.values():
+            by_count.setdefault(int(states[members[0]]["step"].item()), []).extend(members)
+        return [(count, states[members[0]]["step"], members) for count, members in by_count.items()]
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -205,5 +224,5 @@ class FusedAdam(torch.optim.Optimizer):
                     group["betas"][0], group["betas"][1], group["eps"], group["weight_decay"],
                     L.stream_of(plist[0])), "nerf_adam_step")
                 for p in plist:
-                    self.state[p]["step"] += 1
+                    self.state[p]["step"] = self.state[p]["step"] + 1   # not in place: clipped steps share the tensor
         return loss

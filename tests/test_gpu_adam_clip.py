@@ -135,6 +135,28 @@ def test_same_as_clipping_first(dev):
 
 
 @pytest.mark.gpu
+def test_step_counts_stay_apart(dev):
+    """A parameter that misses a step, clipping switched off and on again, states loaded piecemeal: every parameter is
+    stepped with its own count, as torch's Adam does it."""
+    from nerf_amd.optim import FusedAdam
+    shapes = [(40, 3), (17,), (4097,)]
+    ps, _ = make(shapes, 1.0, 5, dev)
+    a = [torch.nn.Parameter(p.clone().to(dev)) for p in ps]
+    b = [torch.nn.Parameter(p.clone().to(dev)) for p in ps]
+    mine, ref = FusedAdam(a, lr=1e-2, max_grad_norm=1e9), torch.optim.Adam(b, lr=1e-2)
+    for step in range(7):
+        gs = make(shapes, 1.0, 50 + step, dev)[1]
+        for k, (p, q, g) in enumerate(zip(a, b, gs)):
+            p.grad, q.grad = (None, None) if (step, k) in ((1, 0), (2, 2), (4, 1)) else (g.to(dev), g.to(dev))
+        mine.max_grad_norm = None if step in (3, 4) else 1e9
+        mine.step()
+        ref.step()
+        for k, (p, q) in enumerate(zip(a, b)):
+            assert float(mine.state[p]["step"]) == float(ref.state[q]["step"]), (step, k)
+            assert torch.allclose(p, q, rtol=2e-6, atol=1e-7 * (step + 1)), (step, k)
+
+
+@pytest.mark.gpu
 def test_infinite_and_nan_gradients(dev):
     from nerf_amd.optim import FusedAdam
     for bad in (float("inf"), float("nan")):
