@@ -5,11 +5,13 @@
 // The forward pass is a gather bound by memory.  The gradient is formed without atomics, so that equal inputs give equal
 // bits and a row that most of the batch asks for (one image's code in a whole ray batch, a frequent token) costs no more
 // than its bytes: the positions are sorted by id with a stable radix sort (ids that take no gradient -- out of range, or
-// the padding row -- sort behind all others as id V), and every row of d_table is then written exactly once, zeros
-// included, from the run of sorted positions that its id owns:
-//   - each aligned chunk of 64 sorted positions that lies inside one run is summed into a partial row;
-//   - runs of at least 128 positions are summed by a workgroup, from their whole chunks' partials and the positions at
-//     both ends; shorter ones by a few lanes from d_out itself.
+// the padding row -- sort behind all others as id V).  The sorted positions are cut into chunks of equal size, whatever
+// runs of equal ids they hold, one wave each, so that the work is even however skewed the ids are:
+//   - a wave adds up its chunk's rows, run by run.  A run that lies inside the chunk is finished and written; the
+//     stretches of runs that cross the chunk's borders are left as partial rows, at most two a chunk;
+//   - a second launch joins the partial rows of each run that crosses chunks.
+// The rows that no id names are zeros: the whole table is cleared by workgroups of the first sorting launch, which fill
+// the compute units that the sort leaves idle.
 // Sums are held in float, in an order that the ids alone decide, and rounded once.
 #include <algorithm>
 
@@ -17,37 +19,53 @@
 
 namespace nerf {
 
-constexpr int EMB_CHUNK = 64;        // sorted positions of a partial row
-constexpr int EMB_LONG = 128;        // runs from this length on contain at least one whole chunk
-constexpr int EMB_CANDIDATES = 16;   // chunks whose long run, if one starts there, one workgroup sums
+constexpr int JOIN_THREADS = 512;
+constexpr int JOIN_CHUNKS = 64;      // most chunks whose crossing runs one workgroup joins
 
-constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64, SORT_ITEMS = 8;
-constexpr int SORT_TILE = SORT_THREADS * SORT_ITEMS;   // keys that a workgroup ranks at once
+constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
+constexpr int SORT_ITEMS = 4, SORT_TILE = SORT_THREADS * SORT_ITEMS;   // keys that a workgroup ranks at once
 constexpr int SORT_BITS = 10, SORT_DIGITS = 1 << SORT_BITS;
+constexpr int SMALL_ITEMS = 16, SMALL_TILE = SORT_THREADS * SMALL_ITEMS;   // keys that one workgroup sorts by itself ...
+constexpr int SMALL_BITS = 8, SMALL_DIGITS = 1 << SMALL_BITS;              // ... in LDS, beside smaller counters
+constexpr int SORT_FEW_TILES = 32;
+constexpr unsigned NO_KEY = 0xffffffffu;
 
 // ---- forward ---------------------------------------------------------------------------------------------------
-template <class T, int VEC, class ID>
+// A group of lanes per row, ROWS rows at a time: their ids, then their elements, are under way together.
+template <class T, int VEC, class ID, int ROWS>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(const T* __restrict__ table, int64_t V, int D, const ID* __restrict__ ids, int64_t N,
                                                             float scale, int l_lanes, T* __restrict__ out) {
-    const int lanes = 1 << l_lanes, vectors = D / VEC;
-    const int64_t step = (int64_t)gridDim.x * (256 >> l_lanes);
-    for (int64_t n = (int64_t)blockIdx.x * (256 >> l_lanes) + (threadIdx.x >> l_lanes); n < N; n += step) {
-        const int64_t id = (int64_t)ids[n];
-        const bool good = id >= 0 && id < V;
-        for (int i = (threadIdx.x & (lanes - 1)) + (int)blockIdx.y * lanes; i < vectors; i += lanes * (int)gridDim.y) {
-            float v[VEC];
-            if (good) {
-                load_run<VEC>(table + id * D + (int64_t)i * VEC, v);
+    const int lanes = 1 << l_lanes, vectors = D / VEC, at_once = 256 >> l_lanes, first = (threadIdx.x & (lanes - 1)) + (int)blockIdx.y * lanes;
+    for (int64_t n0 = (int64_t)blockIdx.x * ROWS * at_once + (threadIdx.x >> l_lanes); n0 < N; n0 += (int64_t)gridDim.x * ROWS * at_once) {
+        int64_t id[ROWS];
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) v[k] *= scale;
-            } else {
+        for (int r = 0; r < ROWS; ++r) id[r] = n0 + r * at_once < N ? (int64_t)ids[n0 + r * at_once] : -1;
+        for (int i = first; i < vectors; i += lanes * (int)gridDim.y) {
+            float v[ROWS][VEC];
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) v[k] = __builtin_nanf("");
+            for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) v[r][k] = __builtin_nanf("");
+                if (id[r] >= 0 && id[r] < V) load_run<VEC>(table + id[r] * D + (int64_t)i * VEC, v[r]);
             }
-            store_run<VEC>(out + n * D + (int64_t)i * VEC, v);
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) v[r][k] *= scale;
+                if (n0 + r * at_once < N) store_run<VEC>(out + (n0 + r * at_once) * D + (int64_t)i * VEC, v[r]);
+            }
         }
     }
 }
+
+// Zeros over the table's gradient, 16 bytes a store: workgroup `block` of `blocks`, 1024 threads each.
+__device__ __forceinline__ void clear_table(char* __restrict__ p, int64_t bytes, int64_t block, int64_t blocks) {
+    const int64_t wide = bytes >> 4;
+    for (int64_t i = block * 1024 + threadIdx.x; i < wide; i += blocks * 1024) reinterpret_cast<uint4*>(p)[i] = uint4{0u, 0u, 0u, 0u};
+    if (block == 0 && (int64_t)threadIdx.x < bytes - (wide << 4)) p[(wide << 4) + threadIdx.x] = 0;
+}
+
+__global__ __launch_bounds__(1024) void clear_kernel(char* __restrict__ p, int64_t bytes) { clear_table(p, bytes, blockIdx.x, gridDim.x); }
 
 // ---- stable radix sort of (id, position) -------------------------------------------------------------------------
 template <class ID>
@@ -61,33 +79,42 @@ __device__ __forceinline__ unsigned sort_key(ID id, int64_t V, int64_t padding) 
 // digit find each other by ballots, take their ranks from the old count, and the last of them writes the new one.
 // On return rank[r] is the key's place within its wave and digit, and after digit_starts() count[w][d] is where the
 // wave's keys of digit d start in the sorted tile.
-__device__ __forceinline__ void rank_in_wave(const unsigned (&key)[SORT_ITEMS], const bool (&on)[SORT_ITEMS], int shift, int bits,
-                                             volatile unsigned* __restrict__ count, unsigned (&rank)[SORT_ITEMS]) {
+template <int ITEMS, int DIGITS>
+__device__ __forceinline__ void rank_in_wave(const unsigned (&key)[ITEMS], const bool (&on)[ITEMS], int shift, int bits, unsigned (&count)[SORT_WAVES][DIGITS],
+                                             unsigned (&rank)[ITEMS]) {
     const unsigned mask = (1u << bits) - 1u;
-    const unsigned long long below = (1ull << (threadIdx.x & 63)) - 1ull;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const unsigned long long below = (1ull << lane) - 1ull;
 #pragma unroll
-    for (int r = 0; r < SORT_ITEMS; ++r) {
+    for (int r = 0; r < ITEMS; ++r) {
         const unsigned d = (key[r] >> shift) & mask;
         unsigned long long same = __ballot(on[r]);
-        for (int b = 0; b < bits; ++b) {
-            const bool bit = (d >> b) & 1u;
-            const unsigned long long set = __ballot(bit);
-            same &= bit ? set : ~set;
+        unsigned lo = (unsigned)same, hi = (unsigned)(same >> 32);
+        for (int b = 0; b < bits; ++b) {   // four vector instructions a bit: this loop is what ranking costs
+            const int m = (int)(d << (31 - b)) >> 31;   // all ones where the bit is set
+            const unsigned long long set = __ballot(m != 0);
+            lo &= ~((unsigned)set ^ (unsigned)m);
+            hi &= ~((unsigned)(set >> 32) ^ (unsigned)m);
         }
+        same = (unsigned long long)hi << 32 | lo;
         rank[r] = 0;
         if (on[r]) {
-            const unsigned old = count[d];
+            const unsigned old = count[wave][d];
             rank[r] = old + (unsigned)__popcll(same & below);
-            if ((same >> (threadIdx.x & 63)) == 1ull) count[d] = old + (unsigned)__popcll(same);   // the highest of them
+            if ((same >> lane) == 1ull) count[wave][d] = old + (unsigned)__popcll(same);   // the highest of them
         }
+        // the next round reads what other lanes of this wave have just written: LDS keeps a wave's accesses in order,
+        // the compiler has to as well
         __builtin_amdgcn_wave_barrier();
+        asm volatile("" ::: "memory");
     }
 }
 
 // Exclusive sum over the workgroup's 1024 threads.
-__device__ __forceinline__ unsigned block_exclusive(unsigned v, unsigned* __restrict__ s_wave) {
+__device__ __forceinline__ unsigned block_exclusive(unsigned v, unsigned (&s_wave)[SORT_WAVES]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     unsigned inc = v;
+#pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
         const unsigned o = __shfl_up(inc, d, 64);
         if (lane >= d) inc += o;
@@ -95,56 +122,75 @@ __device__ __forceinline__ unsigned block_exclusive(unsigned v, unsigned* __rest
     if (lane == 63) s_wave[wave] = inc;
     __syncthreads();
     unsigned base = 0;
-    for (int w = 0; w < wave; ++w) base += s_wave[w];
+#pragma unroll
+    for (int w = 0; w < SORT_WAVES; ++w) base += w < wave ? s_wave[w] : 0u;
     __syncthreads();
     return base + inc - v;
 }
 
-// count[w][d] -> where the keys of wave w and digit d start in the sorted tile (thread d does digit d); returns the
-// number of keys of the thread's digit and, in `start`, where they begin.
-__device__ __forceinline__ unsigned digit_starts(unsigned (*__restrict__ count)[SORT_DIGITS], unsigned* __restrict__ s_wave, unsigned& start) {
-    unsigned total = 0;
-    for (int w = 0; w < SORT_WAVES; ++w) total += count[w][threadIdx.x];
+// count[w][d] -> where the keys of wave w and digit d start in the sorted tile (thread d does digit d); `start`: where
+// the digit's keys begin.
+template <int DIGITS>
+__device__ __forceinline__ void digit_starts(unsigned (&count)[SORT_WAVES][DIGITS], unsigned (&s_wave)[SORT_WAVES], int digits, unsigned& start) {
+    const int d = threadIdx.x;
+    unsigned c[SORT_WAVES], total = 0;
+#pragma unroll
+    for (int w = 0; w < SORT_WAVES; ++w) {
+        c[w] = d < digits ? count[w][d] : 0u;
+        total += c[w];
+    }
     start = block_exclusive(total, s_wave);
     unsigned at = start;
-    for (int w = 0; w < SORT_WAVES; ++w) {
-        const unsigned c = count[w][threadIdx.x];
-        count[w][threadIdx.x] = at;
-        at += c;
+    if (d < digits) {
+#pragma unroll
+        for (int w = 0; w < SORT_WAVES; ++w) {
+            count[w][d] = at;
+            at += c[w];
+        }
     }
-    return total;
 }
 
-// Up to SORT_TILE keys: every pass in one workgroup, the pairs changing places through LDS.
-template <class ID>
+template <int DIGITS>
+__device__ __forceinline__ void clear_counts(unsigned (&count)[SORT_WAVES][DIGITS], int digits) {
+#pragma unroll
+    for (int w = 0; w < SORT_WAVES; ++w)
+        if ((int)threadIdx.x < digits) count[w][threadIdx.x] = 0u;
+}
+
+// Up to SMALL_TILE keys: every pass in one workgroup, the pairs changing places through LDS.
+template <class ID, int ITEMS>
 __global__ __launch_bounds__(SORT_THREADS) void sort_small_kernel(const ID* __restrict__ ids, int n, int64_t V, int64_t padding, int passes, int bits,
-                                                                  unsigned* __restrict__ keys, unsigned* __restrict__ vals) {
-    __shared__ unsigned s_count[SORT_WAVES][SORT_DIGITS];
-    __shared__ unsigned s_key[SORT_TILE];
-    __shared__ unsigned short s_val[SORT_TILE];
+                                                                  uint2* __restrict__ sorted, char* __restrict__ clear, int64_t clear_bytes) {
+    if (blockIdx.x > 0) {
+        clear_table(clear, clear_bytes, blockIdx.x - 1, gridDim.x - 1);
+        return;
+    }
+    __shared__ unsigned s_count[SORT_WAVES][SMALL_DIGITS];
+    __shared__ unsigned s_key[SORT_THREADS * ITEMS];
+    __shared__ unsigned short s_val[SORT_THREADS * ITEMS];
     __shared__ unsigned s_wave[SORT_WAVES];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int items = (n + SORT_THREADS - 1) / SORT_THREADS;   // rounds in use: the tile is packed to the front of every wave
-    unsigned key[SORT_ITEMS], rank[SORT_ITEMS], val[SORT_ITEMS];
-    bool on[SORT_ITEMS];
+    unsigned key[ITEMS], rank[ITEMS], val[ITEMS];
+    bool on[ITEMS];
 #pragma unroll
-    for (int r = 0; r < SORT_ITEMS; ++r) {
+    for (int r = 0; r < ITEMS; ++r) {
         const int i = wave * 64 * items + r * 64 + lane;
         on[r] = r < items && i < n;
         key[r] = on[r] ? sort_key(ids[i], V, padding) : 0u;
         val[r] = (unsigned)i;
     }
     for (int p = 0; p < passes; ++p) {
-        for (int i = threadIdx.x; i < SORT_WAVES * SORT_DIGITS; i += SORT_THREADS) (&s_count[0][0])[i] = 0u;
+        clear_counts(s_count, 1 << bits);
         __syncthreads();
-        rank_in_wave(key, on, p * bits, bits, s_count[wave], rank);
+        rank_in_wave(key, on, p * bits, bits, s_count, rank);
         __syncthreads();
         unsigned start;
-        digit_starts(s_count, s_wave, start);
+        digit_starts(s_count, s_wave, 1 << bits, start);
         __syncthreads();
         const unsigned mask = (1u << bits) - 1u;
 #pragma unroll
-        for (int r = 0; r < SORT_ITEMS; ++r) {
+        for (int r = 0; r < ITEMS; ++r) {
             if (on[r]) {
                 const unsigned to = s_count[wave][(key[r] >> (p * bits)) & mask] + rank[r];
                 s_key[to] = key[r];
@@ -153,7 +199,7 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_small_kernel(const ID* __re
         }
         __syncthreads();
 #pragma unroll
-        for (int r = 0; r < SORT_ITEMS; ++r) {
+        for (int r = 0; r < ITEMS; ++r) {
             const int i = wave * 64 * items + r * 64 + lane;
             if (on[r]) {
                 key[r] = s_key[i];
@@ -162,20 +208,23 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_small_kernel(const ID* __re
         }
     }
 #pragma unroll
-    for (int r = 0; r < SORT_ITEMS; ++r) {
+    for (int r = 0; r < ITEMS; ++r) {
         const int i = wave * 64 * items + r * 64 + lane;
-        if (on[r]) {
-            keys[i] = key[r];
-            vals[i] = val[r];
-        }
+        if (on[r]) sorted[i] = uint2{key[r], val[r]};
     }
 }
 
 // More keys: per pass, the digits of every tile are counted, the counts summed over the tiles in front, and the tiles
-// ranked and scattered.  table: [tiles][digits], then [digits] totals.
+// ranked and scattered.  table: [tiles][digits], then [digits] totals.  With few tiles the scattering workgroups sum the
+// counts themselves (`summed` false): a launch less.
 template <class ID, bool FIRST>
-__global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const ID* __restrict__ ids, const unsigned* __restrict__ keys, int64_t n, int64_t V,
-                                                                  int64_t padding, int shift, int bits, unsigned* __restrict__ table) {
+__global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const ID* __restrict__ ids, const uint2* __restrict__ from, int64_t n, int64_t V,
+                                                                  int64_t padding, int shift, int bits, int tiles, unsigned* __restrict__ table,
+                                                                  char* __restrict__ clear, int64_t clear_bytes) {
+    if (FIRST && (int)blockIdx.x >= tiles) {
+        clear_table(clear, clear_bytes, blockIdx.x - tiles, gridDim.x - tiles);
+        return;
+    }
     __shared__ unsigned s_count[SORT_DIGITS];
     const int digits = 1 << bits;
     for (int i = threadIdx.x; i < digits; i += SORT_THREADS) s_count[i] = 0u;
@@ -184,7 +233,7 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const ID* __re
     for (int r = 0; r < SORT_ITEMS; ++r) {
         const int64_t i = base + r * SORT_THREADS + threadIdx.x;
         if (i < n) {
-            const unsigned key = FIRST ? sort_key(ids[i], V, padding) : keys[i];
+            const unsigned key = FIRST ? sort_key(ids[i], V, padding) : from[i].x;
             atomicAdd(&s_count[(key >> shift) & (digits - 1)], 1u);   // whole numbers: the order does not matter
         }
     }
@@ -219,216 +268,318 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_prefix_kernel(unsigned* __r
     }
 }
 
+// The tile is put in order in LDS first, so that neighbouring lanes write neighbouring places of the output.
 template <class ID, bool FIRST>
-__global__ __launch_bounds__(SORT_THREADS) void sort_scatter_kernel(const ID* __restrict__ ids, const unsigned* __restrict__ keys, const unsigned* __restrict__ vals,
-                                                                    int64_t n, int64_t V, int64_t padding, int shift, int bits, const unsigned* __restrict__ table,
-                                                                    int tiles, unsigned* __restrict__ keys_out, unsigned* __restrict__ vals_out) {
+__global__ __launch_bounds__(SORT_THREADS) void sort_scatter_kernel(const ID* __restrict__ ids, const uint2* __restrict__ from, int64_t n, int64_t V, int64_t padding,
+                                                                    int shift, int bits, const unsigned* __restrict__ table, int tiles, bool summed,
+                                                                    uint2* __restrict__ to) {
     __shared__ unsigned s_count[SORT_WAVES][SORT_DIGITS];
     __shared__ unsigned s_to[SORT_DIGITS];   // what a rank in the sorted tile lacks to its place in the output, per digit
     __shared__ unsigned s_wave[SORT_WAVES];
+    __shared__ uint2 s_pair[SORT_TILE];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, digits = 1 << bits;
-    const int64_t base = (int64_t)blockIdx.x * SORT_TILE + wave * 64 * SORT_ITEMS;
-    unsigned key[SORT_ITEMS], rank[SORT_ITEMS];
+    const int64_t tile = (int64_t)blockIdx.x * SORT_TILE;
+    unsigned key[SORT_ITEMS], val[SORT_ITEMS], rank[SORT_ITEMS];
     bool on[SORT_ITEMS];
 #pragma unroll
     for (int r = 0; r < SORT_ITEMS; ++r) {
-        const int64_t i = base + r * 64 + lane;
+        const int64_t i = tile + (wave * SORT_ITEMS + r) * 64 + lane;
         on[r] = i < n;
-        key[r] = on[r] ? (FIRST ? sort_key(ids[i], V, padding) : keys[i]) : 0u;
+        key[r] = val[r] = 0u;
+        if (on[r]) {
+            if (FIRST) {
+                key[r] = sort_key(ids[i], V, padding);
+                val[r] = (unsigned)i;
+            } else {
+                const uint2 pair = from[i];
+                key[r] = pair.x;
+                val[r] = pair.y;
+            }
+        }
     }
-    for (int i = threadIdx.x; i < SORT_WAVES * SORT_DIGITS; i += SORT_THREADS) (&s_count[0][0])[i] = 0u;
+    // where the digit starts in the whole output, and what the tiles in front hold of it
+    unsigned total = 0, front = 0;
+    if ((int)threadIdx.x < digits) {
+        if (summed) {
+            total = table[(int64_t)tiles * digits + threadIdx.x];
+            front = table[(int64_t)blockIdx.x * digits + threadIdx.x];
+        } else {
+#pragma unroll 8
+            for (int t = 0; t < tiles; ++t) {
+                const unsigned n_t = table[(int64_t)t * digits + threadIdx.x];
+                total += n_t;
+                front += t < (int)blockIdx.x ? n_t : 0u;
+            }
+        }
+    }
+    clear_counts(s_count, digits);
     __syncthreads();
-    rank_in_wave(key, on, shift, bits, s_count[wave], rank);
+    rank_in_wave(key, on, shift, bits, s_count, rank);
     __syncthreads();
     unsigned start;
-    digit_starts(s_count, s_wave, start);
-    // where the digit starts in the whole output, and what the tiles in front hold of it
-    const unsigned total = (int)threadIdx.x < digits ? table[(int64_t)tiles * digits + threadIdx.x] : 0u;
+    digit_starts(s_count, s_wave, digits, start);
     const unsigned first = block_exclusive(total, s_wave);
-    if ((int)threadIdx.x < digits) s_to[threadIdx.x] = first + table[(int64_t)blockIdx.x * digits + threadIdx.x] - start;
+    if ((int)threadIdx.x < digits) s_to[threadIdx.x] = first + front - start;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < SORT_ITEMS; ++r)
+        if (on[r]) s_pair[s_count[wave][(key[r] >> shift) & (unsigned)(digits - 1)] + rank[r]] = uint2{key[r], val[r]};
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < SORT_ITEMS; ++r) {
-        if (on[r]) {
-            const unsigned d = (key[r] >> shift) & (unsigned)(digits - 1);
-            const unsigned to = s_count[wave][d] + rank[r] + s_to[d];
-            const int64_t i = base + r * 64 + lane;
-            keys_out[to] = key[r];
-            vals_out[to] = FIRST ? (unsigned)i : vals[i];
+        const int i = r * SORT_THREADS + (int)threadIdx.x;
+        if (tile + i < n) {
+            const uint2 pair = s_pair[i];
+            to[(unsigned)i + s_to[(pair.x >> shift) & (unsigned)(digits - 1)]] = pair;
         }
     }
 }
 
 // ---- sums over the runs --------------------------------------------------------------------------------------------
-// Lanes of a group on one row: LR lanes of VEC elements, column tile blockIdx.y.
-template <int VEC>
-struct RowLanes {
-    int lanes, group, c;
-    bool on;
-    int64_t col;
-    __device__ __forceinline__ RowLanes(int l_lanes, int D) {
-        lanes = 1 << l_lanes;
-        group = threadIdx.x >> l_lanes;
-        c = threadIdx.x & (lanes - 1);
-        const int64_t v = (int64_t)blockIdx.y * lanes + c;
-        col = v * VEC;
-        on = col < D;
-    }
+struct EmbSums {
+    const uint2* sorted;    // (id, position) in the order of the ids
+    int64_t N, V;
+    int D, l_lanes;         // log2 of the lanes on a row
+    int l_chunk;            // log2 of the positions of a chunk
+    int col_tiles;          // column tiles of a row: 64 lanes cover one
+    int64_t chunks;
+    int join_chunks;        // chunks whose crossing runs one workgroup of the join looks after
+    float scale;
+    float* part;            // [chunks][2][D]: the stretch of the run that comes in from the chunk in front, and of the run that starts here and goes on
 };
 
-template <class T, int VEC>
-__device__ __forceinline__ void add_row(const T* __restrict__ d_out, int64_t row, int D, int64_t col, float (&sum)[VEC]) {
-    float v[VEC];
-    load_run<VEC>(d_out + row * D + col, v);
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) sum[k] += v[k];
-}
+// A wave holds 64 / lanes sorted positions at a time, one per group of lanes, and adds them up by a scan that stops where
+// the id changes; what the last group holds is carried into the next round.  The rows of ROUNDS rounds are under way at
+// once.  WHOLE: all 64 lanes on one row -- the id is the wave's, and nothing changes lanes.
+template <class T, int VEC, bool WHOLE>
+__global__ __launch_bounds__(256) void embedding_sums_kernel(EmbSums p, const T* __restrict__ d_out, T* __restrict__ d_table) {
+    constexpr int ROUNDS = 8;
+    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), chunk = id / p.col_tiles;
+    if (chunk >= p.chunks) return;
+    const int l_lanes = WHOLE ? 6 : p.l_lanes;
+    const int lane = threadIdx.x & 63, lanes = 1 << l_lanes, groups = 64 >> l_lanes, group = lane >> l_lanes, c = lane & (lanes - 1);
+    const int64_t col = ((id - chunk * p.col_tiles) * lanes + c) * VEC;
+    const bool on = col < p.D;
+    const int64_t base = chunk << p.l_chunk, end = min(base + (1ll << p.l_chunk), p.N);
+    const unsigned before = base > 0 ? p.sorted[base - 1].x : NO_KEY, after = end < p.N ? p.sorted[end].x : NO_KEY;
+    const unsigned V = (unsigned)p.V;
+    float* __restrict__ part = p.part + chunk * 2 * p.D + col;
 
-template <class T, int VEC>
-__global__ __launch_bounds__(256) void embedding_partial_kernel(const T* __restrict__ d_out, int D, const unsigned* __restrict__ keys,
-                                                                const unsigned* __restrict__ vals, int64_t chunks, unsigned V, int l_lanes,
-                                                                float* __restrict__ part) {
-    const int64_t chunk = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (chunk >= chunks) return;
-    const unsigned key = keys[chunk * EMB_CHUNK];
-    if (key >= V || keys[chunk * EMB_CHUNK + EMB_CHUNK - 1] != key) return;
-    const int lane = threadIdx.x & 63;
-    const RowLanes<VEC> w(l_lanes, D);
-    const int groups = 64 >> l_lanes, group = lane >> l_lanes;
-    float sum[VEC];
+    const auto write = [&](unsigned key, const float (&v)[VEC], bool goes_on) {
+        if (!on) return;
+        if (key == before) {
+            store_run<VEC>(part, v);
+        } else if (goes_on) {
+            store_run<VEC>(part + p.D, v);
+        } else {
+            float out[VEC];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) sum[k] = 0.0f;
-#pragma unroll 4
-    for (int i = group; i < EMB_CHUNK; i += groups) {
-        if (w.on) add_row<T, VEC>(d_out, vals[chunk * EMB_CHUNK + i], D, w.col, sum);
-    }
-    for (int d = w.lanes; d < 64; d <<= 1)
+            for (int k = 0; k < VEC; ++k) out[k] = v[k] * p.scale;
+            store_run<VEC>(d_table + (int64_t)key * p.D + col, out);
+        }
+    };
+
+    unsigned carry_key = NO_KEY;
+    float carry[VEC];
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) sum[k] += __shfl_xor(sum[k], d, 64);
-    if (group == 0 && w.on) store_run<VEC>(part + chunk * D + w.col, sum);
-}
-
-__device__ __forceinline__ int64_t lower_bound(const unsigned* __restrict__ keys, int64_t n, unsigned key) {
-    int64_t lo = 0, hi = n;
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (keys[mid] < key) lo = mid + 1;
-        else hi = mid;
-    }
-    return lo;
-}
-
-// Blocks [0, long_blocks): the long runs whose first aligned position is one of the block's candidates.
-// The others: `rows` rows each.
-template <class T, int VEC>
-__global__ __launch_bounds__(256) void embedding_rows_kernel(const T* __restrict__ d_out, int D, const unsigned* __restrict__ keys,
-                                                             const unsigned* __restrict__ vals, int64_t N, int64_t V, float scale, int l_lanes, int rows,
-                                                             int64_t long_blocks, const float* __restrict__ part, T* __restrict__ d_table) {
-    __shared__ int64_t s_lo[257];
-    __shared__ float s_sum[256 * VEC];
-    const RowLanes<VEC> w(l_lanes, D);
-    const int groups = 256 >> l_lanes;
-    if ((int64_t)blockIdx.x < long_blocks) {
-        if (threadIdx.x < EMB_CANDIDATES) {
-            const int64_t at = ((int64_t)blockIdx.x * EMB_CANDIDATES + threadIdx.x) * EMB_CHUNK;
-            int64_t lo = -1, hi = -1;
-            // a run of EMB_LONG that starts in the chunk before `at` or at it holds the whole chunk from `at` on
-            if (at + EMB_CHUNK <= N) {
-                const unsigned key = keys[at];
-                if (key < (unsigned)V && keys[at + EMB_CHUNK - 1] == key && (at == 0 || keys[at - EMB_CHUNK] != key)) {
-                    lo = lower_bound(keys, at, key);
-                    hi = at + lower_bound(keys + at, N - at, key + 1u);
-                    if (hi - lo < EMB_LONG) lo = -1;
+    for (int k = 0; k < VEC; ++k) carry[k] = 0.0f;
+    for (int64_t at = base; at < end; at += ROUNDS * groups) {
+        unsigned key[ROUNDS];
+        float row[ROUNDS][VEC];
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) {
+            const int64_t i = at + r * groups + group;
+            uint2 pair{NO_KEY, 0u};
+            if (i < end) pair = p.sorted[i];
+            key[r] = pair.x >= V ? NO_KEY : pair.x;   // ids that take no gradient
+            if (WHOLE) key[r] = (unsigned)__builtin_amdgcn_readfirstlane((int)key[r]);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) row[r][k] = 0.0f;
+            if (on && key[r] != NO_KEY) load_run<VEC>(d_out + (int64_t)pair.y * p.D + col, row[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) {
+            if (at + r * groups >= end) break;
+            const unsigned k = key[r];
+            if (WHOLE) {
+                if (k != carry_key) {
+                    if (carry_key != NO_KEY) write(carry_key, carry, false);
+                    carry_key = k;
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) carry[q] = row[r][q];
+                } else {
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) carry[q] += row[r][q];
+                }
+                continue;
+            }
+            float v[VEC];
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) v[q] = row[r][q];
+            for (int d = 1; d < groups; d <<= 1) {
+                const bool take = __shfl_up(k, d << l_lanes, 64) == k && group >= d;
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) {
+                    const float o = __shfl_up(v[q], d << l_lanes, 64);
+                    if (take) v[q] += o;
                 }
             }
-            s_lo[threadIdx.x] = lo;
-            s_lo[EMB_CANDIDATES + threadIdx.x] = hi;
+            if (carry_key != NO_KEY && __shfl(k, c, 64) != carry_key && group == 0) write(carry_key, carry, false);   // it ended with the last round
+            if (k == carry_key) {
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) v[q] += carry[q];
+            }
+            const unsigned next = __shfl_down(k, lanes, 64);
+            if (group + 1 < groups && next != k && k != NO_KEY) write(k, v, false);
+            const int last = 64 - lanes + c;
+            carry_key = __shfl(k, last, 64);
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) carry[q] = __shfl(v[q], last, 64);
         }
-        __syncthreads();
-        for (int q = 0; q < EMB_CANDIDATES; ++q) {
-            const int64_t lo = s_lo[q], hi = s_lo[EMB_CANDIDATES + q];
-            if (lo < 0) continue;
-            const int64_t first = (lo + EMB_CHUNK - 1) / EMB_CHUNK, last = hi / EMB_CHUNK;   // whole chunks
-            const int64_t head = first * EMB_CHUNK - lo, tail = hi - last * EMB_CHUNK;
+    }
+    if (carry_key != NO_KEY && group == 0) write(carry_key, carry, carry_key == after);
+}
+
+// The runs that cross chunks: a run belongs to the chunk that it starts in.  Those over a few chunks are joined by a
+// group of lanes each, longer ones by the whole workgroup.
+template <class T, int VEC>
+__global__ __launch_bounds__(JOIN_THREADS) void embedding_join_kernel(EmbSums p, T* __restrict__ d_table) {
+    constexpr int FEW = 8;
+    __shared__ int s_over[JOIN_CHUNKS];       // chunks that the run goes on over, FEW: at least so many; 0: none starts here
+    __shared__ unsigned s_key[JOIN_CHUNKS];
+    __shared__ int s_count[JOIN_THREADS / 64];
+    __shared__ float s_sum[JOIN_THREADS * VEC];
+    const int64_t first = (int64_t)blockIdx.x * p.join_chunks;
+    // a run goes on into a chunk that starts with its id
+    const auto start_key = [&](int64_t chunk) { return chunk < p.chunks ? p.sorted[chunk << p.l_chunk].x : NO_KEY; };
+    if ((int)threadIdx.x < p.join_chunks) {
+        const int64_t chunk = first + threadIdx.x, end = (chunk + 1) << p.l_chunk;
+        int over = 0;
+        if (end < p.N) {
+            const unsigned key = p.sorted[end - 1].x, next = p.sorted[end].x, before = chunk == 0 ? NO_KEY : p.sorted[(chunk << p.l_chunk) - 1].x;
+            unsigned starts[FEW - 1];
+#pragma unroll
+            for (int k = 0; k < FEW - 1; ++k) starts[k] = start_key(chunk + 2 + k);
+            if (key < (unsigned)p.V && next == key && before != key) {
+                over = 1;
+#pragma unroll
+                for (int k = 0; k < FEW - 1; ++k) over += over == k + 1 && starts[k] == key;
+            }
+            s_key[threadIdx.x] = key;
+        }
+        s_over[threadIdx.x] = over;
+    }
+    __syncthreads();
+    const int lanes = 1 << p.l_lanes, groups = JOIN_THREADS >> p.l_lanes, group = threadIdx.x >> p.l_lanes, c = threadIdx.x & (lanes - 1);
+    const int64_t col = ((int64_t)blockIdx.y * lanes + c) * VEC;
+    const bool on = col < p.D;
+    const float* __restrict__ part = p.part + col;
+    const auto add = [&](int64_t chunk, int64_t i, float (&sum)[VEC]) {
+        float v[VEC];
+        load_run<VEC>(part + (i * 2 + (i == chunk ? 1 : 0)) * p.D, v);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) sum[k] += v[k];
+    };
+    const auto finish = [&](unsigned key, float (&sum)[VEC]) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) sum[k] *= p.scale;
+        store_run<VEC>(d_table + (int64_t)key * p.D + col, sum);
+    };
+    if (on) {
+        for (int q = group; q < p.join_chunks; q += groups) {
+            const int over = s_over[q];
+            if (over == 0 || over == FEW) continue;
+            const int64_t chunk = first + q;
             float sum[VEC];
 #pragma unroll
             for (int k = 0; k < VEC; ++k) sum[k] = 0.0f;
-            if (w.on) {
 #pragma unroll 4
-                for (int64_t i = w.group; i < head + tail; i += groups)
-                    add_row<T, VEC>(d_out, vals[i < head ? lo + i : last * EMB_CHUNK + (i - head)], D, w.col, sum);
-#pragma unroll 8
-                for (int64_t i = first + w.group; i < last; i += groups) add_row<float, VEC>(part, i, D, w.col, sum);
-            }
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) s_sum[threadIdx.x * VEC + k] = sum[k];
-            __syncthreads();
-            if (w.group == 0 && w.on) {
-                for (int g = 1; g < groups; ++g)
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) sum[k] += s_sum[(g * w.lanes + w.c) * VEC + k];
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) sum[k] *= scale;
-                store_run<VEC>(d_table + (int64_t)keys[lo] * D + w.col, sum);
-            }
+            for (int64_t i = chunk; i <= chunk + over; ++i) add(chunk, i, sum);
+            finish(s_key[q], sum);
         }
-        return;
     }
-    const int64_t v0 = ((int64_t)blockIdx.x - long_blocks) * rows;
-    for (int i = threadIdx.x; i <= rows; i += 256) s_lo[i] = lower_bound(keys, N, (unsigned)min(v0 + i, V));
-    __syncthreads();
-    if (!w.on) return;
-    for (int q = w.group; q < rows && v0 + q < V; q += groups) {
-        const int64_t lo = s_lo[q], hi = s_lo[q + 1];
-        if (hi - lo >= EMB_LONG) continue;
+    for (int q = 0; q < p.join_chunks; ++q) {
+        if (s_over[q] != FEW) continue;
+        const int64_t chunk = first + q;
+        // the last chunk that the run goes on into, by JOIN_THREADS probes a round: in [lo, hi)
+        int64_t lo = chunk + FEW, hi = p.chunks;
+        while (hi - lo > 1) {
+            const int64_t step = (hi - lo - 1 + JOIN_THREADS - 1) / JOIN_THREADS, at = lo + (threadIdx.x + 1) * step;
+            const int in_wave = __popcll(__ballot(at < hi && start_key(at) == s_key[q]));
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0) s_count[threadIdx.x >> 6] = in_wave;
+            __syncthreads();
+            int through = 0;
+            for (int k = 0; k < JOIN_THREADS / 64; ++k) through += s_count[k];
+            lo += through * step;
+            hi = min(hi, lo + step);
+        }
+        const int64_t last = lo;
         float sum[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) sum[k] = 0.0f;
-#pragma unroll 4
-        for (int64_t i = lo; i < hi; ++i) add_row<T, VEC>(d_out, vals[i], D, w.col, sum);
+        if (on) {
+#pragma unroll 8
+            for (int64_t i = chunk + group; i <= last; i += groups) add(chunk, i, sum);
+        }
+        const int used = (int)min((int64_t)groups, last - chunk + 1);   // groups that hold something
+        __syncthreads();
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) sum[k] *= scale;
-        store_run<VEC>(d_table + (v0 + q) * D + w.col, sum);
+        for (int k = 0; k < VEC; ++k) s_sum[threadIdx.x * VEC + k] = sum[k];
+        __syncthreads();
+        if (group == 0 && on) {
+#pragma unroll 4
+            for (int g = 1; g < used; ++g)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) sum[k] += s_sum[(g * lanes + c) * VEC + k];
+            finish(s_key[q], sum);
+        }
     }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
+static int vector_of(int D, int size) {   // elements per lane: the widest power of two that divides a row, 16 bytes at most
+    int v = 16 / size;
+    while (D % v) v >>= 1;
+    return v;
+}
+
+static int lanes_log2(int vectors) {
+    int l = 0;
+    while (l < 6 && (1 << l) < vectors) ++l;
+    return l;
+}
+
 struct EmbWork {                       // the workspace, cut into arrays that start on 256-byte boundaries
     int passes, bits;
-    int64_t tiles, chunks;
-    size_t keys[2], vals[2], table, part, bytes;
+    int64_t tiles;
+    size_t pairs[2], table, part, bytes;
 };
+
+// log2 of the positions of a chunk: at least four rounds of a wave; long enough that the two partial rows of a chunk
+// (8 bytes an element, written and read) stay a small part of its rows' bytes
+static int chunk_log2(int l_lanes) { return std::max(5, 8 - l_lanes); }
 
 static EmbWork embedding_work(int64_t N, int64_t V, int D) {
     EmbWork w;
     int bits = 1;
     while ((1ll << bits) < V + 1) ++bits;
-    w.passes = (int)ceil_div(bits, SORT_BITS);
+    const bool small = N <= SMALL_TILE;
+    w.passes = (int)ceil_div(bits, small ? SMALL_BITS : SORT_BITS);
     w.bits = (int)ceil_div(bits, w.passes);
-    w.tiles = ceil_div(N, SORT_TILE);
-    w.chunks = N / EMB_CHUNK;
+    w.tiles = small ? 1 : ceil_div(N, SORT_TILE);
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t from = at;
         at += (bytes + 255) / 256 * 256;
         return from;
     };
-    for (int k = 0; k < 2; ++k) {
-        const bool used = k == 0 || w.tiles > 1;
-        w.keys[k] = take(used ? 4 * N : 0);
-        w.vals[k] = take(used ? 4 * N : 0);
-    }
-    w.table = take(w.tiles > 1 ? 4ull * (w.tiles + 1) << w.bits : 0);
-    w.part = take(N >= EMB_LONG ? 4ull * w.chunks * D : 0);
+    w.pairs[0] = take(8 * N);
+    w.pairs[1] = take(small ? 0 : 8 * N);
+    w.table = take(small ? 0 : 4ull * (w.tiles + 1) << w.bits);
+    w.part = take(N > 32 ? 8ull * D * (size_t)ceil_div(N, 32) : 0);   // chunks hold 32 positions or more
     w.bytes = at;
     return w;
-}
-
-static int vector_of(int D, int size) {   // elements per lane: the widest power of two that divides a row, 16 bytes at most
-    int v = 16 / size;
-    while (D % v) v >>= 1;
-    return v;
 }
 
 // f(integral_constant VEC) for the vector that a row of D elements of T allows
@@ -441,34 +592,39 @@ static int with_vector(int D, F&& f) {
     return f(std::integral_constant<int, sizeof(T) == 4 ? 4 : 8>{});
 }
 
-static int lanes_log2(int vectors) {
-    int l = 0;
-    while (l < 6 && (1 << l) < vectors) ++l;
-    return l;
-}
-
 template <class T, class ID>
 static int embedding_fwd_typed(const T* table, int64_t V, int D, const ID* ids, int64_t N, float scale, T* out, hipStream_t stream) {
     return with_vector<T>(D, [&](auto vec) {
         constexpr int VEC = decltype(vec)::value;
         const int l = lanes_log2(D / VEC);
-        const int64_t blocks = std::min<int64_t>(ceil_div(N, 256 >> l), 1 << 20);   // a launch holds fewer than 2^32 threads
-        // few rows: their columns are spread over workgroups too
-        const int wide = (int)std::min<int64_t>(ceil_div(D / VEC, 1 << l), std::max<int64_t>(1, ceil_div(1024, blocks)));
-        hipLaunchKernelGGL((embedding_fwd_kernel<T, VEC, ID>), dim3((unsigned)blocks, wide), dim3(256), 0, stream, table, V, D, ids, N, scale, l, out);
-        return check_launch("nerf_embedding_fwd");
+        const auto launch = [&](auto rows) {
+            constexpr int ROWS = decltype(rows)::value;
+            const int64_t blocks = std::min<int64_t>(ceil_div(N, (256 >> l) * ROWS), 1 << 20);   // a launch holds fewer than 2^32 threads
+            // few rows: their columns are spread over workgroups too
+            const int wide = (int)std::min<int64_t>(ceil_div(D / VEC, 1 << l), std::max<int64_t>(1, ceil_div(1024, blocks)));
+            hipLaunchKernelGGL((embedding_fwd_kernel<T, VEC, ID, ROWS>), dim3((unsigned)blocks, wide), dim3(256), 0, stream, table, V, D, ids, N, scale, l, out);
+            return check_launch("nerf_embedding_fwd");
+        };
+        // four rows a group once that still leaves four workgroups to a compute unit
+        return N >= 4 * 1024ll * (256 >> l) ? launch(std::integral_constant<int, 4>{}) : launch(std::integral_constant<int, 1>{});
     });
 }
 
 template <class ID>
-static int embedding_sort(const ID* ids, int64_t N, int64_t V, int64_t padding, const EmbWork& w, char* work, const unsigned** keys, const unsigned** vals,
-                          hipStream_t stream) {
-    unsigned* k[2] = {reinterpret_cast<unsigned*>(work + w.keys[0]), reinterpret_cast<unsigned*>(work + w.keys[1])};
-    unsigned* v[2] = {reinterpret_cast<unsigned*>(work + w.vals[0]), reinterpret_cast<unsigned*>(work + w.vals[1])};
+static int embedding_sort(const ID* ids, int64_t N, int64_t V, int64_t padding, const EmbWork& w, char* work, char* clear, int64_t clear_bytes,
+                          const uint2** sorted, hipStream_t stream) {
+    // workgroups that clear: 16 KB each while that leaves them one to a compute unit or fewer, then more
+    const int clearing = (int)std::min<int64_t>(1024, ceil_div(clear_bytes, 16384));
+    uint2* pairs[2] = {reinterpret_cast<uint2*>(work + w.pairs[0]), reinterpret_cast<uint2*>(work + w.pairs[1])};
     if (w.tiles <= 1) {
-        hipLaunchKernelGGL((sort_small_kernel<ID>), dim3(1), dim3(SORT_THREADS), 0, stream, ids, (int)N, V, padding, w.passes, w.bits, k[0], v[0]);
-        *keys = k[0];
-        *vals = v[0];
+        const auto launch = [&](auto items) {
+            hipLaunchKernelGGL((sort_small_kernel<ID, decltype(items)::value>), dim3(1 + clearing), dim3(SORT_THREADS), 0, stream, ids, (int)N, V, padding, w.passes,
+                               w.bits, pairs[0], clear, clear_bytes);
+        };
+        if (N <= SORT_THREADS) launch(std::integral_constant<int, 1>{});
+        else if (N <= 4 * SORT_THREADS) launch(std::integral_constant<int, 4>{});
+        else launch(std::integral_constant<int, SMALL_ITEMS>{});
+        *sorted = pairs[0];
         return check_launch("nerf_embedding_bwd(sort)");
     }
     unsigned* table = reinterpret_cast<unsigned*>(work + w.table);
@@ -476,46 +632,50 @@ static int embedding_sort(const ID* ids, int64_t N, int64_t V, int64_t padding, 
     for (int p = 0; p < w.passes; ++p) {
         const int to = p == 0 ? 0 : 1 - from, shift = p * w.bits;
         const dim3 grid((unsigned)w.tiles), block(SORT_THREADS);
-        if (p == 0) hipLaunchKernelGGL((sort_count_kernel<ID, true>), grid, block, 0, stream, ids, nullptr, N, V, padding, shift, w.bits, table);
-        else hipLaunchKernelGGL((sort_count_kernel<ID, false>), grid, block, 0, stream, ids, k[from], N, V, padding, shift, w.bits, table);
-        hipLaunchKernelGGL(sort_prefix_kernel, dim3((unsigned)ceil_div(1 << w.bits, 64)), block, 0, stream, table, (int)w.tiles, 1 << w.bits);
         if (p == 0)
-            hipLaunchKernelGGL((sort_scatter_kernel<ID, true>), grid, block, 0, stream, ids, nullptr, nullptr, N, V, padding, shift, w.bits, table, (int)w.tiles,
-                               k[to], v[to]);
+            hipLaunchKernelGGL((sort_count_kernel<ID, true>), dim3((unsigned)(w.tiles + clearing)), block, 0, stream, ids, (const uint2*)nullptr, N, V, padding, shift, w.bits,
+                               (int)w.tiles, table, clear, clear_bytes);
         else
-            hipLaunchKernelGGL((sort_scatter_kernel<ID, false>), grid, block, 0, stream, ids, k[from], v[from], N, V, padding, shift, w.bits, table,
-                               (int)w.tiles, k[to], v[to]);
+            hipLaunchKernelGGL((sort_count_kernel<ID, false>), grid, block, 0, stream, ids, (const uint2*)pairs[from], N, V, padding, shift, w.bits,
+                               (int)w.tiles, table, (char*)nullptr, int64_t(0));
+        const bool summed = w.tiles > SORT_FEW_TILES;
+        if (summed)
+            hipLaunchKernelGGL(sort_prefix_kernel, dim3((unsigned)ceil_div(1 << w.bits, 64)), block, 0, stream, table, (int)w.tiles, 1 << w.bits);
+        if (p == 0)
+            hipLaunchKernelGGL((sort_scatter_kernel<ID, true>), grid, block, 0, stream, ids, (const uint2*)nullptr, N, V, padding, shift, w.bits, table, (int)w.tiles,
+                               summed, pairs[to]);
+        else
+            hipLaunchKernelGGL((sort_scatter_kernel<ID, false>), grid, block, 0, stream, ids, (const uint2*)pairs[from], N, V, padding, shift, w.bits, table,
+                               (int)w.tiles, summed, pairs[to]);
         if (int rc = check_launch("nerf_embedding_bwd(sort)")) return rc;
         from = to;
     }
-    *keys = k[from];
-    *vals = v[from];
+    *sorted = pairs[from];
     return NERF_OK;
 }
 
 template <class T>
-static int embedding_sums(const T* d_out, int64_t N, int64_t V, int D, const unsigned* keys, const unsigned* vals, float scale, const EmbWork& w, char* work,
+static int embedding_sums(const T* d_out, int64_t N, int64_t V, int D, const uint2* sorted, float scale, const EmbWork& w, char* work,
                           T* d_table, hipStream_t stream) {
     return with_vector<T>(D, [&](auto vec) {
         constexpr int VEC = decltype(vec)::value;
-        const int l = lanes_log2(D / VEC);
-        const unsigned col_tiles = (unsigned)ceil_div(D / VEC, 1 << l);
-        float* part = reinterpret_cast<float*>(work + w.part);
-        int64_t long_blocks = 0;
-        if (N >= EMB_LONG) {
-            hipLaunchKernelGGL((embedding_partial_kernel<T, VEC>), dim3((unsigned)ceil_div(w.chunks, 4), col_tiles), dim3(256), 0, stream, d_out, D, keys, vals,
-                               w.chunks, (unsigned)V, l, part);
-            if (int rc = check_launch("nerf_embedding_bwd(partial)")) return rc;
-            long_blocks = ceil_div(w.chunks, EMB_CANDIDATES);
-        }
-        const int at_once = 256 >> l;
-        const int rounds = (int)std::max<int64_t>(1, std::min<int64_t>(256 / at_once, V * col_tiles / (2048ll * at_once)));
-        const int rows = at_once * rounds;
-        const int64_t blocks = long_blocks + ceil_div(V, rows);
-        NERF_REQUIRE(blocks < (1ll << 31), "nerf_embedding_bwd: too many workgroups");
-        hipLaunchKernelGGL((embedding_rows_kernel<T, VEC>), dim3((unsigned)blocks, col_tiles), dim3(256), 0, stream, d_out, D, keys, vals, N, V, scale, l, rows,
-                           long_blocks, part, d_table);
-        return check_launch("nerf_embedding_bwd(rows)");
+        EmbSums p;
+        p.sorted = sorted; p.N = N; p.V = V; p.D = D; p.scale = scale;
+        p.l_lanes = lanes_log2(D / VEC);
+        p.l_chunk = chunk_log2(p.l_lanes);
+        p.col_tiles = (int)ceil_div(D / VEC, 1 << p.l_lanes);
+        p.chunks = ceil_div(N, 1 << p.l_chunk);
+        p.join_chunks = std::min(JOIN_CHUNKS, 2 * (JOIN_THREADS >> p.l_lanes));
+        p.part = reinterpret_cast<float*>(work + w.part);
+        const int64_t blocks = ceil_div(p.chunks * p.col_tiles, 4);
+        NERF_REQUIRE(blocks < (1ll << 24), "nerf_embedding_bwd: too many workgroups");   // a launch holds fewer than 2^32 threads
+        if (p.l_lanes == 6) hipLaunchKernelGGL((embedding_sums_kernel<T, VEC, true>), dim3((unsigned)blocks), dim3(256), 0, stream, p, d_out, d_table);
+        else hipLaunchKernelGGL((embedding_sums_kernel<T, VEC, false>), dim3((unsigned)blocks), dim3(256), 0, stream, p, d_out, d_table);
+        if (int rc = check_launch("nerf_embedding_bwd(sums)")) return rc;
+        if (p.chunks <= 1) return NERF_OK;
+        hipLaunchKernelGGL((embedding_join_kernel<T, VEC>), dim3((unsigned)ceil_div(p.chunks, p.join_chunks), (unsigned)p.col_tiles), dim3(JOIN_THREADS), 0, stream, p,
+                           d_table);
+        return check_launch("nerf_embedding_bwd(join)");
     });
 }
 
@@ -563,15 +723,21 @@ extern "C" int nerf_embedding_bwd(const void* d_out, int type, const void* ids, 
     NERF_REQUIRE(aligned16(d_out) && aligned16(d_table) && aligned16(workspace), "%s: pointers must be 16-byte aligned", who);
     NERF_REQUIRE(workspace_bytes >= nerf_embedding_bwd_workspace_bytes(N, V, D) && (workspace || N == 0), "%s: workspace of %zu bytes, %zu needed", who,
                  workspace_bytes, nerf_embedding_bwd_workspace_bytes(N, V, D));
-    const EmbWork w = embedding_work(N, V, D);
-    const unsigned *keys = nullptr, *vals = nullptr;
-    if (N > 0) {
-        const int rc = ids_bytes == 8 ? embedding_sort(static_cast<const int64_t*>(ids), N, V, padding_idx, w, static_cast<char*>(workspace), &keys, &vals, (hipStream_t)stream)
-                                      : embedding_sort(static_cast<const int32_t*>(ids), N, V, padding_idx, w, static_cast<char*>(workspace), &keys, &vals, (hipStream_t)stream);
-        if (rc) return rc;
+    const int64_t clear_bytes = V * D * (type == NERF_F32 ? 4 : 2);
+    if (N == 0) {
+        hipLaunchKernelGGL(clear_kernel, dim3((unsigned)std::min<int64_t>(1024, ceil_div(clear_bytes, 16384))), dim3(1024), 0, (hipStream_t)stream,
+                           static_cast<char*>(d_table), clear_bytes);
+        return check_launch(who);
     }
+    const EmbWork w = embedding_work(N, V, D);
+    char* const work = static_cast<char*>(workspace);
+    char* const clear = static_cast<char*>(d_table);
+    const uint2* sorted = nullptr;
+    const int rc = ids_bytes == 8 ? embedding_sort(static_cast<const int64_t*>(ids), N, V, padding_idx, w, work, clear, clear_bytes, &sorted, (hipStream_t)stream)
+                                  : embedding_sort(static_cast<const int32_t*>(ids), N, V, padding_idx, w, work, clear, clear_bytes, &sorted, (hipStream_t)stream);
+    if (rc) return rc;
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        return embedding_sums(static_cast<const T*>(d_out), N, V, D, keys, vals, scale, w, static_cast<char*>(workspace), static_cast<T*>(d_table), (hipStream_t)stream);
+        return embedding_sums(static_cast<const T*>(d_out), N, V, D, sorted, scale, w, work, static_cast<T*>(d_table), (hipStream_t)stream);
     });
 }

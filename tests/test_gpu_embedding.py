@@ -16,6 +16,9 @@ def make_ids(kind, N, V, gen):
         return torch.full((N,), V // 2, dtype=torch.int64)
     if kind == "skewed":
         return (torch.pow(torch.tensor(V + 1.0, dtype=torch.float64), u).long() - 1).clamp_(0, V - 1)
+    if kind == "borders":    # runs of 1 to 10 chunks of any power of two from 32 to 256 positions, ending at their borders and one past
+        lengths = [(32 << (k % 4)) * (1 + k % 10) + (k % 3 == 2) - (k % 7 == 6) for k in range(V)]
+        return torch.repeat_interleave(torch.arange(V), torch.tensor(lengths))[:N][torch.randperm(N, generator=gen)]
     if kind == "runs":       # long runs of one id, then another, some rows never
         return ((torch.arange(N) * 7) // max(1, N) * 3) % V
     return (u * V).long().clamp_(0, V - 1)
@@ -33,7 +36,9 @@ def want_grad(ids, d_out, V, scale, pad):
     (1, 1, 1, "one"), (2, 63, 3, "uniform"), (40, 64, 32, "uniform"), (40, 65536, 32, "uniform"), (7, 127, 5, "runs"), (7, 128, 4, "one"), (9, 129, 8, "one"),
     (1023, 1000, 64, "skewed"), (1024, 8192, 16, "skewed"), (1025, 8193, 2, "uniform"), (70001, 20000, 100, "skewed"), (70001, 300, 520, "uniform"),
     (1100000, 100003, 2, "uniform"), (1100000, 9000, 1, "skewed"), (300, 30000, 65, "runs"), (3, 200000, 6, "one"), (524288, 262144, 2, "skewed"),
-    (50, 5000, 1024, "skewed"), (100, 777, 2056, "uniform"), (2049, 16384, 24, "one"), (300000, 65, 7, "uniform")])
+    (50, 5000, 1024, "skewed"), (100, 777, 2056, "uniform"), (2049, 16384, 24, "one"), (300000, 65, 7, "uniform"),
+    (700, 1024, 12, "skewed"), (700, 1025, 12, "skewed"), (90, 4096, 40, "uniform"), (90, 4097, 40, "uniform"), (70001, 16385, 3, "skewed"), (8, 16385, 260, "runs"),
+    (60, 28000, 2, "borders"), (60, 28000, 16, "borders"), (60, 28000, 48, "borders"), (30, 12000, 512, "borders"), (40, 16500, 1, "borders")])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_rows_and_exact_sums(dev, V, N, D, kind, dtype):
     from nerf_amd import ops
