@@ -14,6 +14,11 @@
 // recurrence from the other end, with the same products A.  h is recomputed from x and the state the tile was entered
 // with (kept in float by the forward pass): x costs the bytes that a saved h would, and h is not rounded on the way.
 //
+// Where there are few sequences and many steps the time axis is spread over workgroups as well, in one of two ways:
+// segments, whose (A, X) a pass of its own finds first; or, in the forward pass and with enough columns for it to keep the
+// memory busy, tiles in a chain, each of which finds the state it is entered with from what the tiles in front of it have
+// published: one pass over the data.
+//
 // Layout: x [B,T,C], gate [B,T,G]; the C/G = P channels of a gate are neighbours.  G = C: one "unit" of C columns per
 // batch entry; G < C: one unit of P columns per (batch entry, gate).  A workgroup of 256 threads is cut into groups of
 // CL x S threads: CL lanes side by side on the columns of a unit (VEC each), S slices of K steps.  Both passes are
@@ -29,6 +34,8 @@ constexpr int scan_steps(int gates) { return gates > 1 ? 4 : 8; }
 constexpr int SCAN_THREADS = 256;
 constexpr int SCAN_COLS = 64;      // most columns of a unit that one workgroup takes side by side
 constexpr int SCAN_WANT_BLOCKS = 1024;
+constexpr int CHAIN_GROUP = 32;    // tiles of the chain between two published states
+constexpr int CHAIN_BLOCKS = 8;    // fewest chains side by side
 
 struct ScanShape {
     int64_t B, T;
@@ -50,13 +57,13 @@ static int log2_up(int64_t n) {
 }
 
 // A function of the sizes alone: the backward pass finds the forward pass's tiles again.
-static ScanShape scan_shape(int64_t B, int64_t T, int C, int G) {
+static ScanShape scan_shape(int64_t B, int64_t T, int C, int G, int steps = 0) {
     ScanShape s;
     s.B = B; s.T = T; s.C = C; s.G = G;
     s.units_per_b = G == C ? 1 : G;
     s.P = C / s.units_per_b;
     s.vec = s.P % 4 == 0 ? 4 : 1;
-    s.steps = scan_steps(G == C ? s.vec : 1);
+    s.steps = steps ? steps : scan_steps(G == C ? s.vec : 1);
     s.lcl = log2_up(std::min<int64_t>(ceil_div(s.P, s.vec), SCAN_COLS / s.vec));
     s.ls = std::min(log2_up(ceil_div(T, s.steps)), 8 - s.lcl);
     s.col_tiles = (int)ceil_div(s.P, (int64_t)s.vec << s.lcl);
@@ -72,6 +79,31 @@ static ScanShape scan_shape(int64_t B, int64_t T, int C, int G) {
     return s;
 }
 
+// Steps per thread of the forward pass in a chain: long tiles, as many steps as the registers hold beside four workgroups on
+// a compute unit.
+constexpr int CHAIN_STEPS = 8, CHAIN_STEPS_16BIT = 16;
+// Whether the tiles of the forward pass form chains: a workgroup holds one tile of one chain, there are enough chains (a
+// chain advances by a group of tiles in about 4 us), and they are long enough to be worth clearing their words first.
+// 65536 steps of bfloat16 with float32 gates, chain against segments: 1024 channels (16 chains) 143 against 178 us, 512 (8)
+// 74 against 80, 256 (4) 68 against 47; 2048 of float32 359 against 526; 8 x 2048 x 1024 of bfloat16 25 against 35.
+static bool scan_chained(const ScanShape& s, int steps = CHAIN_STEPS) {
+    return s.segments > 1 && s.lcl + s.ls == 8 && s.blocks >= CHAIN_BLOCKS && s.T >= 4ll * ((int64_t)steps << s.ls);
+}
+
+// What a chain's tiles publish, in 8-byte words of a value and a mark: per workgroup column block and tile the (A, X) of
+// up to SCAN_COLS columns, per group of tiles the states it is entered with; and the next tile to take.
+struct ChainWork {
+    int64_t tickets, words, states, bytes;   // offsets
+};
+static ChainWork chain_work(const ScanShape& s) {
+    ChainWork w;
+    w.tickets = 0;
+    w.words = 128 * s.blocks;
+    w.states = w.words + s.blocks * s.tiles * (SCAN_COLS * 16);
+    w.bytes = w.states + s.blocks * ceil_div(s.tiles, CHAIN_GROUP) * (SCAN_COLS * 8);
+    return w;
+}
+
 struct ScanArgs {
     ScanShape s;
     const void* gate;
@@ -80,7 +112,11 @@ struct ScanArgs {
     int reverse, blend;
     void* h;
     float* last;           // [B,C] or null
-    float* carry;          // [tiles - 1][B,C]: the state every tile but the first is entered with; null: not kept
+    float* carry;          // [tiles - 1][B,C]: the state every tile (of the backward pass) but the first is entered with; null: not kept
+    int l_carry;           // log2 of that tile's steps
+    unsigned long long* chain_words;    // a chain's published (A, X), states and tickets
+    unsigned long long* chain_states;
+    unsigned* chain_tickets;
     float* agg;            // [2][segments][B,C]: A and X (backward: A and R) of the segments
     // backward
     const void* d_h;       // null: zeros
@@ -205,27 +241,32 @@ __device__ __forceinline__ void scan_wave(const ScanPlace<VEC>& w, float (&A)[VE
     }
 }
 
-// From the inclusive wave scan (A, X) and the state `carry` that the tile is entered with (the same in all slices of a
-// column): `in` = the state this slice is entered with, `carry` = the state the tile is left with.
-// s_a, s_x: [waves][SCAN_COLS] of this exchange's own, written here and read behind one barrier.
+// The waves' own (A, X) where a group has several: s_a, s_x [waves][SCAN_COLS] of this exchange's own, written here and
+// read behind the barrier.
+template <int VEC, bool UP>
+__device__ __forceinline__ void scan_exchange(const ScanPlace<VEC>& w, const float (&A)[VEC], const float (&X)[VEC], float (*s_a)[SCAN_COLS], float (*s_x)[SCAN_COLS]) {
+    if (w.NW == 1) return;
+    if (w.slw == (UP ? w.SW - 1 : 0)) {   // its inclusive value is the wave's
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            s_a[threadIdx.x >> 6][w.c * VEC + v] = A[v];
+            s_x[threadIdx.x >> 6][w.c * VEC + v] = X[v];
+        }
+    }
+    __syncthreads();
+}
+
+// From the inclusive wave scan (A, X), exchanged, and the state `carry` that the tile is entered with (the same in all
+// slices of a column): `in` = the state this slice is entered with, `carry` = the state the tile is left with.
 template <int VEC, bool UP>
 __device__ __forceinline__ void scan_carry(const ScanPlace<VEC>& w, const float (&A)[VEC], const float (&X)[VEC], float (&carry)[VEC], float (&in)[VEC],
                                            float (*s_a)[SCAN_COLS], float (*s_x)[SCAN_COLS]) {
-    const bool edge = UP ? w.slw == w.SW - 1 : w.slw == 0;   // its inclusive value is the wave's
     float from[VEC];
     if (w.NW > 1) {
-        const int wave = threadIdx.x >> 6;
-        if (edge) {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                s_a[wave][w.c * VEC + v] = A[v];
-                s_x[wave][w.c * VEC + v] = X[v];
-            }
-        }
-        __syncthreads();
-        const int mine = wave - w.first_wave;
+        const int mine = (threadIdx.x >> 6) - w.first_wave;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) from[v] = carry[v];
+#pragma unroll 1
         for (int n = 0; n < w.NW; ++n) {
             const int k = UP ? n : w.NW - 1 - n;
 #pragma unroll
@@ -249,6 +290,35 @@ __device__ __forceinline__ void scan_carry(const ScanPlace<VEC>& w, const float 
         const float px = UP ? __shfl_up(X[v], w.CL, 64) : __shfl_down(X[v], w.CL, 64);
         in[v] = first ? from[v] : scan_apply(pa, from[v], px);
     }
+}
+
+// The state a segment is entered with, from `carry` = what the recurrence starts from: the (A, X) of the segments in
+// front of it (UP) or behind it, a stretch of them per slice, joined like the slices of a tile.
+template <int VEC, bool UP>
+__device__ __forceinline__ void scan_fold(const ScanArgs& p, const ScanPlace<VEC>& w, int64_t seg, float (*s_a)[SCAN_COLS], float (*s_x)[SCAN_COLS], float (&carry)[VEC]) {
+    const int64_t first = UP ? 0 : seg + 1, n = UP ? seg : p.s.segments - 1 - seg, BC = p.s.B * p.s.C;
+    if (n == 0) return;
+    const int64_t per = (n + w.S - 1) >> p.s.ls, begin = w.sl * per, end = min(begin + per, n);
+    float A[VEC], X[VEC], in[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) { A[v] = 1.0f; X[v] = 0.0f; }
+    if (w.on) {
+#pragma unroll 4
+        for (int64_t i = begin; i < end; ++i) {
+            const int64_t k = first + (UP ? i : end - 1 - (i - begin));
+            float A_k[VEC], X_k[VEC];
+            load_run<VEC>(p.agg + k * BC + w.bc, A_k);
+            load_run<VEC>(p.agg + (p.s.segments + k) * BC + w.bc, X_k);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                X[v] = scan_apply(A_k[v], X[v], X_k[v]);
+                A[v] *= A_k[v];
+            }
+        }
+    }
+    scan_wave<VEC, UP>(w, A, X);
+    scan_exchange<VEC, UP>(w, A, X, s_a, s_x);
+    scan_carry<VEC, UP>(w, A, X, carry, in, s_a, s_x);
 }
 
 // (A, X) of the thread's K steps; x is multiplied by its weight first if the recurrence blends.
@@ -280,9 +350,134 @@ __device__ __forceinline__ void scan_local_back(const Steps<GT, GV, K>& a, const
         }
 }
 
+// ---- chains -----------------------------------------------------------------------------------------------------
+// The tiles of a chain are taken in order, by ticket, so that whatever a tile waits for belongs to tiles that have been
+// taken before it and are running or done: the first tile of a chain that is not done waits for nothing, and every wait
+// ends.  A tile publishes its (A, X); the last one of each group of CHAIN_GROUP publishes the state the next group is
+// entered with; so a state is at most CHAIN_GROUP - 1 compositions, always the same ones in the same order, behind a
+// published one, and the chain advances by groups and not by tiles.  A word carries its own mark beside the value: it is
+// read until the mark is there, and no order between words is needed.
+constexpr int CHAIN_PATIENCE = 1 << 20;   // reads of a word; a chain that is cut short by a fault elsewhere gives NaN and not a hang
+
+__device__ __forceinline__ void chain_put(unsigned long long* p, float v) {
+    __hip_atomic_store(p, 1ull << 32 | __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// Every read of a word that is not there yet goes to memory: they are kept few.  SLEEP: units of 64 clocks between reads.
+template <int N, int SLEEP>
+__device__ __forceinline__ void chain_get(const unsigned long long* p, int stride, float (&v)[N]) {
+    unsigned long long word[N];
+#pragma unroll 1
+    for (int spin = 0;; ++spin) {
+        bool there = true;
+#pragma unroll
+        for (int i = 0; i < N; ++i) word[i] = __hip_atomic_load(p + i * stride, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+        for (int i = 0; i < N; ++i) there = there && word[i] >> 32;
+        if (there) break;
+        if (spin == CHAIN_PATIENCE) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) word[i] = 0x7fc00000u;
+            break;
+        }
+        __builtin_amdgcn_s_sleep(SLEEP);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __uint_as_float((unsigned)word[i]);
+}
+
+__device__ __forceinline__ int64_t chain_ticket(const ScanArgs& p, int64_t chain) {
+    __shared__ unsigned s_ticket;
+    if (threadIdx.x == 0) s_ticket = atomicAdd(p.chain_tickets + chain * 32, 1u);
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane((int)s_ticket);   // the whole workgroup's: kept out of the vector registers
+}
+
+// Where a tile's words and its group's state lie.  Word i of a lane lies i * CL words on, so that the lanes of a slice read
+// and write whole lines: nothing of this is kept in a cache, and every line touched is a transfer of its own.
+template <int VEC>
+struct ChainPlace {
+    int64_t group;
+    int k;                        // place in the group
+    unsigned long long *words;    // of the group's first tile
+    unsigned long long *states;
+    __device__ __forceinline__ ChainPlace(const ScanArgs& p, const ScanPlace<VEC>& w, int64_t chain, int64_t order) {
+        group = order / CHAIN_GROUP;
+        k = (int)(order % CHAIN_GROUP);
+        words = p.chain_words + (chain * p.s.tiles + group * CHAIN_GROUP) * (2 * SCAN_COLS) + w.c;
+        states = p.chain_states + (chain * ((p.s.tiles + CHAIN_GROUP - 1) / CHAIN_GROUP) + group) * SCAN_COLS + w.c;
+    }
+};
+
+// Publishes the (A, X) of the order-th tile of the chain, which are also returned.  The waves' have been exchanged
+// through s_a and s_x.
+template <int VEC>
+__device__ __forceinline__ void chain_publish(const ScanArgs& p, const ScanPlace<VEC>& w, int64_t chain, int64_t order, float (*s_a)[SCAN_COLS], float (*s_x)[SCAN_COLS]) {
+    const ChainPlace<VEC> at(p, w, chain, order);
+    if (w.sl != 0 || at.k == CHAIN_GROUP - 1) return;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        float A = 1.0f, X = 0.0f;
+        for (int n = 0; n < w.NW; ++n) {
+            X = scan_apply(s_a[n][w.c * VEC + v], X, s_x[n][w.c * VEC + v]);
+            A *= s_a[n][w.c * VEC + v];
+        }
+        chain_put(at.words + at.k * (2 * SCAN_COLS) + 2 * v * w.CL, A);
+        chain_put(at.words + at.k * (2 * SCAN_COLS) + (2 * v + 1) * w.CL, X);
+    }
+}
+
+// `state`: what the recurrence starts from -> what this tile is entered with.  s_part is [CHAIN_GROUP][2][SCAN_COLS].
+template <int VEC>
+__device__ __forceinline__ void chain_state(const ScanArgs& p, const ScanPlace<VEC>& w, int64_t chain, int64_t order, float (*s_a)[SCAN_COLS], float (*s_x)[SCAN_COLS],
+                                            float (*s_part)[2][SCAN_COLS], float (&state)[VEC]) {
+    const ChainPlace<VEC> at(p, w, chain, order);
+    const int k = at.k, col = w.c * VEC;
+    const int64_t group = at.group;
+#pragma unroll 1
+    for (int q = w.sl; q < k; q += w.S) {
+        float ax[2 * VEC];
+        chain_get<2 * VEC, 8>(at.words + q * (2 * SCAN_COLS), w.CL, ax);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            s_part[q][0][col + v] = ax[2 * v];
+            s_part[q][1][col + v] = ax[2 * v + 1];
+        }
+    }
+    if (group > 0 && w.sl == w.S - 1) {   // the slice that has the fewest tiles to wait for
+        float h[VEC];
+        if (w.c == 0) {   // one lane waits
+            float first[1];
+            chain_get<1, 4>(at.states, 0, first);
+        }
+        chain_get<VEC, 4>(at.states, w.CL, h);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) s_part[CHAIN_GROUP - 1][0][col + v] = h[v];
+    }
+    __syncthreads();
+    if (group > 0) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) state[v] = s_part[CHAIN_GROUP - 1][0][col + v];
+    }
+#pragma unroll 2
+    for (int q = 0; q < k; ++q)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) state[v] = scan_apply(s_part[q][0][col + v], state[v], s_part[q][1][col + v]);
+    if (w.sl == 0 && k == CHAIN_GROUP - 1 && order + 1 < p.s.tiles) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            float h = state[v];
+#pragma unroll 1
+            for (int n = 0; n < w.NW; ++n) {
+                    h = scan_apply(s_a[n][col + v], h, s_x[n][col + v]);
+            }
+            chain_put(at.states + SCAN_COLS + v * w.CL, h);
+        }
+    }
+}
+
 // (A, X) of whole segments -- all but the last one -- or, BACK, (A, R) of all but the first.  Nothing is written per step,
 // so a slice takes one stretch of the segment and goes through it alone; the slices are joined once at the end.
-// Bound by the reads (65536 x 1024 bfloat16 with float32 gates: 402 MB at @@ TB/s).
+// Bound by the reads (65536 x 1024 bfloat16 with float32 gates: 402 MB at 4.5 TB/s, what reads alone reach here).
 template <class GT, class XT, int VEC, int GV, bool BACK>
 __global__ __launch_bounds__(SCAN_THREADS) void scan_segments_kernel(ScanArgs p) {
     constexpr int K = scan_steps(GV);
@@ -354,27 +549,21 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_segments_kernel(ScanArgs p)
     }
 }
 
-template <class GT, class XT, int VEC, int GV>
-__global__ __launch_bounds__(SCAN_THREADS) void scan_fwd_kernel(ScanArgs p) {
-    constexpr int K = scan_steps(GV);
-    __shared__ float s_a[2][4][SCAN_COLS], s_x[2][4][SCAN_COLS];
+template <class GT, class XT, int VEC, int GV, int K, bool CHAIN>
+__global__ __launch_bounds__(SCAN_THREADS, CHAIN ? 4 : 1) void scan_fwd_kernel(ScanArgs p) {
+    __shared__ float s_a[2][4][SCAN_COLS], s_x[2][4][SCAN_COLS], s_part[CHAIN ? CHAIN_GROUP : 1][2][SCAN_COLS];
     const ScanShape& s = p.s;
-    const int64_t seg = blockIdx.x / s.blocks, BC = s.B * s.C;
-    const ScanPlace<VEC> w(s, blockIdx.x % s.blocks);
-    const int64_t t_begin = seg * s.seg_tiles, t_end = min(t_begin + s.seg_tiles, s.tiles);
+    const int64_t block = blockIdx.x % s.blocks, BC = s.B * s.C;
+    const int64_t seg = CHAIN ? chain_ticket(p, block) : blockIdx.x / s.blocks;
+    const ScanPlace<VEC> w(s, block);
+    const int64_t t_begin = CHAIN ? seg : seg * s.seg_tiles, t_end = CHAIN ? seg + 1 : min(t_begin + s.seg_tiles, s.tiles);
     float carry[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) carry[v] = 0.0f;
     if (w.on) {
         if (p.state) load_run<VEC>(p.state + w.bc, carry);
-        for (int64_t k = 0; k < seg; ++k) {
-            float A[VEC], X[VEC];
-            load_run<VEC>(p.agg + k * BC + w.bc, A);
-            load_run<VEC>(p.agg + (s.segments + k) * BC + w.bc, X);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) carry[v] = scan_apply(A[v], carry[v], X[v]);
-        }
     }
+    if (!CHAIN) scan_fold<VEC, true>(p, w, seg, s_a[~t_begin & 1], s_x[~t_begin & 1], carry);
     const int64_t x_step = p.reverse ? -(int64_t)s.C : s.C, gate_step = p.reverse ? -(int64_t)s.G : s.G;
     Steps<GT, GV, K> a, a_next;
     Steps<XT, VEC, K> x, x_next;
@@ -386,7 +575,7 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_fwd_kernel(ScanArgs p) {
     };
     // the next tile is under way while this one is scanned -- where a thread holds few steps: with a shared gate it holds
     // twice as many, and the registers are worth more as a fourth workgroup on the compute unit
-    constexpr bool AHEAD = GV > 1;
+    constexpr bool AHEAD = GV > 1 && !CHAIN;
     if (AHEAD) fetch(t_begin, a_next, x_next);
     for (int64_t tile = t_begin; tile < t_end; ++tile) {
         if (AHEAD) {
@@ -398,11 +587,16 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_fwd_kernel(ScanArgs p) {
         }
         const int64_t i0 = tile * s.tile_steps + w.sl * K, at = w.at(s, i0, p.reverse);
         const int count = w.count(s, i0);
-        if (p.carry && tile > 0 && w.on && w.sl == 0) store_run<VEC>(p.carry + (tile - 1) * BC + w.bc, carry);
         float A[VEC], X[VEC], h[VEC];
         scan_local(a, x, p.blend, A, X);
         scan_wave<VEC, true>(w, A, X);
+        scan_exchange<VEC, true>(w, A, X, s_a[tile & 1], s_x[tile & 1]);
+        if (CHAIN) {
+            chain_publish<VEC>(p, w, block, tile, s_a[tile & 1], s_x[tile & 1]);
+            chain_state<VEC>(p, w, block, tile, s_a[tile & 1], s_x[tile & 1], s_part, carry);
+        }
         scan_carry<VEC, true>(w, A, X, carry, h, s_a[tile & 1], s_x[tile & 1]);
+        if (p.carry && count > 0 && i0 > 0 && (i0 & ((1 << p.l_carry) - 1)) == 0) store_run<VEC>(p.carry + ((i0 >> p.l_carry) - 1) * BC + w.bc, h);
         a.forget();
         x.forget();
         XT* __restrict__ out = static_cast<XT*>(p.h) + at;
@@ -419,6 +613,8 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_fwd_kernel(ScanArgs p) {
     if (p.last && t_end == s.tiles && w.on && w.sl == 0) store_run<VEC>(p.last + w.bc, carry);
 }
 
+// The time axis is spread by segments here.  (As a chain -- 16 KB of LDS, 168 registers, three workgroups on a compute unit
+// against four -- it took 340 us for 65536 x 1024 bfloat16 with float32 gates, the two kernels 303.)
 template <class GT, class XT, int VEC, int GV>
 __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
     constexpr int K = scan_steps(GV);
@@ -433,14 +629,8 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
     for (int v = 0; v < VEC; ++v) r_carry[v] = 0.0f;
     if (w.on) {
         if (p.d_last) load_run<VEC>(p.d_last + w.bc, r_carry);
-        for (int64_t k = s.segments - 1; k > seg; --k) {
-            float A[VEC], R[VEC];
-            load_run<VEC>(p.agg + k * BC + w.bc, A);
-            load_run<VEC>(p.agg + (s.segments + k) * BC + w.bc, R);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) r_carry[v] = scan_apply(A[v], r_carry[v], R[v]);
-        }
     }
+    scan_fold<VEC, false>(p, w, seg, s_b[t_end & 1], s_r[t_end & 1], r_carry);
     const int64_t x_step = p.reverse ? -(int64_t)s.C : s.C, gate_step = p.reverse ? -(int64_t)s.G : s.G;
     // (the next tile under way as in the forward pass was slower here: 151 registers against 119, 240 us against 215 for a
     // bfloat16 sequence of 65536 x 1024)
@@ -462,10 +652,12 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
         }
         scan_local(a, x, p.blend, A, X);
         scan_wave<VEC, true>(w, A, X);
+        scan_exchange<VEC, true>(w, A, X, s_a[tile & 1], s_x[tile & 1]);
         scan_carry<VEC, true>(w, A, X, carry, h, s_a[tile & 1], s_x[tile & 1]);
         a.forget();
         scan_local_back(a, dh, A, X);
         scan_wave<VEC, false>(w, A, X);
+        scan_exchange<VEC, false>(w, A, X, s_b[tile & 1], s_r[tile & 1]);
         scan_carry<VEC, false>(w, A, X, r_carry, r, s_b[tile & 1], s_r[tile & 1]);
         a.forget();
         x.forget();
@@ -508,7 +700,7 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
             }
         }
     }
-    if (p.d_state && seg == 0 && w.on && w.sl == 0) store_run<VEC>(p.d_state + w.bc, r_carry);
+    if (p.d_state && t_begin == 0 && w.on && w.sl == 0) store_run<VEC>(p.d_state + w.bc, r_carry);
 }
 
 // d_gate = the sum over the column tiles, in their order
@@ -523,8 +715,33 @@ __global__ __launch_bounds__(256) void scan_gate_sum_kernel(const float* __restr
 
 enum { SCAN_FWD, SCAN_BWD };
 
+__global__ __launch_bounds__(256) void chain_clear_kernel(uint4* __restrict__ p, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = uint4{0u, 0u, 0u, 0u};
+}
+
+template <class GT, class XT, int VEC, int GV, int K>
+static int scan_chain_launch(ScanArgs p, const char* who, hipStream_t stream) {
+    p.s = scan_shape(p.s.B, p.s.T, p.s.C, p.s.G, K);
+    const ChainWork work = chain_work(p.s);
+    char* const at = reinterpret_cast<char*>(p.agg);
+    p.chain_tickets = reinterpret_cast<unsigned*>(at + work.tickets);
+    p.chain_words = reinterpret_cast<unsigned long long*>(at + work.words);
+    p.chain_states = reinterpret_cast<unsigned long long*>(at + work.states);
+    hipLaunchKernelGGL(chain_clear_kernel, dim3((unsigned)std::min<int64_t>(2048, ceil_div(work.bytes, 4096))), dim3(256), 0, stream,
+                       reinterpret_cast<uint4*>(at), work.bytes / 16);
+    if (int rc = check_launch(who)) return rc;
+    hipLaunchKernelGGL((scan_fwd_kernel<GT, XT, VEC, GV, K, true>), dim3((unsigned)(p.s.blocks * p.s.tiles)), dim3(SCAN_THREADS), 0, stream, p);
+    return check_launch(who);
+}
+
 template <class GT, class XT, int VEC, int GV>
 static int scan_launch(const ScanArgs& p, int dir, const char* who, hipStream_t stream) {
+    if (dir == SCAN_FWD && scan_chained(p.s)) {
+        if constexpr (sizeof(XT) == 2 && (GV == 1 || sizeof(GT) == 2)) {
+            if (scan_chained(p.s, CHAIN_STEPS_16BIT)) return scan_chain_launch<GT, XT, VEC, GV, CHAIN_STEPS_16BIT>(p, who, stream);
+        }
+        return scan_chain_launch<GT, XT, VEC, GV, CHAIN_STEPS>(p, who, stream);
+    }
     const ScanShape& s = p.s;
     if (s.segments > 1) {
         const dim3 grid((unsigned)(s.blocks * (s.segments - 1)));
@@ -533,7 +750,7 @@ static int scan_launch(const ScanArgs& p, int dir, const char* who, hipStream_t 
         if (int rc = check_launch(who)) return rc;
     }
     const dim3 grid((unsigned)(s.blocks * s.segments));
-    if (dir == SCAN_FWD) hipLaunchKernelGGL((scan_fwd_kernel<GT, XT, VEC, GV>), grid, dim3(SCAN_THREADS), 0, stream, p);
+    if (dir == SCAN_FWD) hipLaunchKernelGGL((scan_fwd_kernel<GT, XT, VEC, GV, scan_steps(GV), false>), grid, dim3(SCAN_THREADS), 0, stream, p);
     else hipLaunchKernelGGL((scan_bwd_kernel<GT, XT, VEC, GV>), grid, dim3(SCAN_THREADS), 0, stream, p);
     if (int rc = check_launch(who)) return rc;
     if (dir == SCAN_BWD && p.d_gate && s.G != s.C && s.col_tiles > 1) {
@@ -558,6 +775,12 @@ static int scan_run(const ScanArgs& p, int gate_type, int x_type, int dir, const
     });
 }
 
+// Floats of the workspace that hold what the workgroups along the time axis tell each other (a multiple of 4).
+static size_t scan_states_floats(const ScanShape& s, bool backward) {
+    if (!backward && scan_chained(s)) return (size_t)chain_work(scan_shape(s.B, s.T, s.C, s.G, CHAIN_STEPS)).bytes / 4;
+    return s.segments > 1 ? (size_t)(2 * s.segments * ceil_div(s.B * s.C, 4) * 4) : 0;
+}
+
 static int scan_check(const char* who, int64_t B, int64_t T, int C, int G, int gate_type, int x_type) {
     NERF_REQUIRE(B >= 0 && T >= 0 && C >= 0 && G >= 0, "%s: B=%lld T=%lld C=%d G=%d", who, (long long)B, (long long)T, C, G);
     NERF_REQUIRE(C == 0 || (G > 0 && C % G == 0), "%s: %d gates do not divide %d channels", who, G, C);
@@ -566,7 +789,7 @@ static int scan_check(const char* who, int64_t B, int64_t T, int C, int G, int g
     NERF_REQUIRE(B <= (1ll << 40) && T <= (1ll << 40) && B * (double)T * C < 9e17, "%s: too large", who);
     const ScanShape s = scan_shape(B, T, C, G);
     // a launch holds fewer than 2^32 threads
-    NERF_REQUIRE(s.blocks * s.segments < (1ll << 24) && (s.col_tiles == 1 || B * (double)T * G < (double)(1ll << 32)), "%s: too many workgroups", who);
+    NERF_REQUIRE(s.blocks * (scan_chained(s) ? s.tiles : s.segments) < (1ll << 24) && (s.col_tiles == 1 || B * (double)T * G < (double)(1ll << 32)), "%s: too many workgroups", who);
     return NERF_OK;
 }
 
@@ -582,7 +805,7 @@ extern "C" size_t nerf_linear_scan_carry_floats(int64_t B, int64_t T, int C, int
 extern "C" size_t nerf_linear_scan_workspace_floats(int64_t B, int64_t T, int C, int G, int backward) {
     if (B <= 0 || T <= 0 || C <= 0 || G <= 0 || C % G) return 0;
     const ScanShape s = scan_shape(B, T, C, G);
-    size_t n = s.segments > 1 ? (size_t)(2 * s.segments * B * C) : 0;
+    size_t n = scan_states_floats(s, backward);
     if (backward && G != C && s.col_tiles > 1) n += (size_t)s.col_tiles * (size_t)(B * T * G);
     return n;
 }
@@ -599,6 +822,7 @@ extern "C" int nerf_linear_scan_fwd(const void* gate, int gate_type, const void*
                  "%s: pointers must be 16-byte aligned", who);
     ScanArgs p{};
     p.s = scan_shape(B, T, C, G);
+    p.l_carry = log2_up(p.s.tile_steps);
     NERF_REQUIRE(workspace || nerf_linear_scan_workspace_floats(B, T, C, G, 0) == 0, "%s: null workspace", who);
     p.gate = gate; p.x = x; p.state = state; p.reverse = reverse != 0; p.blend = blend != 0;
     p.h = h; p.last = last; p.carry = carry; p.agg = workspace;
@@ -618,12 +842,13 @@ extern "C" int nerf_linear_scan_bwd(const void* gate, int gate_type, const void*
                  "%s: pointers must be 16-byte aligned", who);
     ScanArgs p{};
     p.s = scan_shape(B, T, C, G);
+    p.l_carry = log2_up(p.s.tile_steps);
     NERF_REQUIRE(carry || p.s.tiles == 1, "%s: null carry (the forward pass keeps it)", who);
     NERF_REQUIRE(workspace || nerf_linear_scan_workspace_floats(B, T, C, G, 1) == 0, "%s: null workspace", who);
     p.gate = gate; p.x = x; p.state = state; p.reverse = reverse != 0; p.blend = blend != 0;
     p.carry = const_cast<float*>(carry);
     p.d_h = d_h; p.d_last = d_last; p.d_gate = d_gate; p.d_x = d_x; p.d_state = d_state;
     p.agg = workspace;
-    p.d_gate_part = workspace ? workspace + (p.s.segments > 1 ? 2 * p.s.segments * B * C : 0) : nullptr;
+    p.d_gate_part = workspace ? workspace + scan_states_floats(p.s, true) : nullptr;
     return scan_run(p, gate_type, x_type, SCAN_BWD, who, (hipStream_t)stream);
 }

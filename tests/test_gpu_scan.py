@@ -93,7 +93,7 @@ def check(dev, B, T, C, G, tx=F32, tg=None, reverse=False, blend=False, state=Fa
         assert_close(g, w, t, (name, (B, T, C, G), tx, tg, reverse, blend, state))
     with torch.no_grad():                      # the inference form: the same bits
         h2 = ops.linear_scan(*leaves, reverse=reverse, blend=blend)
-    assert torch.equal(h2, h)
+    assert torch.equal(h2, h)                  # (a chain's states do not depend on which tile waits for which)
     again = torch.autograd.grad(list(ops.linear_scan(*leaves, reverse=reverse, blend=blend, return_state=True)),
                                 [t for t in leaves if t is not None], [d_h.to(dev), d_last.to(dev)])
     assert all(torch.equal(a, b) for a, b in zip(grads, again))   # sums in a fixed order
@@ -117,7 +117,10 @@ def test_types(dev, tx, tg, reverse, blend, B, T, C, G):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("B,T,C,G", [(4099, 5, 3, 1), (700, 64, 1, 1), (300, 192, 3, 1), (9, 192, 3, 3), (130, 1, 260, 260), (1, 20000, 4, 4),
-                                     (1, 9000, 68, 1), (2, 1500, 520, 2), (1, 4097, 300, 1), (17, 100, 600, 600), (2, 40, 1030, 1)])
+                                     (1, 9000, 68, 1), (2, 1500, 520, 2), (1, 4097, 300, 1), (17, 100, 600, 600), (2, 40, 1030, 1),
+                                     # tiles in a chain: two, some, several groups of them; every way to lay out the lanes
+                                     (3, 70, 132, 132), (3, 600, 132, 132), (9, 1021, 100, 100), (2, 3000, 520, 520), (8, 2500, 64, 1), (8, 2500, 5, 1), (600, 5000, 1, 1), (8, 40000, 4, 4),
+                                     (4, 1021, 65, 65), (4, 700, 130, 2), (8, 9000, 12, 4)])
 def test_sizes(dev, B, T, C, G):
     check(dev, B, T, C, G, reverse=True, blend=True, state=True, seed=5)
 
