@@ -16,7 +16,6 @@ import time
 import torch
 
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), ".."))
-from nerf_amd import ops  # noqa: E402
 from nerf_amd.Camera import Camera  # noqa: E402
 from nerf_amd.models.NeRF import NeRF  # noqa: E402
 from nerf_amd.graph import GraphedStep  # noqa: E402
@@ -64,7 +63,7 @@ def main():
     model = NeRF().to(dev)
     fine = NeRF().to(dev) if args.importance else None
     params = list(model.parameters()) + (list(fine.parameters()) if fine else [])
-    opt = FusedAdam(params, lr=5e-4, capturable=args.graph)
+    opt = FusedAdam(params, lr=5e-4, capturable=args.graph, max_grad_norm=1.0)   # clips all gradients together as it reads them
     sched = torch.optim.lr_scheduler.ExponentialLR(opt, gamma=0.98)
     views = ring_views(dev, H, W, float(args.size), near, far, args.samples)
     z_lin = torch.linspace(near, far, args.samples).to(dev)
@@ -76,7 +75,6 @@ def main():
         out = render_rays(model, s_o, s_d, near, far, args.samples, z_lin=z_lin, fine_model=fine, n_importance=args.importance)
         loss = nerf_loss(out, s_img)       # MSE of the coarse colour, plus the fine colour's when there is a fine pass
         loss.backward()
-        ops.clip_grad_norm_(params, 1.0)
         opt.step()
         return loss, out["rgb_fine" if fine else "rgb"].detach()
 

@@ -8,7 +8,6 @@ from __future__ import annotations
 from typing import Optional, Sequence
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 
@@ -192,12 +191,48 @@ def hashgrid_debug(x: torch.Tensor, tables: Sequence[torch.Tensor], res: Sequenc
     return out, idx, w
 
 
+class _Once(torch.autograd.Function):
+    """Gradients that a kernel formed, as tensors whose own gradient nobody can ask for."""
+
+    @staticmethod
+    def forward(ctx, anchor, *formed):
+        return tuple(t.view_as(t) for t in formed)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("this operator of nerf_amd is differentiable once: its gradients have no gradient")
+
+
+def _once(*formed):
+    """The gradients of an operator that is differentiable once.  Where a graph of them is asked for (``create_graph``),
+    differentiating them raises, whatever they depend on; otherwise this does nothing."""
+    if not torch.is_grad_enabled():
+        return formed
+    there = [i for i, t in enumerate(formed) if t is not None]
+    if not there:
+        return formed
+    anchor = torch.empty(0, device=formed[there[0]].device, requires_grad=True)
+    tied = dict(zip(there, _Once.apply(anchor, *(formed[i] for i in there))))
+    return tuple(tied.get(i) for i in range(len(formed)))
+
+
 # ----------------------------------------------------------- embedding ----
 def _embedding_fwd(ids, table, scale):
     V, D = table.shape
     out = torch.empty(*ids.shape, D, device=table.device, dtype=table.dtype)
     L.launch("nerf_embedding_fwd", table, L.ptr(table), L.TYPES[table.dtype], V, D, L.ptr(ids), ids.element_size(), ids.numel(), scale, L.ptr(out))
     return out
+
+
+def _embedding_bwd(ids, d_out, V, D, scale, padding_idx):
+    """The table's gradient for dense ids and d_out."""
+    N = ids.numel()
+    nbytes = L.lib().nerf_embedding_bwd_workspace_bytes(N, V, D)
+    work = torch.empty(nbytes, device=d_out.device, dtype=torch.uint8) if nbytes else None
+    d_table = torch.empty(V, D, device=d_out.device, dtype=d_out.dtype)
+    L.launch("nerf_embedding_bwd", d_out, d_out.data_ptr(), L.TYPES[d_out.dtype], ids.data_ptr(), ids.element_size(), N, V, D, scale, padding_idx,
+             d_table.data_ptr(), L.ptr(work), nbytes)
+    return d_table
 
 
 class _Embedding(torch.autograd.Function):
@@ -207,22 +242,13 @@ class _Embedding(torch.autograd.Function):
     def forward(ctx, table, ids, scale, padding_idx):
         out = _embedding_fwd(ids, L.dense(table), scale)
         ctx.save_for_backward(ids)
-        ctx.meta = (tuple(table.shape), scale, padding_idx)
+        ctx.meta = (table.shape[0], table.shape[1], scale, padding_idx)
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d_out):
         (ids,) = ctx.saved_tensors
-        (V, D), scale, padding_idx = ctx.meta
-        d_out = L.dense(d_out)
-        N = ids.numel()
-        nbytes = L.lib().nerf_embedding_bwd_workspace_bytes(N, V, D)
-        work = torch.empty(nbytes, device=d_out.device, dtype=torch.uint8) if nbytes else None
-        d_table = torch.empty(V, D, device=d_out.device, dtype=d_out.dtype)
-        L.launch("nerf_embedding_bwd", d_out, L.ptr(d_out), L.TYPES[d_out.dtype], L.ptr(ids), ids.element_size(), N, V, D, scale, padding_idx,
-                 L.ptr(d_table), L.ptr(work), nbytes)
-        return d_table, None, None, None
+        return (*_once(_embedding_bwd(ids, L.dense(d_out.detach()), *ctx.meta)), None, None, None)
 
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
@@ -490,21 +516,20 @@ class _LinearScan(torch.autograd.Function):
         return h, last
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, d_h, d_last):
         gate, x, state, carry = ctx.saved_tensors
         B, T, C = x.shape
         G = gate.shape[2]
         need_gate, need_x, need_state = ctx.needs_input_grad[:3]
-        d_h, d_last = (None if t is None else L.dense(t) for t in (d_h, d_last))
-        d_gate = torch.empty_like(gate) if need_gate else None
+        d_h, d_last = (None if t is None else L.dense(t.detach()) for t in (d_h, d_last))
+        d_gate = torch.empty_like(gate) if need_gate else None   # (the saved tensors are dense)
         d_x = torch.empty_like(x) if need_x else None
         d_state = torch.empty_like(state) if need_state else None
         n = L.lib().nerf_linear_scan_workspace_floats(B, T, C, G, 1)
         work = torch.empty(n, device=x.device) if n else None
         L.launch("nerf_linear_scan_bwd", x, L.ptr(gate), L.TYPES[gate.dtype], L.ptr(x), L.TYPES[x.dtype], L.ptr(state), L.ptr(carry),
                  L.ptr(d_h), L.ptr(d_last), B, T, C, G, *ctx.meta, L.ptr(d_gate), L.ptr(d_x), L.ptr(d_state), L.ptr(work))
-        return d_gate, d_x, d_state, None, None, None
+        return (*_once(d_gate, d_x, d_state), None, None, None)
 
 
 def linear_scan(gate: torch.Tensor, x: torch.Tensor, state: Optional[torch.Tensor] = None, reverse: bool = False, blend: bool = False,

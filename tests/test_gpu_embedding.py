@@ -168,8 +168,8 @@ def test_shapes_strides_and_empty(dev):
     ops.embedding(torch.zeros(2, dtype=torch.long, device=dev), t).sum().backward()
     leaf = table.clone().requires_grad_(True)
     (g,) = torch.autograd.grad(ops.embedding(ids, leaf), leaf, torch.ones_like(want), create_graph=True)
-    with pytest.raises(RuntimeError):            # differentiable once
-        g.sum().backward()
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        (g.sum() + leaf.sum()).backward()
 
 
 @pytest.mark.gpu

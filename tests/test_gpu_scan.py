@@ -250,10 +250,14 @@ def test_empty_and_partial_gradients(dev):
     grads = torch.autograd.grad(ops.linear_scan(*leaves, return_state=True)[1], leaves, d_last.to(dev))
     for k in range(3):
         assert_close(grads[k], want[2 + k], tol[2 + k], k)
-    with pytest.raises(RuntimeError):         # differentiable once
-        leaves = [t.to(dev).requires_grad_(True) for t in (gate, x)]
-        (g,) = torch.autograd.grad(ops.linear_scan(*leaves).sum(), leaves[1], create_graph=True)
-        g.sum().backward()
+    # differentiable once: a graph of the gradients may be made, differentiating them raises -- also where the operator's
+    # part would be one term of several
+    leaves = [t.to(dev).requires_grad_(True) for t in (gate, x)]
+    plain = torch.autograd.grad(ops.linear_scan(*leaves).sum(), leaves)
+    tied = torch.autograd.grad(ops.linear_scan(*leaves).sum(), leaves, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, tied))
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        (tied[1].square().sum() + leaves[1].sum()).backward()
 
 
 @pytest.mark.gpu
