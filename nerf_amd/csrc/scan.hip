@@ -62,7 +62,7 @@ static ScanShape scan_shape(int64_t B, int64_t T, int C, int G, int steps = 0) {
     s.B = B; s.T = T; s.C = C; s.G = G;
     s.units_per_b = G == C ? 1 : G;
     s.P = C / s.units_per_b;
-    s.vec = s.P % 4 == 0 ? 4 : 1;
+    s.vec = s.P % 4 == 0 ? 4 : G != C && s.P <= 3 ? s.P : 1;   // colours: a lane takes all channels of its steps
     s.steps = steps ? steps : scan_steps(G == C ? s.vec : 1);
     s.lcl = log2_up(std::min<int64_t>(ceil_div(s.P, s.vec), SCAN_COLS / s.vec));
     s.ls = std::min(log2_up(ceil_div(T, s.steps)), 8 - s.lcl);
@@ -183,7 +183,7 @@ struct ScanPlace {
 // value is used two or three times, and kept as it is it takes half the registers where its type has 16 bits.
 template <class T, int N, int K>
 struct Steps {
-    static constexpr int WORDS = sizeof(T) * N < 4 ? 1 : sizeof(T) * N / 4;
+    static constexpr int WORDS = (sizeof(T) * N + 3) / 4;
     unsigned w[K][WORDS];
     __device__ __forceinline__ float operator()(int k, int v) const {
         if (N == 1) v = 0;   // one gate for all columns
@@ -198,12 +198,15 @@ struct Steps {
 #pragma unroll
             for (int v = 0; v < N; ++v) r.v[v] = (T)fill;
             if (k < count) r = *reinterpret_cast<const Run<T, N>*>(p + k * step);
-            if constexpr (sizeof(T) * N < 4) w[k][0] = __builtin_bit_cast(unsigned short, r);
-            else {
-                struct Words { unsigned w[WORDS]; };
-                const Words words = __builtin_bit_cast(Words, r);
+            if constexpr (sizeof(T) == 4) {
 #pragma unroll
-                for (int i = 0; i < WORDS; ++i) w[k][i] = words.w[i];
+                for (int i = 0; i < WORDS; ++i) w[k][i] = __builtin_bit_cast(unsigned, r.v[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < WORDS; ++i) {
+                    w[k][i] = __builtin_bit_cast(unsigned short, r.v[2 * i]);
+                    if (2 * i + 1 < N) w[k][i] |= (unsigned)__builtin_bit_cast(unsigned short, r.v[2 * i + 1 < N ? 2 * i + 1 : 0]) << 16;
+                }
             }
         }
     }
@@ -224,44 +227,48 @@ struct Steps {
     }
 };
 
+// Everywhere below: A [GV], one product for all VEC columns of a lane where they share a gate (GV = 1), else one each.
+template <int GV>
+__device__ __forceinline__ constexpr int scan_gate(int v) { return GV == 1 ? 0 : v; }
+
 // Inclusive scan of (A, X) over the slices that the wave holds of the group; UP: from the first slice, else from the last.
-template <int VEC, bool UP>
-__device__ __forceinline__ void scan_wave(const ScanPlace<VEC>& w, float (&A)[VEC], float (&X)[VEC]) {
+template <bool UP, int VEC, int GV>
+__device__ __forceinline__ void scan_wave(const ScanPlace<VEC>& w, float (&A)[GV], float (&X)[VEC]) {
     for (int d = 1; d < w.SW; d <<= 1) {
         const bool take = UP ? w.slw >= d : w.slw + d < w.SW;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            const float pa = UP ? __shfl_up(A[v], d * w.CL, 64) : __shfl_down(A[v], d * w.CL, 64);
             const float px = UP ? __shfl_up(X[v], d * w.CL, 64) : __shfl_down(X[v], d * w.CL, 64);
-            if (take) {
-                X[v] = scan_apply(A[v], px, X[v]);
-                A[v] *= pa;
-            }
+            if (take) X[v] = scan_apply(A[scan_gate<GV>(v)], px, X[v]);
+        }
+#pragma unroll
+        for (int g = 0; g < GV; ++g) {
+            const float pa = UP ? __shfl_up(A[g], d * w.CL, 64) : __shfl_down(A[g], d * w.CL, 64);
+            if (take) A[g] *= pa;
         }
     }
 }
 
 // The waves' own (A, X) where a group has several: s_a, s_x [waves][SCAN_COLS] of this exchange's own, written here and
 // read behind the barrier.
-template <int VEC, bool UP>
-__device__ __forceinline__ void scan_exchange(const ScanPlace<VEC>& w, const float (&A)[VEC], const float (&X)[VEC], float (*s_a)[SCAN_COLS], float (*s_x)[SCAN_COLS]) {
+template <bool UP, int VEC, int GV>
+__device__ __forceinline__ void scan_exchange(const ScanPlace<VEC>& w, const float (&A)[GV], const float (&X)[VEC], float (*s_a)[SCAN_COLS], float (*s_x)[SCAN_COLS]) {
     if (w.NW == 1) return;
     if (w.slw == (UP ? w.SW - 1 : 0)) {   // its inclusive value is the wave's
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            s_a[threadIdx.x >> 6][w.c * VEC + v] = A[v];
-            s_x[threadIdx.x >> 6][w.c * VEC + v] = X[v];
-        }
+        for (int g = 0; g < GV; ++g) s_a[threadIdx.x >> 6][w.c * VEC + g] = A[g];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) s_x[threadIdx.x >> 6][w.c * VEC + v] = X[v];
     }
     __syncthreads();
 }
 
 // From the inclusive wave scan (A, X), exchanged, and the state `carry` that the tile is entered with (the same in all
 // slices of a column): `in` = the state this slice is entered with, `carry` = the state the tile is left with.
-template <int VEC, bool UP>
-__device__ __forceinline__ void scan_carry(const ScanPlace<VEC>& w, const float (&A)[VEC], const float (&X)[VEC], float (&carry)[VEC], float (&in)[VEC],
+template <bool UP, int VEC, int GV>
+__device__ __forceinline__ void scan_carry(const ScanPlace<VEC>& w, const float (&A)[GV], const float (&X)[VEC], float (&carry)[VEC], float (&in)[VEC],
                                            float (*s_a)[SCAN_COLS], float (*s_x)[SCAN_COLS]) {
-    float from[VEC];
+    float from[VEC], pa[GV];
     if (w.NW > 1) {
         const int mine = (threadIdx.x >> 6) - w.first_wave;
 #pragma unroll
@@ -272,82 +279,95 @@ __device__ __forceinline__ void scan_carry(const ScanPlace<VEC>& w, const float 
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
                 if (k == mine) from[v] = carry[v];
-                carry[v] = scan_apply(s_a[w.first_wave + k][w.c * VEC + v], carry[v], s_x[w.first_wave + k][w.c * VEC + v]);
+                carry[v] = scan_apply(s_a[w.first_wave + k][w.c * VEC + scan_gate<GV>(v)], carry[v], s_x[w.first_wave + k][w.c * VEC + v]);
             }
         }
     } else {
         const int last = (w.lane & ~(w.CL * w.SW - 1)) + (UP ? (w.SW - 1) * w.CL : 0) + w.c;
 #pragma unroll
+        for (int g = 0; g < GV; ++g) pa[g] = __shfl(A[g], last, 64);
+#pragma unroll
         for (int v = 0; v < VEC; ++v) {
             from[v] = carry[v];
-            carry[v] = scan_apply(__shfl(A[v], last, 64), carry[v], __shfl(X[v], last, 64));
+            carry[v] = scan_apply(pa[scan_gate<GV>(v)], carry[v], __shfl(X[v], last, 64));
         }
     }
     const bool first = UP ? w.slw == 0 : w.slw == w.SW - 1;
 #pragma unroll
+    for (int g = 0; g < GV; ++g) pa[g] = UP ? __shfl_up(A[g], w.CL, 64) : __shfl_down(A[g], w.CL, 64);
+#pragma unroll
     for (int v = 0; v < VEC; ++v) {
-        const float pa = UP ? __shfl_up(A[v], w.CL, 64) : __shfl_down(A[v], w.CL, 64);
         const float px = UP ? __shfl_up(X[v], w.CL, 64) : __shfl_down(X[v], w.CL, 64);
-        in[v] = first ? from[v] : scan_apply(pa, from[v], px);
+        in[v] = first ? from[v] : scan_apply(pa[scan_gate<GV>(v)], from[v], px);
     }
+}
+
+template <int VEC, int GV>
+__device__ __forceinline__ void scan_identity(float (&A)[GV], float (&X)[VEC]) {
+#pragma unroll
+    for (int g = 0; g < GV; ++g) A[g] = 1.0f;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) X[v] = 0.0f;
+}
+// (A, X) <- first (A, X), then (A2, X2)
+template <int VEC, int GV>
+__device__ __forceinline__ void scan_append(float (&A)[GV], float (&X)[VEC], const float (&A2)[GV], const float (&X2)[VEC]) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) X[v] = scan_apply(A2[scan_gate<GV>(v)], X[v], X2[v]);
+#pragma unroll
+    for (int g = 0; g < GV; ++g) A[g] *= A2[g];
 }
 
 // The state a segment is entered with, from `carry` = what the recurrence starts from: the (A, X) of the segments in
 // front of it (UP) or behind it, a stretch of them per slice, joined like the slices of a tile.
-template <int VEC, bool UP>
+template <bool UP, int GV, int VEC>
 __device__ __forceinline__ void scan_fold(const ScanArgs& p, const ScanPlace<VEC>& w, int64_t seg, float (*s_a)[SCAN_COLS], float (*s_x)[SCAN_COLS], float (&carry)[VEC]) {
     const int64_t first = UP ? 0 : seg + 1, n = UP ? seg : p.s.segments - 1 - seg, BC = p.s.B * p.s.C;
     if (n == 0) return;
     const int64_t per = (n + w.S - 1) >> p.s.ls, begin = w.sl * per, end = min(begin + per, n);
-    float A[VEC], X[VEC], in[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) { A[v] = 1.0f; X[v] = 0.0f; }
+    float A[GV], X[VEC], in[VEC];
+    scan_identity(A, X);
     if (w.on) {
 #pragma unroll 4
         for (int64_t i = begin; i < end; ++i) {
             const int64_t k = first + (UP ? i : end - 1 - (i - begin));
-            float A_k[VEC], X_k[VEC];
-            load_run<VEC>(p.agg + k * BC + w.bc, A_k);
+            float A_k[GV], X_k[VEC];
+            load_run<GV>(p.agg + k * BC + w.bc, A_k);   // (of the same value for all columns of a gate the first)
             load_run<VEC>(p.agg + (p.s.segments + k) * BC + w.bc, X_k);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                X[v] = scan_apply(A_k[v], X[v], X_k[v]);
-                A[v] *= A_k[v];
-            }
+            scan_append(A, X, A_k, X_k);
         }
     }
-    scan_wave<VEC, UP>(w, A, X);
-    scan_exchange<VEC, UP>(w, A, X, s_a, s_x);
-    scan_carry<VEC, UP>(w, A, X, carry, in, s_a, s_x);
+    scan_wave<UP>(w, A, X);
+    scan_exchange<UP>(w, A, X, s_a, s_x);
+    scan_carry<UP>(w, A, X, carry, in, s_a, s_x);
 }
 
 // (A, X) of the thread's K steps; x is multiplied by its weight first if the recurrence blends.
 template <int VEC, int K, class GT, int GV, class XT>
-__device__ __forceinline__ void scan_local(const Steps<GT, GV, K>& a, const Steps<XT, VEC, K>& x, int blend, float (&A)[VEC], float (&X)[VEC]) {
+__device__ __forceinline__ void scan_local(const Steps<GT, GV, K>& a, const Steps<XT, VEC, K>& x, int blend, float (&A)[GV], float (&X)[VEC]) {
+    scan_identity(A, X);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) { A[v] = 1.0f; X[v] = 0.0f; }
-#pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             const float ak = a(k, v), xk = x(k, v);
             X[v] = fmaf(ak, X[v], blend ? (1.0f - ak) * xk : xk);
-            A[v] *= ak;
         }
+#pragma unroll
+        for (int g = 0; g < GV; ++g) A[g] *= a(k, g);
+    }
 }
 // (A, R) of the same steps from the other end: r_{i-1} = a_i (dh_i + r_i)
 template <int VEC, int K, class GT, int GV, class XT>
-__device__ __forceinline__ void scan_local_back(const Steps<GT, GV, K>& a, const Steps<XT, VEC, K>& dh, float (&A)[VEC], float (&R)[VEC]) {
+__device__ __forceinline__ void scan_local_back(const Steps<GT, GV, K>& a, const Steps<XT, VEC, K>& dh, float (&A)[GV], float (&R)[VEC]) {
+    scan_identity(A, R);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) { A[v] = 1.0f; R[v] = 0.0f; }
+    for (int k = K - 1; k >= 0; --k) {
 #pragma unroll
-    for (int k = K - 1; k >= 0; --k)
+        for (int v = 0; v < VEC; ++v) R[v] = a(k, v) * (dh(k, v) + R[v]);
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const float ak = a(k, v);
-            R[v] = ak * (dh(k, v) + R[v]);
-            A[v] *= ak;
-        }
+        for (int g = 0; g < GV; ++g) A[g] *= a(k, g);
+    }
 }
 
 // ---- chains -----------------------------------------------------------------------------------------------------
@@ -408,26 +428,30 @@ struct ChainPlace {
     }
 };
 
-// Publishes the (A, X) of the order-th tile of the chain, which are also returned.  The waves' have been exchanged
-// through s_a and s_x.
-template <int VEC>
+// Publishes the (A, X) of the order-th tile of the chain.  The waves' have been exchanged through s_a and s_x.
+template <int GV, int VEC>
 __device__ __forceinline__ void chain_publish(const ScanArgs& p, const ScanPlace<VEC>& w, int64_t chain, int64_t order, float (*s_a)[SCAN_COLS], float (*s_x)[SCAN_COLS]) {
     const ChainPlace<VEC> at(p, w, chain, order);
     if (w.sl != 0 || at.k == CHAIN_GROUP - 1) return;
+    float A[GV], X[VEC];
+    scan_identity(A, X);
+    for (int n = 0; n < w.NW; ++n) {
+        float A_n[GV], X_n[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-        float A = 1.0f, X = 0.0f;
-        for (int n = 0; n < w.NW; ++n) {
-            X = scan_apply(s_a[n][w.c * VEC + v], X, s_x[n][w.c * VEC + v]);
-            A *= s_a[n][w.c * VEC + v];
-        }
-        chain_put(at.words + at.k * (2 * SCAN_COLS) + 2 * v * w.CL, A);
-        chain_put(at.words + at.k * (2 * SCAN_COLS) + (2 * v + 1) * w.CL, X);
+        for (int g = 0; g < GV; ++g) A_n[g] = s_a[n][w.c * VEC + g];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) X_n[v] = s_x[n][w.c * VEC + v];
+        scan_append(A, X, A_n, X_n);
     }
+    unsigned long long* const to = at.words + at.k * (2 * SCAN_COLS);
+#pragma unroll
+    for (int g = 0; g < GV; ++g) chain_put(to + g * w.CL, A[g]);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) chain_put(to + (GV + v) * w.CL, X[v]);
 }
 
 // `state`: what the recurrence starts from -> what this tile is entered with.  s_part is [CHAIN_GROUP][2][SCAN_COLS].
-template <int VEC>
+template <int GV, int VEC>
 __device__ __forceinline__ void chain_state(const ScanArgs& p, const ScanPlace<VEC>& w, int64_t chain, int64_t order, float (*s_a)[SCAN_COLS], float (*s_x)[SCAN_COLS],
                                             float (*s_part)[2][SCAN_COLS], float (&state)[VEC]) {
     const ChainPlace<VEC> at(p, w, chain, order);
@@ -435,13 +459,12 @@ __device__ __forceinline__ void chain_state(const ScanArgs& p, const ScanPlace<V
     const int64_t group = at.group;
 #pragma unroll 1
     for (int q = w.sl; q < k; q += w.S) {
-        float ax[2 * VEC];
-        chain_get<2 * VEC, 8>(at.words + q * (2 * SCAN_COLS), w.CL, ax);
+        float ax[GV + VEC];
+        chain_get<GV + VEC, 8>(at.words + q * (2 * SCAN_COLS), w.CL, ax);
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            s_part[q][0][col + v] = ax[2 * v];
-            s_part[q][1][col + v] = ax[2 * v + 1];
-        }
+        for (int g = 0; g < GV; ++g) s_part[q][0][col + g] = ax[g];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) s_part[q][1][col + v] = ax[GV + v];
     }
     if (group > 0 && w.sl == w.S - 1) {   // the slice that has the fewest tiles to wait for
         float h[VEC];
@@ -461,15 +484,13 @@ __device__ __forceinline__ void chain_state(const ScanArgs& p, const ScanPlace<V
 #pragma unroll 2
     for (int q = 0; q < k; ++q)
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) state[v] = scan_apply(s_part[q][0][col + v], state[v], s_part[q][1][col + v]);
+        for (int v = 0; v < VEC; ++v) state[v] = scan_apply(s_part[q][0][col + scan_gate<GV>(v)], state[v], s_part[q][1][col + v]);
     if (w.sl == 0 && k == CHAIN_GROUP - 1 && order + 1 < p.s.tiles) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             float h = state[v];
 #pragma unroll 1
-            for (int n = 0; n < w.NW; ++n) {
-                    h = scan_apply(s_a[n][col + v], h, s_x[n][col + v]);
-            }
+            for (int n = 0; n < w.NW; ++n) h = scan_apply(s_a[n][col + scan_gate<GV>(v)], h, s_x[n][col + v]);
             chain_put(at.states + SCAN_COLS + v * w.CL, h);
         }
     }
@@ -488,9 +509,8 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_segments_kernel(ScanArgs p)
     const int64_t rounds = min(s.seg_tiles, s.tiles - seg * s.seg_tiles);
     const int64_t begin = seg * s.seg_tiles * s.tile_steps + w.sl * rounds * K;   // of the slice's stretch
     const int64_t x_step = p.reverse ? -(int64_t)s.C : s.C, gate_step = p.reverse ? -(int64_t)s.G : s.G;
-    float A[VEC], X[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) { A[v] = 1.0f; X[v] = 0.0f; }
+    float A[GV], X[VEC];
+    scan_identity(A, X);
     Steps<GT, GV, K> a, a_next;
     Steps<XT, VEC, K> x, x_next;
     const auto fetch = [&](int64_t n, Steps<GT, GV, K>& to_a, Steps<XT, VEC, K>& to_x) {
@@ -505,47 +525,37 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_segments_kernel(ScanArgs p)
         a = a_next;
         x = x_next;
         if (n + 1 < rounds) fetch(n + 1, a_next, x_next);   // under way while these steps are summed
-        float A_now[VEC], X_now[VEC];
+        float A_now[GV], X_now[VEC];
         if (BACK) scan_local_back(a, x, A_now, X_now);
         else scan_local(a, x, p.blend, A_now, X_now);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            X[v] = scan_apply(A_now[v], X[v], X_now[v]);
-            A[v] *= A_now[v];
-        }
+        scan_append(A, X, A_now, X_now);
     }
-    scan_wave<VEC, !BACK>(w, A, X);   // the last slice (BACK: the first) of a wave holds the wave's
-    if (w.slw == (BACK ? 0 : w.SW - 1)) {
+    scan_wave<!BACK>(w, A, X);   // the last slice (BACK: the first) of a wave holds the wave's
+    const auto write = [&] {
         const int64_t BC = s.B * s.C;
-        if (w.NW == 1) {
-            if (w.on) {
-                store_run<VEC>(p.agg + seg * BC + w.bc, A);
-                store_run<VEC>(p.agg + (s.segments + seg) * BC + w.bc, X);
-            }
-            return;
-        }
+        float A_all[VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            s_a[threadIdx.x >> 6][w.c * VEC + v] = A[v];
-            s_x[threadIdx.x >> 6][w.c * VEC + v] = X[v];
-        }
+        for (int v = 0; v < VEC; ++v) A_all[v] = A[scan_gate<GV>(v)];
+        store_run<VEC>(p.agg + seg * BC + w.bc, A_all);
+        store_run<VEC>(p.agg + (s.segments + seg) * BC + w.bc, X);
+    };
+    if (w.NW == 1) {
+        if (w.on && w.slw == (BACK ? 0 : w.SW - 1)) write();
+        return;
     }
-    if (w.NW == 1) return;
-    __syncthreads();
+    scan_exchange<!BACK>(w, A, X, s_a, s_x);
     if (w.on && w.sl == 0) {
-        const int64_t BC = s.B * s.C;
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) { A[v] = 1.0f; X[v] = 0.0f; }
+        scan_identity(A, X);
         for (int k = 0; k < w.NW; ++k) {
             const int from = w.first_wave + (BACK ? w.NW - 1 - k : k);
+            float A_k[GV], X_k[VEC];
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                X[v] = scan_apply(s_a[from][w.c * VEC + v], X[v], s_x[from][w.c * VEC + v]);
-                A[v] *= s_a[from][w.c * VEC + v];
-            }
+            for (int g = 0; g < GV; ++g) A_k[g] = s_a[from][w.c * VEC + g];
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) X_k[v] = s_x[from][w.c * VEC + v];
+            scan_append(A, X, A_k, X_k);
         }
-        store_run<VEC>(p.agg + seg * BC + w.bc, A);
-        store_run<VEC>(p.agg + (s.segments + seg) * BC + w.bc, X);
+        write();
     }
 }
 
@@ -563,7 +573,7 @@ __global__ __launch_bounds__(SCAN_THREADS, CHAIN ? 4 : 1) void scan_fwd_kernel(S
     if (w.on) {
         if (p.state) load_run<VEC>(p.state + w.bc, carry);
     }
-    if (!CHAIN) scan_fold<VEC, true>(p, w, seg, s_a[~t_begin & 1], s_x[~t_begin & 1], carry);
+    if (!CHAIN) scan_fold<true, GV>(p, w, seg, s_a[~t_begin & 1], s_x[~t_begin & 1], carry);
     const int64_t x_step = p.reverse ? -(int64_t)s.C : s.C, gate_step = p.reverse ? -(int64_t)s.G : s.G;
     Steps<GT, GV, K> a, a_next;
     Steps<XT, VEC, K> x, x_next;
@@ -587,15 +597,15 @@ __global__ __launch_bounds__(SCAN_THREADS, CHAIN ? 4 : 1) void scan_fwd_kernel(S
         }
         const int64_t i0 = tile * s.tile_steps + w.sl * K, at = w.at(s, i0, p.reverse);
         const int count = w.count(s, i0);
-        float A[VEC], X[VEC], h[VEC];
+        float A[GV], X[VEC], h[VEC];
         scan_local(a, x, p.blend, A, X);
-        scan_wave<VEC, true>(w, A, X);
-        scan_exchange<VEC, true>(w, A, X, s_a[tile & 1], s_x[tile & 1]);
+        scan_wave<true>(w, A, X);
+        scan_exchange<true>(w, A, X, s_a[tile & 1], s_x[tile & 1]);
         if (CHAIN) {
-            chain_publish<VEC>(p, w, block, tile, s_a[tile & 1], s_x[tile & 1]);
-            chain_state<VEC>(p, w, block, tile, s_a[tile & 1], s_x[tile & 1], s_part, carry);
+            chain_publish<GV>(p, w, block, tile, s_a[tile & 1], s_x[tile & 1]);
+            chain_state<GV>(p, w, block, tile, s_a[tile & 1], s_x[tile & 1], s_part, carry);
         }
-        scan_carry<VEC, true>(w, A, X, carry, h, s_a[tile & 1], s_x[tile & 1]);
+        scan_carry<true>(w, A, X, carry, h, s_a[tile & 1], s_x[tile & 1]);
         if (p.carry && count > 0 && i0 > 0 && (i0 & ((1 << p.l_carry) - 1)) == 0) store_run<VEC>(p.carry + ((i0 >> p.l_carry) - 1) * BC + w.bc, h);
         a.forget();
         x.forget();
@@ -630,7 +640,7 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
     if (w.on) {
         if (p.d_last) load_run<VEC>(p.d_last + w.bc, r_carry);
     }
-    scan_fold<VEC, false>(p, w, seg, s_b[t_end & 1], s_r[t_end & 1], r_carry);
+    scan_fold<false, GV>(p, w, seg, s_b[t_end & 1], s_r[t_end & 1], r_carry);
     const int64_t x_step = p.reverse ? -(int64_t)s.C : s.C, gate_step = p.reverse ? -(int64_t)s.G : s.G;
     // (the next tile under way as in the forward pass was slower here: 151 registers against 119, 240 us against 215 for a
     // bfloat16 sequence of 65536 x 1024)
@@ -639,7 +649,7 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
         const int count = w.count(s, i0);
         Steps<GT, GV, K> a;
         Steps<XT, VEC, K> x, dh;
-        float A[VEC], X[VEC], h[VEC], r[VEC], carry[VEC];
+        float A[GV], X[VEC], h[VEC], r[VEC], carry[VEC];
         a.load(static_cast<const GT*>(p.gate) + gate_at, gate_step, count, 1.0f);
         x.load(static_cast<const XT*>(p.x) + at, x_step, count, 0.0f);
         if (p.d_h) dh.load(static_cast<const XT*>(p.d_h) + at, x_step, count, 0.0f);
@@ -651,14 +661,14 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
             else if (p.state) load_run<VEC>(p.state + w.bc, carry);
         }
         scan_local(a, x, p.blend, A, X);
-        scan_wave<VEC, true>(w, A, X);
-        scan_exchange<VEC, true>(w, A, X, s_a[tile & 1], s_x[tile & 1]);
-        scan_carry<VEC, true>(w, A, X, carry, h, s_a[tile & 1], s_x[tile & 1]);
+        scan_wave<true>(w, A, X);
+        scan_exchange<true>(w, A, X, s_a[tile & 1], s_x[tile & 1]);
+        scan_carry<true>(w, A, X, carry, h, s_a[tile & 1], s_x[tile & 1]);
         a.forget();
         scan_local_back(a, dh, A, X);
-        scan_wave<VEC, false>(w, A, X);
-        scan_exchange<VEC, false>(w, A, X, s_b[tile & 1], s_r[tile & 1]);
-        scan_carry<VEC, false>(w, A, X, r_carry, r, s_b[tile & 1], s_r[tile & 1]);
+        scan_wave<false>(w, A, X);
+        scan_exchange<false>(w, A, X, s_b[tile & 1], s_r[tile & 1]);
+        scan_carry<false>(w, A, X, r_carry, r, s_b[tile & 1], s_r[tile & 1]);
         a.forget();
         x.forget();
         dh.forget();
@@ -765,6 +775,8 @@ static int scan_launch(const ScanArgs& p, int dir, const char* who, hipStream_t 
 template <class GT, class XT>
 static int scan_run_typed(const ScanArgs& p, int dir, const char* who, hipStream_t stream) {
     if (p.s.vec == 1) return scan_launch<GT, XT, 1, 1>(p, dir, who, stream);
+    if (p.s.vec == 2) return scan_launch<GT, XT, 2, 1>(p, dir, who, stream);
+    if (p.s.vec == 3) return scan_launch<GT, XT, 3, 1>(p, dir, who, stream);
     return p.s.G == p.s.C ? scan_launch<GT, XT, 4, 4>(p, dir, who, stream) : scan_launch<GT, XT, 4, 1>(p, dir, who, stream);
 }
 

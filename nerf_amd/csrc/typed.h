@@ -4,8 +4,9 @@
 
 namespace nerf {
 
+// N consecutive elements, aligned as an array of them that starts on a 16-byte boundary is.
 template <class T, int N>
-struct __attribute__((aligned(sizeof(T) * N))) Run {
+struct __attribute__((aligned((sizeof(T) * N) & -(sizeof(T) * N)))) Run {
     T v[N];
 };
 

@@ -110,7 +110,7 @@ def test_lengths_and_layouts(dev, T, C, G):
 @pytest.mark.parametrize("tx,tg", [(F32, F32), (BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)])
 @pytest.mark.parametrize("reverse", [False, True])
 @pytest.mark.parametrize("blend", [False, True])
-@pytest.mark.parametrize("B,T,C,G", [(3, 70, 132, 132), (2, 200, 96, 3), (4, 33, 7, 7), (1, 517, 30, 6)])
+@pytest.mark.parametrize("B,T,C,G", [(3, 70, 132, 132), (2, 200, 96, 3), (4, 33, 7, 7), (1, 517, 30, 6), (5, 300, 3, 1), (2, 70, 6, 2), (3, 129, 4, 2), (9, 2500, 3, 1)])
 def test_types(dev, tx, tg, reverse, blend, B, T, C, G):
     check(dev, B, T, C, G, tx, tg, reverse, blend, state=B % 2 == 0, seed=B)
 
@@ -120,7 +120,7 @@ def test_types(dev, tx, tg, reverse, blend, B, T, C, G):
                                      (1, 9000, 68, 1), (2, 1500, 520, 2), (1, 4097, 300, 1), (17, 100, 600, 600), (2, 40, 1030, 1),
                                      # tiles in a chain: two, some, several groups of them; every way to lay out the lanes
                                      (3, 70, 132, 132), (3, 600, 132, 132), (9, 1021, 100, 100), (2, 3000, 520, 520), (8, 2500, 64, 1), (8, 2500, 5, 1), (600, 5000, 1, 1), (8, 40000, 4, 4),
-                                     (4, 1021, 65, 65), (4, 700, 130, 2), (8, 9000, 12, 4)])
+                                     (4, 1021, 65, 65), (4, 700, 130, 2), (8, 9000, 12, 4), (3, 30000, 3, 1), (70, 9000, 6, 3)])
 def test_sizes(dev, B, T, C, G):
     check(dev, B, T, C, G, reverse=True, blend=True, state=True, seed=5)
 
