@@ -43,8 +43,8 @@ struct ScanShape {
     int units_per_b;        // 1 (a gate per channel) or G
     int vec, steps, lcl, ls;   // elements per lane, steps per thread, log2 of CL and of S
     int col_tiles;          // column tiles of a unit
-    int64_t unit_tiles;     // B * units_per_b * col_tiles
-    int64_t blocks;         // workgroups that hold them
+    int64_t unit_tiles;     // B * units_per_b * col_tiles, below 2^32
+    int64_t blocks;         // workgroups that hold them, below 2^24
     int tile_steps;         // S * K
     int64_t tiles;          // time tiles
     int64_t segments, seg_tiles;   // the time axis is cut into segments of seg_tiles tiles when there are few workgroups
@@ -130,12 +130,21 @@ struct ScanArgs {
 // A h + X.  A state of exactly zero stays without effect however large the product of the gates has become.
 __device__ __forceinline__ float scan_apply(float A, float h, float X) { return h == 0.0f ? X : fmaf(A, h, X); }
 
+// Workgroup -> column block and segment, in 32 bits: a launch holds fewer than 2^24 workgroups.
+__device__ __forceinline__ unsigned scan_segment(const ScanShape& s, unsigned& block) {
+    block = blockIdx.x;
+    if (s.segments == 1) return 0;
+    const unsigned seg = blockIdx.x / (unsigned)s.blocks;
+    block -= seg * (unsigned)s.blocks;
+    return seg;
+}
+
 // Where a thread stands: its columns and its slice.
 template <int VEC>
 struct ScanPlace {
     int CL, S, SW, NW;          // lanes on columns, slices, slices of the group in one wave, waves of the group
     int c, sl, slw, lane, first_wave;
-    bool on;                    // has columns
+    bool on, in_unit;           // has columns; stands in a unit, with or without columns of it
     int64_t b;
     int j;                      // first column, in [0, C)
     int64_t g;                  // gate of a shared unit
@@ -154,14 +163,24 @@ struct ScanPlace {
         slw = sl & (SW - 1);
         const int q = tid >> (s.lcl + s.ls);
         first_wave = NW > 1 ? (tid >> 6) & ~(NW - 1) : 0;
-        const int64_t ut = block * (SCAN_THREADS >> (s.lcl + s.ls)) + q;
-        const int64_t u = ut / s.col_tiles;
-        col_tile = (int)(ut - u * s.col_tiles);
-        b = u / s.units_per_b;
-        g = u - b * s.units_per_b;
-        const int in_unit = (col_tile * CL + c) * VEC;
-        on = ut < s.unit_tiles && in_unit < s.P;
-        j = (int)g * s.P + in_unit;
+        const unsigned ut = (unsigned)block * (SCAN_THREADS >> (s.lcl + s.ls)) + q;
+        unsigned u = ut, in_b = 0;
+        col_tile = 0;
+        if (s.col_tiles > 1) {
+            u = ut / (unsigned)s.col_tiles;
+            col_tile = (int)(ut - u * s.col_tiles);
+        }
+        if (s.units_per_b > 1) {
+            const unsigned all = u;
+            u = all / (unsigned)s.units_per_b;
+            in_b = all - u * s.units_per_b;
+        }
+        b = u;
+        g = in_b;
+        const int col = (col_tile * CL + c) * VEC;
+        in_unit = (int64_t)ut < s.unit_tiles;
+        on = in_unit && col < s.P;
+        j = (int)g * s.P + col;
         bc = b * s.C + j;
     }
     // place of step i (in the order of the recurrence) of this thread's columns in a [B,T,C] array / of its gate; from one
@@ -176,6 +195,9 @@ struct ScanPlace {
     // steps of the slice that starts at i0 and exist
     __device__ __forceinline__ int count(const ScanShape& s, int64_t i0) const {
         return !on || i0 >= s.T ? 0 : (int)min((int64_t)s.steps, s.T - i0);
+    }
+    __device__ __forceinline__ int count_in_unit(const ScanShape& s, int64_t i0) const {
+        return !in_unit || i0 >= s.T ? 0 : (int)min((int64_t)s.steps, s.T - i0);
     }
 };
 
@@ -210,6 +232,35 @@ struct Steps {
             }
         }
     }
+    // All K steps where they are one piece of memory of K * N elements, from its lowest address, a multiple of 16 bytes.
+    __device__ __forceinline__ void load_dense(const T* __restrict__ p, int reverse) {
+        constexpr int ALL = K * N * sizeof(T) / 4;
+        unsigned word[ALL];
+#pragma unroll
+        for (int i = 0; i < ALL; i += 4) {
+            const uint4 q = *reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned*>(p) + i);
+            word[i] = q.x; word[i + 1] = q.y; word[i + 2] = q.z; word[i + 3] = q.w;
+        }
+        const auto half = [&](int e) { return word[e / 2] >> (e & 1) * 16 & 0xffffu; };
+        const auto take = [&](int k, int from) {
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) {
+                if constexpr (sizeof(T) == 4) {
+                    w[k][i] = word[from * N + i];
+                } else {
+                    w[k][i] = half(from * N + 2 * i);
+                    if (2 * i + 1 < N) w[k][i] |= half(from * N + 2 * i + 1) << 16;
+                }
+            }
+        };
+        if (reverse) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) take(k, K - 1 - k);
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; ++k) take(k, k);
+        }
+    }
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int k = 0; k < K; ++k)
@@ -226,6 +277,22 @@ struct Steps {
             for (int i = 0; i < WORDS; ++i) asm volatile("" : "+v"(w[k][i]));
     }
 };
+
+// The K steps' outputs as one piece of memory.
+template <class T, int K, int N>
+__device__ __forceinline__ void store_dense(T* __restrict__ p, int reverse, const float (&v)[K][N]) {
+    const auto value = [&](int e) { return (T)(reverse ? v[K - 1 - e / N][e % N] : v[e / N][e % N]); };
+    constexpr int ALL = K * N * sizeof(T) / 4;
+    unsigned word[ALL];
+#pragma unroll
+    for (int i = 0; i < ALL; ++i) {
+        if constexpr (sizeof(T) == 4) word[i] = __builtin_bit_cast(unsigned, value(i));
+        else word[i] = __builtin_bit_cast(unsigned short, value(2 * i)) | (unsigned)__builtin_bit_cast(unsigned short, value(2 * i + 1)) << 16;
+    }
+#pragma unroll
+    for (int i = 0; i < ALL; i += 4)
+        *reinterpret_cast<uint4*>(reinterpret_cast<unsigned*>(p) + i) = uint4{word[i], word[i + 1], word[i + 2], word[i + 3]};
+}
 
 // Everywhere below: A [GV], one product for all VEC columns of a lane where they share a gate (GV = 1), else one each.
 template <int GV>
@@ -504,8 +571,9 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_segments_kernel(ScanArgs p)
     constexpr int K = scan_steps(GV);
     __shared__ float s_a[4][SCAN_COLS], s_x[4][SCAN_COLS];
     const ScanShape& s = p.s;
-    const int64_t seg = blockIdx.x / s.blocks + (BACK ? 1 : 0);
-    const ScanPlace<VEC> w(s, blockIdx.x % s.blocks);
+    unsigned block;
+    const int64_t seg = scan_segment(s, block) + (BACK ? 1 : 0);
+    const ScanPlace<VEC> w(s, block);
     const int64_t rounds = min(s.seg_tiles, s.tiles - seg * s.seg_tiles);
     const int64_t begin = seg * s.seg_tiles * s.tile_steps + w.sl * rounds * K;   // of the slice's stretch
     const int64_t x_step = p.reverse ? -(int64_t)s.C : s.C, gate_step = p.reverse ? -(int64_t)s.G : s.G;
@@ -559,12 +627,14 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_segments_kernel(ScanArgs p)
     }
 }
 
-template <class GT, class XT, int VEC, int GV, int K, bool CHAIN>
+// DENSE: a lane has all channels of a sequence and its steps are one piece of memory (few channels, the rays of a picture):
+// they move 16 bytes at a time.  65536 rays x 192 x 3 float: @@ us step by step, @@ so; x 1: @@ and @@.
+template <class GT, class XT, int VEC, int GV, int K, bool CHAIN, bool DENSE>
 __global__ __launch_bounds__(SCAN_THREADS, CHAIN ? 4 : 1) void scan_fwd_kernel(ScanArgs p) {
     __shared__ float s_a[2][4][SCAN_COLS], s_x[2][4][SCAN_COLS], s_part[CHAIN ? CHAIN_GROUP : 1][2][SCAN_COLS];
     const ScanShape& s = p.s;
-    const int64_t block = blockIdx.x % s.blocks, BC = s.B * s.C;
-    const int64_t seg = CHAIN ? chain_ticket(p, block) : blockIdx.x / s.blocks;
+    unsigned block;
+    const int64_t BC = s.B * s.C, segment = scan_segment(s, block), seg = CHAIN ? chain_ticket(p, block) : segment;
     const ScanPlace<VEC> w(s, block);
     const int64_t t_begin = CHAIN ? seg : seg * s.seg_tiles, t_end = CHAIN ? seg + 1 : min(t_begin + s.seg_tiles, s.tiles);
     float carry[VEC];
@@ -580,6 +650,14 @@ __global__ __launch_bounds__(SCAN_THREADS, CHAIN ? 4 : 1) void scan_fwd_kernel(S
     const auto fetch = [&](int64_t tile, Steps<GT, GV, K>& to_a, Steps<XT, VEC, K>& to_x) {
         const int64_t i0 = tile * s.tile_steps + w.sl * K;
         const int count = tile < t_end ? w.count(s, i0) : 0;
+        if constexpr (DENSE) {
+            if (count == K) {
+                const int64_t low = p.reverse ? i0 + K - 1 : i0;
+                to_a.load_dense(static_cast<const GT*>(p.gate) + w.gate_at(s, low, p.reverse), p.reverse);
+                to_x.load_dense(static_cast<const XT*>(p.x) + w.at(s, low, p.reverse), p.reverse);
+                return;
+            }
+        }
         to_a.load(static_cast<const GT*>(p.gate) + w.gate_at(s, i0, p.reverse), gate_step, count, 1.0f);
         to_x.load(static_cast<const XT*>(p.x) + w.at(s, i0, p.reverse), x_step, count, 0.0f);
     };
@@ -610,28 +688,71 @@ __global__ __launch_bounds__(SCAN_THREADS, CHAIN ? 4 : 1) void scan_fwd_kernel(S
         a.forget();
         x.forget();
         XT* __restrict__ out = static_cast<XT*>(p.h) + at;
+        float piece[DENSE ? K : 1][VEC];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
                 const float ak = a(k, v), xk = x(k, v);
                 h[v] = fmaf(ak, h[v], p.blend ? (1.0f - ak) * xk : xk);
+                if (DENSE) piece[DENSE ? k : 0][v] = h[v];
             }
-            if (k < count) store_run<VEC>(out + k * x_step, h);
+            if (k < count && !(DENSE && count == K)) store_run<VEC>(out + k * x_step, h);
+        }
+        if constexpr (DENSE) {
+            if (count == K) store_dense(p.reverse ? out + (K - 1) * x_step : out, p.reverse, piece);
         }
     }
     if (p.last && t_end == s.tiles && w.on && w.sl == 0) store_run<VEC>(p.last + w.bc, carry);
 }
 
+// Sums of the K steps' values over the CL lanes of a slice, and their place in the gate's gradient.  While there are
+// several values to a lane, neighbours split them: each hands half of its values on and adds what it is handed -- 7
+// exchanges for 8 values over 8 lanes instead of 24.
+template <class GT, int VEC, int K>
+__device__ __forceinline__ void scan_gate_sums(const ScanArgs& p, const ScanPlace<VEC>& w, float (&sum)[K][1], int count, GT* __restrict__ da_out, int64_t gate_at,
+                                               int64_t gate_step) {
+    static_assert(K == 8, "three halvings");
+    int first = 0, d = 1;   // the lane's values are of the steps first, first + 1, ...
+#pragma unroll
+    for (int n = K / 2; n > 0; n >>= 1) {
+        if (d < w.CL) {
+            const bool upper = w.c & d;
+#pragma unroll
+            for (int j = 0; j < n; ++j) {
+                const float give = upper ? sum[j][0] : sum[j + n][0], keep = upper ? sum[j + n][0] : sum[j][0];
+                sum[j][0] = keep + __shfl_xor(give, d, 64);
+            }
+            first += upper ? n : 0;
+            d <<= 1;
+        }
+    }
+    const int held = K / d;
+    bool writes = true;
+    for (; d < w.CL; d <<= 1) {
+        sum[0][0] += __shfl_xor(sum[0][0], d, 64);
+        writes = writes && !(w.c & d);
+    }
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+        const int k = first + j;
+        if (j < held && writes && k < count) {
+            if (p.s.col_tiles == 1) da_out[k * gate_step] = (GT)sum[j][0];
+            else p.d_gate_part[(int64_t)w.col_tile * p.s.B * p.s.T * p.s.G + gate_at + k * gate_step] = sum[j][0];
+        }
+    }
+}
+
 // The time axis is spread by segments here.  (As a chain -- 16 KB of LDS, 168 registers, three workgroups on a compute unit
 // against four -- it took 340 us for 65536 x 1024 bfloat16 with float32 gates, the two kernels 303.)
-template <class GT, class XT, int VEC, int GV>
+template <class GT, class XT, int VEC, int GV, bool DENSE>
 __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
     constexpr int K = scan_steps(GV);
     __shared__ float s_a[2][4][SCAN_COLS], s_x[2][4][SCAN_COLS], s_b[2][4][SCAN_COLS], s_r[2][4][SCAN_COLS];
     const ScanShape& s = p.s;
-    const int64_t seg = blockIdx.x / s.blocks, BC = s.B * s.C;
-    const ScanPlace<VEC> w(s, blockIdx.x % s.blocks);
+    unsigned block;
+    const int64_t seg = scan_segment(s, block), BC = s.B * s.C;
+    const ScanPlace<VEC> w(s, block);
     const int64_t t_begin = seg * s.seg_tiles, t_end = min(t_begin + s.seg_tiles, s.tiles);
     const bool shared_gate = s.G != s.C;
     float r_carry[VEC];
@@ -650,10 +771,22 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
         Steps<GT, GV, K> a;
         Steps<XT, VEC, K> x, dh;
         float A[GV], X[VEC], h[VEC], r[VEC], carry[VEC];
-        a.load(static_cast<const GT*>(p.gate) + gate_at, gate_step, count, 1.0f);
-        x.load(static_cast<const XT*>(p.x) + at, x_step, count, 0.0f);
-        if (p.d_h) dh.load(static_cast<const XT*>(p.d_h) + at, x_step, count, 0.0f);
-        else dh.clear();
+        const int64_t low = DENSE && p.reverse ? at + (K - 1) * x_step : at, gate_low = DENSE && p.reverse ? gate_at + (K - 1) * gate_step : gate_at;
+        const bool whole = DENSE && count == K;
+        if constexpr (DENSE) {
+            if (whole) {
+                a.load_dense(static_cast<const GT*>(p.gate) + gate_low, p.reverse);
+                x.load_dense(static_cast<const XT*>(p.x) + low, p.reverse);
+                if (p.d_h) dh.load_dense(static_cast<const XT*>(p.d_h) + low, p.reverse);
+                else dh.clear();
+            }
+        }
+        if (!whole) {
+            a.load(static_cast<const GT*>(p.gate) + gate_at, gate_step, count, 1.0f);
+            x.load(static_cast<const XT*>(p.x) + at, x_step, count, 0.0f);
+            if (p.d_h) dh.load(static_cast<const XT*>(p.d_h) + at, x_step, count, 0.0f);
+            else dh.clear();
+        }
 #pragma unroll
         for (int v = 0; v < VEC; ++v) carry[v] = 0.0f;
         if (w.on) {
@@ -683,6 +816,7 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
             }
         XT* __restrict__ dx_out = static_cast<XT*>(p.d_x) + at;
         GT* __restrict__ da_out = static_cast<GT*>(p.d_gate) + gate_at;
+        float dx_piece[DENSE ? K : 1][VEC], da_sum[K][1];
 #pragma unroll
         for (int k = K - 1; k >= 0; --k) {
             float da[VEC], dx[VEC];
@@ -692,21 +826,31 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
                 da[v] = g * beside[k][v];
                 dx[v] = p.blend ? (1.0f - ak) * g : g;
                 r[v] = ak * g;
+                if (DENSE) dx_piece[DENSE ? k : 0][v] = dx[v];
             }
-            if (p.d_x && k < count) store_run<VEC>(dx_out + k * x_step, dx);
-            if (!p.d_gate) continue;
-            if (!shared_gate) {
-                if (k < count) store_run<VEC>(da_out + k * gate_step, da);
-            } else {
-                float sum = da[0];
+            if (p.d_x && k < count && !whole) store_run<VEC>(dx_out + k * x_step, dx);
+            da_sum[k][0] = da[0];
+            if (GV == 1) {
 #pragma unroll
-                for (int v = 1; v < VEC; ++v) sum += da[v];
-                if (k >= count) sum = 0.0f;
-                for (int d = 1; d < w.CL; d <<= 1) sum += __shfl_xor(sum, d, 64);
-                if (k < count && w.c == 0) {
-                    if (s.col_tiles == 1) da_out[k * gate_step] = (GT)sum;
-                    else p.d_gate_part[(int64_t)w.col_tile * s.B * s.T * s.G + gate_at + k * gate_step] = sum;
-                }
+                for (int v = 1; v < VEC; ++v) da_sum[k][0] += da[v];
+            } else if (p.d_gate && k < count) {
+                store_run<VEC>(da_out + k * gate_step, da);
+            }
+        }
+        if constexpr (DENSE) {
+            if (whole) {
+                if (p.d_x) store_dense(static_cast<XT*>(p.d_x) + low, p.reverse, dx_piece);
+                if (p.d_gate) store_dense(static_cast<GT*>(p.d_gate) + gate_low, p.reverse, da_sum);
+            }
+        }
+        if constexpr (GV == 1) {
+            if (whole || !p.d_gate) continue;
+            if (!shared_gate) {
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    if (k < count) da_out[k * gate_step] = (GT)da_sum[k][0];
+            } else {
+                scan_gate_sums(p, w, da_sum, w.count_in_unit(s, i0), da_out, gate_at, gate_step);   // lanes without columns write too
             }
         }
     }
@@ -740,7 +884,7 @@ static int scan_chain_launch(ScanArgs p, const char* who, hipStream_t stream) {
     hipLaunchKernelGGL(chain_clear_kernel, dim3((unsigned)std::min<int64_t>(2048, ceil_div(work.bytes, 4096))), dim3(256), 0, stream,
                        reinterpret_cast<uint4*>(at), work.bytes / 16);
     if (int rc = check_launch(who)) return rc;
-    hipLaunchKernelGGL((scan_fwd_kernel<GT, XT, VEC, GV, K, true>), dim3((unsigned)(p.s.blocks * p.s.tiles)), dim3(SCAN_THREADS), 0, stream, p);
+    hipLaunchKernelGGL((scan_fwd_kernel<GT, XT, VEC, GV, K, true, false>), dim3((unsigned)(p.s.blocks * p.s.tiles)), dim3(SCAN_THREADS), 0, stream, p);
     return check_launch(who);
 }
 
@@ -760,8 +904,14 @@ static int scan_launch(const ScanArgs& p, int dir, const char* who, hipStream_t 
         if (int rc = check_launch(who)) return rc;
     }
     const dim3 grid((unsigned)(s.blocks * s.segments));
-    if (dir == SCAN_FWD) hipLaunchKernelGGL((scan_fwd_kernel<GT, XT, VEC, GV, scan_steps(GV), false>), grid, dim3(SCAN_THREADS), 0, stream, p);
-    else hipLaunchKernelGGL((scan_bwd_kernel<GT, XT, VEC, GV>), grid, dim3(SCAN_THREADS), 0, stream, p);
+    bool dense = false;
+    if constexpr (GV == 1) {
+        dense = s.C == VEC && s.G == 1 && s.T * VEC * sizeof(XT) % 16 == 0 && s.T * sizeof(GT) % 16 == 0;
+        if (dense && dir == SCAN_FWD) hipLaunchKernelGGL((scan_fwd_kernel<GT, XT, VEC, 1, scan_steps(1), false, true>), grid, dim3(SCAN_THREADS), 0, stream, p);
+        else if (dense) hipLaunchKernelGGL((scan_bwd_kernel<GT, XT, VEC, 1, true>), grid, dim3(SCAN_THREADS), 0, stream, p);
+    }
+    if (!dense && dir == SCAN_FWD) hipLaunchKernelGGL((scan_fwd_kernel<GT, XT, VEC, GV, scan_steps(GV), false, false>), grid, dim3(SCAN_THREADS), 0, stream, p);
+    else if (!dense) hipLaunchKernelGGL((scan_bwd_kernel<GT, XT, VEC, GV, false>), grid, dim3(SCAN_THREADS), 0, stream, p);
     if (int rc = check_launch(who)) return rc;
     if (dir == SCAN_BWD && p.d_gate && s.G != s.C && s.col_tiles > 1) {
         const int64_t n = s.B * s.T * s.G;
