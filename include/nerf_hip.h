@@ -227,7 +227,8 @@ int nerf_gather_kept_by_slot(const float* d_rgb, const float* d_sigma, const int
  * c / (C/G) (G = C: one per channel, G = 1: one per step); state, last [B,C] float32; last (may be
  * NULL) receives the state after the last step.  The state is held in float32; h is rounded once.
  * Made for |gate| <= 1; larger gates are right as long as float32 holds their products over
- * stretches of the sequence.  Infinities and NaN propagate as in the formula.
+ * stretches of the sequence.  A state that has become infinite or NaN stays one or the other (an
+ * infinity may turn into a NaN; no gate takes it back), and leaves other channels alone.  C <= 131072.
  * carry: nerf_linear_scan_carry_floats(B,T,C,G) floats that the backward pass needs (NULL: not
  * kept).  workspace: nerf_linear_scan_workspace_floats(B,T,C,G,backward) floats, NULL where that is
  * 0.  T >= 1; B = 0 or C = 0 is nothing to do.  Every pointer 16-byte aligned.

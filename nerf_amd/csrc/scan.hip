@@ -33,6 +33,7 @@ namespace nerf {
 constexpr int scan_steps(int gates) { return gates > 1 ? 4 : 8; }
 constexpr int SCAN_THREADS = 256;
 constexpr int SCAN_COLS = 64;      // most columns of a unit that one workgroup takes side by side
+constexpr int SCAN_CHANNELS = 1 << 17;   // most channels
 constexpr int SCAN_WANT_BLOCKS = 1024;
 constexpr int CHAIN_GROUP = 32;    // tiles of the chain between two published states
 constexpr int CHAIN_BLOCKS = 8;    // fewest chains side by side
@@ -150,8 +151,13 @@ struct ScanPlace {
     int64_t g;                  // gate of a shared unit
     int64_t bc;                 // b * C + j
     int col_tile;
+    // Where the workgroup's first unit lies, and how far from it the thread's first step of a tile lies in [B,T,C] and
+    // [B,T,G] (elements; below 2^32 bytes: at most 4096 rows of at most SCAN_CHANNELS channels).  The first is the same for
+    // all lanes, and so is the way from step to step: addresses cost no vector instructions beyond the offsets.
+    int64_t b0, j0, g0;
+    unsigned x_off, g_off;
 
-    __device__ __forceinline__ explicit ScanPlace(const ScanShape& s, int64_t block) {
+    __device__ __forceinline__ explicit ScanPlace(const ScanShape& s, unsigned block, int reverse) {
         const int tid = threadIdx.x;
         CL = 1 << s.lcl;
         S = 1 << s.ls;
@@ -177,11 +183,26 @@ struct ScanPlace {
         }
         b = u;
         g = in_b;
+        const unsigned ut0 = block * (SCAN_THREADS >> (s.lcl + s.ls)), u0 = s.col_tiles > 1 ? ut0 / (unsigned)s.col_tiles : ut0;
+        b0 = s.units_per_b > 1 ? u0 / (unsigned)s.units_per_b : u0;
+        g0 = s.units_per_b > 1 ? u0 - (unsigned)b0 * s.units_per_b : 0;
+        j0 = g0 * s.P + (int64_t)(ut0 - u0 * s.col_tiles) * CL * VEC;
         const int col = (col_tile * CL + c) * VEC;
         in_unit = (int64_t)ut < s.unit_tiles;
         on = in_unit && col < s.P;
         j = (int)g * s.P + col;
         bc = b * s.C + j;
+        const unsigned row = (unsigned)(b - b0) * (unsigned)s.T + (unsigned)(reverse ? (S - 1 - sl) * s.steps + s.steps - 1 : sl * s.steps);
+        x_off = row * (unsigned)s.C + (unsigned)(j - (int)j0);
+        g_off = s.G == s.C ? x_off : row * (unsigned)s.G + (unsigned)(g - g0);
+    }
+    // element that x_off (g_off) counts from, for a tile: its first row in memory
+    __device__ __forceinline__ int64_t row0(const ScanShape& s, int64_t tile, int reverse) const {
+        return b0 * s.T + (reverse ? s.T - (tile + 1) * s.tile_steps : tile * s.tile_steps);
+    }
+    __device__ __forceinline__ int64_t x0(const ScanShape& s, int64_t tile, int reverse) const { return row0(s, tile, reverse) * s.C + j0; }
+    __device__ __forceinline__ int64_t gate0(const ScanShape& s, int64_t tile, int reverse) const {
+        return s.G == s.C ? x0(s, tile, reverse) : row0(s, tile, reverse) * s.G + g0;
     }
     // place of step i (in the order of the recurrence) of this thread's columns in a [B,T,C] array / of its gate; from one
     // step to the next it moves by step(C) / step(G)
@@ -201,6 +222,13 @@ struct ScanPlace {
     }
 };
 
+// p + off, p the same for all lanes
+template <class T>
+__device__ __forceinline__ T* lane_at(T* p, unsigned off) {
+    using Byte = std::conditional_t<std::is_const_v<T>, const char, char>;
+    return reinterpret_cast<T*>(reinterpret_cast<Byte*>(p) + (size_t)(off * (unsigned)sizeof(T)));
+}
+
 // K steps of the thread's columns as they lie in memory, in registers.  The conversion to float is done at each use: a
 // value is used two or three times, and kept as it is it takes half the registers where its type has 16 bits.
 template <class T, int N, int K>
@@ -212,14 +240,14 @@ struct Steps {
         if constexpr (sizeof(T) == 4) return __uint_as_float(w[k][v]);
         else return (float)__builtin_bit_cast(T, (unsigned short)(w[k][v / 2] >> (v & 1) * 16));
     }
-    // `count` of the K steps exist; the others read `fill`
-    __device__ __forceinline__ void load(const T* __restrict__ p, int64_t step, int count, float fill) {
+    // `count` of the K steps exist; the others read `fill`.  p, step: the same for all lanes; off: the lane's.
+    __device__ __forceinline__ void load(const T* __restrict__ p, unsigned off, int64_t step, int count, float fill) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             Run<T, N> r;
 #pragma unroll
             for (int v = 0; v < N; ++v) r.v[v] = (T)fill;
-            if (k < count) r = *reinterpret_cast<const Run<T, N>*>(p + k * step);
+            if (k < count) r = *reinterpret_cast<const Run<T, N>*>(lane_at(p + k * step, off));
             if constexpr (sizeof(T) == 4) {
 #pragma unroll
                 for (int i = 0; i < WORDS; ++i) w[k][i] = __builtin_bit_cast(unsigned, r.v[i]);
@@ -233,12 +261,13 @@ struct Steps {
         }
     }
     // All K steps where they are one piece of memory of K * N elements, from its lowest address, a multiple of 16 bytes.
-    __device__ __forceinline__ void load_dense(const T* __restrict__ p, int reverse) {
+    __device__ __forceinline__ void load_dense(const T* __restrict__ p, unsigned off, int reverse) {
+        const unsigned* __restrict__ from = reinterpret_cast<const unsigned*>(lane_at(p, off));
         constexpr int ALL = K * N * sizeof(T) / 4;
         unsigned word[ALL];
 #pragma unroll
         for (int i = 0; i < ALL; i += 4) {
-            const uint4 q = *reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned*>(p) + i);
+            const uint4 q = *reinterpret_cast<const uint4*>(from + i);
             word[i] = q.x; word[i + 1] = q.y; word[i + 2] = q.z; word[i + 3] = q.w;
         }
         const auto half = [&](int e) { return word[e / 2] >> (e & 1) * 16 & 0xffffu; };
@@ -280,7 +309,8 @@ struct Steps {
 
 // The K steps' outputs as one piece of memory.
 template <class T, int K, int N>
-__device__ __forceinline__ void store_dense(T* __restrict__ p, int reverse, const float (&v)[K][N]) {
+__device__ __forceinline__ void store_dense(T* __restrict__ p, unsigned off, int reverse, const float (&v)[K][N]) {
+    unsigned* __restrict__ to = reinterpret_cast<unsigned*>(lane_at(p, off));
     const auto value = [&](int e) { return (T)(reverse ? v[K - 1 - e / N][e % N] : v[e / N][e % N]); };
     constexpr int ALL = K * N * sizeof(T) / 4;
     unsigned word[ALL];
@@ -291,26 +321,32 @@ __device__ __forceinline__ void store_dense(T* __restrict__ p, int reverse, cons
     }
 #pragma unroll
     for (int i = 0; i < ALL; i += 4)
-        *reinterpret_cast<uint4*>(reinterpret_cast<unsigned*>(p) + i) = uint4{word[i], word[i + 1], word[i + 2], word[i + 3]};
+        *reinterpret_cast<uint4*>(to + i) = uint4{word[i], word[i + 1], word[i + 2], word[i + 3]};
 }
 
 // Everywhere below: A [GV], one product for all VEC columns of a lane where they share a gate (GV = 1), else one each.
 template <int GV>
 __device__ __forceinline__ constexpr int scan_gate(int v) { return GV == 1 ? 0 : v; }
 
+// The value of another lane, by its number; beyond the wave's ends it wraps, for lanes that do not use it.
+__device__ __forceinline__ float lane_get(int lane, float v) {
+    return __int_as_float(__builtin_amdgcn_ds_bpermute(lane << 2, __float_as_int(v)));
+}
+
 // Inclusive scan of (A, X) over the slices that the wave holds of the group; UP: from the first slice, else from the last.
 template <bool UP, int VEC, int GV>
 __device__ __forceinline__ void scan_wave(const ScanPlace<VEC>& w, float (&A)[GV], float (&X)[VEC]) {
     for (int d = 1; d < w.SW; d <<= 1) {
         const bool take = UP ? w.slw >= d : w.slw + d < w.SW;
+        const int from = w.lane + (UP ? -d : d) * w.CL;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            const float px = UP ? __shfl_up(X[v], d * w.CL, 64) : __shfl_down(X[v], d * w.CL, 64);
+            const float px = lane_get(from, X[v]);
             if (take) X[v] = scan_apply(A[scan_gate<GV>(v)], px, X[v]);
         }
 #pragma unroll
         for (int g = 0; g < GV; ++g) {
-            const float pa = UP ? __shfl_up(A[g], d * w.CL, 64) : __shfl_down(A[g], d * w.CL, 64);
+            const float pa = lane_get(from, A[g]);
             if (take) A[g] *= pa;
         }
     }
@@ -352,19 +388,20 @@ __device__ __forceinline__ void scan_carry(const ScanPlace<VEC>& w, const float 
     } else {
         const int last = (w.lane & ~(w.CL * w.SW - 1)) + (UP ? (w.SW - 1) * w.CL : 0) + w.c;
 #pragma unroll
-        for (int g = 0; g < GV; ++g) pa[g] = __shfl(A[g], last, 64);
+        for (int g = 0; g < GV; ++g) pa[g] = lane_get(last, A[g]);
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             from[v] = carry[v];
-            carry[v] = scan_apply(pa[scan_gate<GV>(v)], carry[v], __shfl(X[v], last, 64));
+            carry[v] = scan_apply(pa[scan_gate<GV>(v)], carry[v], lane_get(last, X[v]));
         }
     }
     const bool first = UP ? w.slw == 0 : w.slw == w.SW - 1;
+    const int beside = w.lane + (UP ? -w.CL : w.CL);
 #pragma unroll
-    for (int g = 0; g < GV; ++g) pa[g] = UP ? __shfl_up(A[g], w.CL, 64) : __shfl_down(A[g], w.CL, 64);
+    for (int g = 0; g < GV; ++g) pa[g] = lane_get(beside, A[g]);
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-        const float px = UP ? __shfl_up(X[v], w.CL, 64) : __shfl_down(X[v], w.CL, 64);
+        const float px = lane_get(beside, X[v]);
         in[v] = first ? from[v] : scan_apply(pa[scan_gate<GV>(v)], from[v], px);
     }
 }
@@ -409,20 +446,30 @@ __device__ __forceinline__ void scan_fold(const ScanArgs& p, const ScanPlace<VEC
     scan_carry<UP>(w, A, X, carry, in, s_a, s_x);
 }
 
+// APART: f(true_type) or f(false_type), one branch around a sweep over the steps; else f(blend != 0), a select per step --
+// two sweeps take registers, which is dear where a thread holds many values (backward kernel, float, four columns of a
+// shared gate: 183 against 148, 306 us against 269 for 65536 x 192 x 8; one column gains, 52 us against 41 for x 1).
+template <bool APART, class F>
+__device__ __forceinline__ void by_blend(int blend, F&& f) {
+    if (!APART) f(blend != 0);
+    else if (blend) f(std::true_type{});
+    else f(std::false_type{});
+}
+__device__ __forceinline__ float scan_step(bool blend, float a, float h, float x) { return fmaf(a, h, blend ? (1.0f - a) * x : x); }
+
 // (A, X) of the thread's K steps; x is multiplied by its weight first if the recurrence blends.
 template <int VEC, int K, class GT, int GV, class XT>
 __device__ __forceinline__ void scan_local(const Steps<GT, GV, K>& a, const Steps<XT, VEC, K>& x, int blend, float (&A)[GV], float (&X)[VEC]) {
     scan_identity(A, X);
+    by_blend<(K < 16)>(blend, [&](auto blends) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
+        for (int k = 0; k < K; ++k) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const float ak = a(k, v), xk = x(k, v);
-            X[v] = fmaf(ak, X[v], blend ? (1.0f - ak) * xk : xk);
+            for (int v = 0; v < VEC; ++v) X[v] = scan_step(blends, a(k, v), X[v], x(k, v));
+#pragma unroll
+            for (int g = 0; g < GV; ++g) A[g] *= a(k, g);
         }
-#pragma unroll
-        for (int g = 0; g < GV; ++g) A[g] *= a(k, g);
-    }
+    });
 }
 // (A, R) of the same steps from the other end: r_{i-1} = a_i (dh_i + r_i)
 template <int VEC, int K, class GT, int GV, class XT>
@@ -573,7 +620,7 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_segments_kernel(ScanArgs p)
     const ScanShape& s = p.s;
     unsigned block;
     const int64_t seg = scan_segment(s, block) + (BACK ? 1 : 0);
-    const ScanPlace<VEC> w(s, block);
+    const ScanPlace<VEC> w(s, block, p.reverse);
     const int64_t rounds = min(s.seg_tiles, s.tiles - seg * s.seg_tiles);
     const int64_t begin = seg * s.seg_tiles * s.tile_steps + w.sl * rounds * K;   // of the slice's stretch
     const int64_t x_step = p.reverse ? -(int64_t)s.C : s.C, gate_step = p.reverse ? -(int64_t)s.G : s.G;
@@ -584,9 +631,9 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_segments_kernel(ScanArgs p)
     const auto fetch = [&](int64_t n, Steps<GT, GV, K>& to_a, Steps<XT, VEC, K>& to_x) {
         const int64_t i0 = begin + (BACK ? rounds - 1 - n : n) * K;
         const int count = w.count(s, i0);
-        to_a.load(static_cast<const GT*>(p.gate) + w.gate_at(s, i0, p.reverse), gate_step, count, 1.0f);
+        to_a.load(static_cast<const GT*>(p.gate) + w.gate_at(s, i0, p.reverse), 0u, gate_step, count, 1.0f);   // a stretch may be long: whole addresses
         if (BACK && !p.d_h) to_x.clear();
-        else to_x.load(static_cast<const XT*>(BACK ? p.d_h : p.x) + w.at(s, i0, p.reverse), x_step, count, 0.0f);
+        else to_x.load(static_cast<const XT*>(BACK ? p.d_h : p.x) + w.at(s, i0, p.reverse), 0u, x_step, count, 0.0f);
     };
     fetch(0, a_next, x_next);
     for (int64_t n = 0; n < rounds; ++n) {
@@ -628,14 +675,15 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_segments_kernel(ScanArgs p)
 }
 
 // DENSE: a lane has all channels of a sequence and its steps are one piece of memory (few channels, the rays of a picture):
-// they move 16 bytes at a time.  65536 rays x 192 x 3 float: @@ us step by step, @@ so; x 1: @@ and @@.
+// they move 16 bytes at a time.  65536 rays x 192 x 3 float: 107 us step by step, 84 so; x 1: 69 and 29.  (Backward 139 and
+// 121, 106 and 47.)
 template <class GT, class XT, int VEC, int GV, int K, bool CHAIN, bool DENSE>
 __global__ __launch_bounds__(SCAN_THREADS, CHAIN ? 4 : 1) void scan_fwd_kernel(ScanArgs p) {
     __shared__ float s_a[2][4][SCAN_COLS], s_x[2][4][SCAN_COLS], s_part[CHAIN ? CHAIN_GROUP : 1][2][SCAN_COLS];
     const ScanShape& s = p.s;
     unsigned block;
     const int64_t BC = s.B * s.C, segment = scan_segment(s, block), seg = CHAIN ? chain_ticket(p, block) : segment;
-    const ScanPlace<VEC> w(s, block);
+    const ScanPlace<VEC> w(s, block, p.reverse);
     const int64_t t_begin = CHAIN ? seg : seg * s.seg_tiles, t_end = CHAIN ? seg + 1 : min(t_begin + s.seg_tiles, s.tiles);
     float carry[VEC];
 #pragma unroll
@@ -645,21 +693,22 @@ __global__ __launch_bounds__(SCAN_THREADS, CHAIN ? 4 : 1) void scan_fwd_kernel(S
     }
     if (!CHAIN) scan_fold<true, GV>(p, w, seg, s_a[~t_begin & 1], s_x[~t_begin & 1], carry);
     const int64_t x_step = p.reverse ? -(int64_t)s.C : s.C, gate_step = p.reverse ? -(int64_t)s.G : s.G;
+    const unsigned low = p.reverse ? K - 1 : 0;   // rows from a slice's first step to the one that lies first in memory
     Steps<GT, GV, K> a, a_next;
     Steps<XT, VEC, K> x, x_next;
     const auto fetch = [&](int64_t tile, Steps<GT, GV, K>& to_a, Steps<XT, VEC, K>& to_x) {
         const int64_t i0 = tile * s.tile_steps + w.sl * K;
         const int count = tile < t_end ? w.count(s, i0) : 0;
+        const int64_t x0 = w.x0(s, tile, p.reverse), gate0 = w.gate0(s, tile, p.reverse);
         if constexpr (DENSE) {
             if (count == K) {
-                const int64_t low = p.reverse ? i0 + K - 1 : i0;
-                to_a.load_dense(static_cast<const GT*>(p.gate) + w.gate_at(s, low, p.reverse), p.reverse);
-                to_x.load_dense(static_cast<const XT*>(p.x) + w.at(s, low, p.reverse), p.reverse);
+                to_a.load_dense(static_cast<const GT*>(p.gate) + gate0, w.g_off - low * s.G, p.reverse);
+                to_x.load_dense(static_cast<const XT*>(p.x) + x0, w.x_off - low * s.C, p.reverse);
                 return;
             }
         }
-        to_a.load(static_cast<const GT*>(p.gate) + w.gate_at(s, i0, p.reverse), gate_step, count, 1.0f);
-        to_x.load(static_cast<const XT*>(p.x) + w.at(s, i0, p.reverse), x_step, count, 0.0f);
+        to_a.load(static_cast<const GT*>(p.gate) + gate0, w.g_off, gate_step, count, 1.0f);
+        to_x.load(static_cast<const XT*>(p.x) + x0, w.x_off, x_step, count, 0.0f);
     };
     // the next tile is under way while this one is scanned -- where a thread holds few steps: with a shared gate it holds
     // twice as many, and the registers are worth more as a fourth workgroup on the compute unit
@@ -673,7 +722,7 @@ __global__ __launch_bounds__(SCAN_THREADS, CHAIN ? 4 : 1) void scan_fwd_kernel(S
         } else {
             fetch(tile, a, x);
         }
-        const int64_t i0 = tile * s.tile_steps + w.sl * K, at = w.at(s, i0, p.reverse);
+        const int64_t i0 = tile * s.tile_steps + w.sl * K;
         const int count = w.count(s, i0);
         float A[GV], X[VEC], h[VEC];
         scan_local(a, x, p.blend, A, X);
@@ -687,20 +736,27 @@ __global__ __launch_bounds__(SCAN_THREADS, CHAIN ? 4 : 1) void scan_fwd_kernel(S
         if (p.carry && count > 0 && i0 > 0 && (i0 & ((1 << p.l_carry) - 1)) == 0) store_run<VEC>(p.carry + ((i0 >> p.l_carry) - 1) * BC + w.bc, h);
         a.forget();
         x.forget();
-        XT* __restrict__ out = static_cast<XT*>(p.h) + at;
+        XT* __restrict__ out = static_cast<XT*>(p.h) + w.x0(s, tile, p.reverse);
         float piece[DENSE ? K : 1][VEC];
+        by_blend<(K < 16)>(p.blend, [&](auto blends) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
+            for (int k = 0; k < K; ++k) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const float ak = a(k, v), xk = x(k, v);
-                h[v] = fmaf(ak, h[v], p.blend ? (1.0f - ak) * xk : xk);
-                if (DENSE) piece[DENSE ? k : 0][v] = h[v];
+                for (int v = 0; v < VEC; ++v) {
+                    h[v] = scan_step(blends, a(k, v), h[v], x(k, v));
+                    if (DENSE) piece[DENSE ? k : 0][v] = h[v];
+                }
+                if (!DENSE && k < count) store_run<VEC>(lane_at(out + k * x_step, w.x_off), h);
             }
-            if (k < count && !(DENSE && count == K)) store_run<VEC>(out + k * x_step, h);
-        }
+        });
         if constexpr (DENSE) {
-            if (count == K) store_dense(p.reverse ? out + (K - 1) * x_step : out, p.reverse, piece);
+            if (count == K) {
+                store_dense(out, w.x_off - low * s.C, p.reverse, piece);
+            } else {
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    if (k < count) store_run<VEC>(lane_at(out + k * x_step, w.x_off), piece[k]);
+            }
         }
     }
     if (p.last && t_end == s.tiles && w.on && w.sl == 0) store_run<VEC>(p.last + w.bc, carry);
@@ -721,7 +777,7 @@ __device__ __forceinline__ void scan_gate_sums(const ScanArgs& p, const ScanPlac
 #pragma unroll
             for (int j = 0; j < n; ++j) {
                 const float give = upper ? sum[j][0] : sum[j + n][0], keep = upper ? sum[j + n][0] : sum[j][0];
-                sum[j][0] = keep + __shfl_xor(give, d, 64);
+                sum[j][0] = keep + lane_get(w.lane ^ d, give);
             }
             first += upper ? n : 0;
             d <<= 1;
@@ -730,7 +786,7 @@ __device__ __forceinline__ void scan_gate_sums(const ScanArgs& p, const ScanPlac
     const int held = K / d;
     bool writes = true;
     for (; d < w.CL; d <<= 1) {
-        sum[0][0] += __shfl_xor(sum[0][0], d, 64);
+        sum[0][0] += lane_get(w.lane ^ d, sum[0][0]);
         writes = writes && !(w.c & d);
     }
 #pragma unroll
@@ -752,7 +808,7 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
     const ScanShape& s = p.s;
     unsigned block;
     const int64_t seg = scan_segment(s, block), BC = s.B * s.C;
-    const ScanPlace<VEC> w(s, block);
+    const ScanPlace<VEC> w(s, block, p.reverse);
     const int64_t t_begin = seg * s.seg_tiles, t_end = min(t_begin + s.seg_tiles, s.tiles);
     const bool shared_gate = s.G != s.C;
     float r_carry[VEC];
@@ -766,25 +822,25 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
     // (the next tile under way as in the forward pass was slower here: 151 registers against 119, 240 us against 215 for a
     // bfloat16 sequence of 65536 x 1024)
     for (int64_t tile = t_end - 1; tile >= t_begin; --tile) {
-        const int64_t i0 = tile * s.tile_steps + w.sl * K, at = w.at(s, i0, p.reverse), gate_at = w.gate_at(s, i0, p.reverse);
+        const int64_t i0 = tile * s.tile_steps + w.sl * K, x0 = w.x0(s, tile, p.reverse), gate0 = w.gate0(s, tile, p.reverse);
         const int count = w.count(s, i0);
         Steps<GT, GV, K> a;
         Steps<XT, VEC, K> x, dh;
         float A[GV], X[VEC], h[VEC], r[VEC], carry[VEC];
-        const int64_t low = DENSE && p.reverse ? at + (K - 1) * x_step : at, gate_low = DENSE && p.reverse ? gate_at + (K - 1) * gate_step : gate_at;
+        const unsigned low = p.reverse ? K - 1 : 0, x_low = w.x_off - low * s.C, gate_low = w.g_off - low * s.G;
         const bool whole = DENSE && count == K;
         if constexpr (DENSE) {
             if (whole) {
-                a.load_dense(static_cast<const GT*>(p.gate) + gate_low, p.reverse);
-                x.load_dense(static_cast<const XT*>(p.x) + low, p.reverse);
-                if (p.d_h) dh.load_dense(static_cast<const XT*>(p.d_h) + low, p.reverse);
+                a.load_dense(static_cast<const GT*>(p.gate) + gate0, gate_low, p.reverse);
+                x.load_dense(static_cast<const XT*>(p.x) + x0, x_low, p.reverse);
+                if (p.d_h) dh.load_dense(static_cast<const XT*>(p.d_h) + x0, x_low, p.reverse);
                 else dh.clear();
             }
         }
         if (!whole) {
-            a.load(static_cast<const GT*>(p.gate) + gate_at, gate_step, count, 1.0f);
-            x.load(static_cast<const XT*>(p.x) + at, x_step, count, 0.0f);
-            if (p.d_h) dh.load(static_cast<const XT*>(p.d_h) + at, x_step, count, 0.0f);
+            a.load(static_cast<const GT*>(p.gate) + gate0, w.g_off, gate_step, count, 1.0f);
+            x.load(static_cast<const XT*>(p.x) + x0, w.x_off, x_step, count, 0.0f);
+            if (p.d_h) dh.load(static_cast<const XT*>(p.d_h) + x0, w.x_off, x_step, count, 0.0f);
             else dh.clear();
         }
 #pragma unroll
@@ -805,42 +861,48 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
         a.forget();
         x.forget();
         dh.forget();
-        float beside[K][VEC];   // what multiplies g in the gradient of the gate
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const float ak = a(k, v), xk = x(k, v);
-                beside[k][v] = p.blend ? h[v] - xk : h[v];
-                h[v] = fmaf(ak, h[v], p.blend ? (1.0f - ak) * xk : xk);
-            }
-        XT* __restrict__ dx_out = static_cast<XT*>(p.d_x) + at;
-        GT* __restrict__ da_out = static_cast<GT*>(p.d_gate) + gate_at;
+        XT* __restrict__ dx_out = static_cast<XT*>(p.d_x) + x0;
+        GT* __restrict__ da_out = static_cast<GT*>(p.d_gate) + gate0;
         float dx_piece[DENSE ? K : 1][VEC], da_sum[K][1];
+        by_blend<VEC == 1>(p.blend, [&](auto blends) {
+            const bool blend = blends;
+            float beside[K][VEC];   // what multiplies g in the gradient of the gate
 #pragma unroll
-        for (int k = K - 1; k >= 0; --k) {
-            float da[VEC], dx[VEC];
+            for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const float ak = a(k, v), g = dh(k, v) + r[v];
-                da[v] = g * beside[k][v];
-                dx[v] = p.blend ? (1.0f - ak) * g : g;
-                r[v] = ak * g;
-                if (DENSE) dx_piece[DENSE ? k : 0][v] = dx[v];
+                for (int v = 0; v < VEC; ++v) {
+                    beside[k][v] = blend ? h[v] - x(k, v) : h[v];
+                    h[v] = scan_step(blend, a(k, v), h[v], x(k, v));
+                }
+#pragma unroll
+            for (int k = K - 1; k >= 0; --k) {
+                float da[VEC], dx[VEC];
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    const float ak = a(k, v), g = dh(k, v) + r[v];
+                    da[v] = g * beside[k][v];
+                    dx[v] = blend ? (1.0f - ak) * g : g;
+                    r[v] = ak * g;
+                    if (DENSE) dx_piece[DENSE ? k : 0][v] = dx[v];
+                }
+                if (!DENSE && p.d_x && k < count) store_run<VEC>(lane_at(dx_out + k * x_step, w.x_off), dx);
+                da_sum[k][0] = da[0];
+                if (GV == 1) {
+#pragma unroll
+                    for (int v = 1; v < VEC; ++v) da_sum[k][0] += da[v];
+                } else if (p.d_gate && k < count) {
+                    store_run<VEC>(lane_at(da_out + k * gate_step, w.g_off), da);
+                }
             }
-            if (p.d_x && k < count && !whole) store_run<VEC>(dx_out + k * x_step, dx);
-            da_sum[k][0] = da[0];
-            if (GV == 1) {
-#pragma unroll
-                for (int v = 1; v < VEC; ++v) da_sum[k][0] += da[v];
-            } else if (p.d_gate && k < count) {
-                store_run<VEC>(da_out + k * gate_step, da);
-            }
-        }
+        });
         if constexpr (DENSE) {
             if (whole) {
-                if (p.d_x) store_dense(static_cast<XT*>(p.d_x) + low, p.reverse, dx_piece);
-                if (p.d_gate) store_dense(static_cast<GT*>(p.d_gate) + gate_low, p.reverse, da_sum);
+                if (p.d_x) store_dense(dx_out, x_low, p.reverse, dx_piece);
+                if (p.d_gate) store_dense(da_out, gate_low, p.reverse, da_sum);
+            } else {
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    if (p.d_x && k < count) store_run<VEC>(lane_at(dx_out + k * x_step, w.x_off), dx_piece[k]);
             }
         }
         if constexpr (GV == 1) {
@@ -848,9 +910,9 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
             if (!shared_gate) {
 #pragma unroll
                 for (int k = 0; k < K; ++k)
-                    if (k < count) da_out[k * gate_step] = (GT)da_sum[k][0];
+                    if (k < count) *lane_at(da_out + k * gate_step, w.g_off) = (GT)da_sum[k][0];
             } else {
-                scan_gate_sums(p, w, da_sum, w.count_in_unit(s, i0), da_out, gate_at, gate_step);   // lanes without columns write too
+                scan_gate_sums(p, w, da_sum, w.count_in_unit(s, i0), lane_at(da_out, w.g_off), w.gate_at(s, i0, p.reverse), gate_step);   // lanes without columns write too
             }
         }
     }
@@ -947,6 +1009,7 @@ static int scan_check(const char* who, int64_t B, int64_t T, int C, int G, int g
     NERF_REQUIRE(B >= 0 && T >= 0 && C >= 0 && G >= 0, "%s: B=%lld T=%lld C=%d G=%d", who, (long long)B, (long long)T, C, G);
     NERF_REQUIRE(C == 0 || (G > 0 && C % G == 0), "%s: %d gates do not divide %d channels", who, G, C);
     NERF_REQUIRE(known_type(x_type) && (gate_type == NERF_F32 || gate_type == x_type), "%s: gate type %d with x type %d", who, gate_type, x_type);
+    NERF_REQUIRE(C <= SCAN_CHANNELS, "%s: %d channels, at most %d", who, C, SCAN_CHANNELS);
     if (B == 0 || T == 0 || C == 0) return NERF_OK;
     NERF_REQUIRE(B <= (1ll << 40) && T <= (1ll << 40) && B * (double)T * C < 9e17, "%s: too large", who);
     const ScanShape s = scan_shape(B, T, C, G);

@@ -542,7 +542,7 @@ def linear_scan(gate: torch.Tensor, x: torch.Tensor, state: Optional[torch.Tenso
     channel, G = 1 one per step, anything between heads.  ``state`` [..., C]: h before the first step (zeros if None).
     float32, bfloat16 or float16; a gate of another type than ``x`` is taken as float32.  The state is held in float32
     and h rounded once to the type of ``x``.  A gate of zero starts a new sequence.  Gates are meant to lie in [-1, 1];
-    larger ones are right while float32 holds their products.
+    larger ones are right while float32 holds their products.  At most 131072 channels.
     ``return_state``: ``(h, last)``, ``last`` [..., C] float32 the state after the last step, unrounded: what the next call
     takes as ``state`` (a long sequence in parts, or one step at a time with T = 1).
     Differentiable once in ``gate``, ``x`` and ``state``."""

@@ -316,6 +316,29 @@ def test_streams_and_graph(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [3, 900])
+@pytest.mark.parametrize("G", [32768, 131072, 1])
+def test_most_channels(dev, T, G):
+    """The widest rows, with a gate for every few columns, a gate each and one for all: some columns in 64 bits."""
+    from nerf_amd import ops
+    B, C = 2, 131072
+    gen = torch.Generator(device=dev).manual_seed(T)
+    gate = torch.rand(B, T, G, device=dev, generator=gen).requires_grad_(True)
+    x = torch.empty(B, T, C, device=dev).normal_(generator=gen).requires_grad_(True)
+    h = ops.linear_scan(gate, x, reverse=True, blend=True)
+    d_gate, d_x = torch.autograd.grad(h, [gate, x], x.detach())
+    for c in (0, 65532, C - 8):
+        cols = slice(c, c + 8)
+        gates = slice(c * G // C, max((c + 8) * G // C, 1))
+        g, v = gate.detach()[..., gates].cpu(), x.detach()[..., cols].cpu()
+        want, tol = ref_scan(g, v, None, True, True, v, None), bounds(g, v, None, True, True, v, None)
+        assert_close(h[..., cols], want[0], tol[0], ("h", c))
+        assert_close(d_x[..., cols], want[3], tol[3], ("d_x", c))
+        if G > 1:
+            assert_close(d_gate[..., gates], want[2], tol[2], ("d_gate", c))
+
+
+@pytest.mark.gpu
 def test_more_than_two_to_the_31_elements(dev):
     """Offsets past 32 bits: the last rows of a large batch against the same rows alone."""
     from nerf_amd import ops
@@ -364,7 +387,7 @@ def test_entry_points_refuse():
             a[int(i[1:])] = v
         return lib.nerf_linear_scan_fwd(*a)
     for k in ({"_0": None}, {"_2": None}, {"_11": None}, {"_1": 3}, {"_1": 1}, {"_3": 7}, {"_8": 3}, {"_8": 0}, {"_5": -1}, {"_6": 0}, {"_0": odd}, {"_2": odd},
-              {"_11": odd}, {"_4": odd}, {"_12": odd}, {"_13": odd}, {"_5": 1 << 50}, {"_6": 1 << 39, "_5": 1}):
+              {"_11": odd}, {"_4": odd}, {"_12": odd}, {"_13": odd}, {"_5": 1 << 50}, {"_6": 1 << 39, "_5": 1}, {"_7": (1 << 17) + 2}):
         assert fwd(**k) == -22, k
         assert lib.nerf_last_error()
     assert fwd(_5=0) == 0 and fwd(_7=0) == 0   # nothing to do
