@@ -151,9 +151,8 @@ struct ScanPlace {
     int64_t g;                  // gate of a shared unit
     int64_t bc;                 // b * C + j
     int col_tile;
-    // Where the workgroup's first unit lies, and how far from it the thread's first step of a tile lies in [B,T,C] and
-    // [B,T,G] (elements; below 2^32 bytes: at most 4096 rows of at most SCAN_CHANNELS channels).  The first is the same for
-    // all lanes, and so is the way from step to step: addresses cost no vector instructions beyond the offsets.
+    // Where the workgroup's first unit lies, and how far from it the slice's first step does, in [B,T,C] and [B,T,G]
+    // (elements; at most 2^30 bytes: 2048 rows of at most SCAN_CHANNELS channels, or 4096 of 16 bits).
     int64_t b0, j0, g0;
     unsigned x_off, g_off;
 
@@ -222,13 +221,42 @@ struct ScanPlace {
     }
 };
 
-// p + off, p the same for all lanes
-template <class T>
-__device__ __forceinline__ T* lane_at(T* p, unsigned off) {
-    using Byte = std::conditional_t<std::is_const_v<T>, const char, char>;
-    return reinterpret_cast<T*>(reinterpret_cast<Byte*>(p) + (size_t)(off * (unsigned)sizeof(T)));
+// Reads from an address that is the same for all lanes on, at 32-bit offsets of the lanes' own, in bytes, below BUFFER_END.
+// An offset of BUFFER_END or more reads zeros: steps that do not exist need no branch, and addresses no 64-bit arithmetic.
+// (Writes go by ordinary addresses: after a 16-byte buffer store with an offset in a scalar register the compiler lets the
+// stored registers be overwritten while they are still being read.)
+constexpr unsigned BUFFER_END = 0x7fffffffu, BUFFER_NONE = 0x80000000u;
+using Buffer = __amdgpu_buffer_rsrc_t;
+__device__ __forceinline__ Buffer buffer(const void* p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)BUFFER_END, 4 << 15 | 7 << 12);   // 32-bit words
 }
-
+typedef unsigned Words2 __attribute__((ext_vector_type(2)));
+typedef unsigned Words3 __attribute__((ext_vector_type(3)));
+typedef unsigned Words4 __attribute__((ext_vector_type(4)));
+// N elements of T as they lie in memory
+template <class T, int N>
+__device__ __forceinline__ void buffer_load(Buffer p, unsigned off, unsigned (&w)[(sizeof(T) * N + 3) / 4]) {
+    constexpr int BYTES = sizeof(T) * N;
+    if constexpr (BYTES == 2) {
+        w[0] = __builtin_amdgcn_raw_buffer_load_b16(p, off, 0, 0);
+    } else if constexpr (BYTES == 4) {
+        w[0] = __builtin_amdgcn_raw_buffer_load_b32(p, off, 0, 0);
+    } else if constexpr (BYTES == 6) {
+        const unsigned lo = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(p, off, 0, 0), hi = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(p, off + 2, 0, 0);
+        w[0] = lo | hi << 16;
+        w[1] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(p, off + 4, 0, 0);
+    } else if constexpr (BYTES == 8) {
+        const Words2 q = __builtin_amdgcn_raw_buffer_load_b64(p, off, 0, 0);
+        w[0] = q.x; w[1] = q.y;
+    } else if constexpr (BYTES == 12) {
+        const Words3 q = __builtin_amdgcn_raw_buffer_load_b96(p, off, 0, 0);
+        w[0] = q.x; w[1] = q.y; w[2] = q.z;
+    } else {
+        static_assert(BYTES == 16, "");
+        const Words4 q = __builtin_amdgcn_raw_buffer_load_b128(p, off, 0, 0);
+        w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+    }
+}
 // K steps of the thread's columns as they lie in memory, in registers.  The conversion to float is done at each use: a
 // value is used two or three times, and kept as it is it takes half the registers where its type has 16 bits.
 template <class T, int N, int K>
@@ -240,14 +268,14 @@ struct Steps {
         if constexpr (sizeof(T) == 4) return __uint_as_float(w[k][v]);
         else return (float)__builtin_bit_cast(T, (unsigned short)(w[k][v / 2] >> (v & 1) * 16));
     }
-    // `count` of the K steps exist; the others read `fill`.  p, step: the same for all lanes; off: the lane's.
-    __device__ __forceinline__ void load(const T* __restrict__ p, unsigned off, int64_t step, int count, float fill) {
+    // `count` of the K steps exist; the others read `fill`.
+    __device__ __forceinline__ void load(const T* __restrict__ p, int64_t step, int count, float fill) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             Run<T, N> r;
 #pragma unroll
             for (int v = 0; v < N; ++v) r.v[v] = (T)fill;
-            if (k < count) r = *reinterpret_cast<const Run<T, N>*>(lane_at(p + k * step, off));
+            if (k < count) r = *reinterpret_cast<const Run<T, N>*>(p + k * step);
             if constexpr (sizeof(T) == 4) {
 #pragma unroll
                 for (int i = 0; i < WORDS; ++i) w[k][i] = __builtin_bit_cast(unsigned, r.v[i]);
@@ -260,14 +288,27 @@ struct Steps {
             }
         }
     }
+    // The same through a buffer, the first step at off, the next ones `step` bytes on (modulo 2^32).
+    __device__ __forceinline__ void load(Buffer p, unsigned off, unsigned step, int count, float fill) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) buffer_load<T, N>(p, k < count ? off + k * step : BUFFER_NONE, w[k]);
+        if (fill != 0.0f && count < K) {   // (zeros were read)
+            unsigned bits;
+            if constexpr (sizeof(T) == 4) bits = __float_as_uint(fill);
+            else bits = 0x10001u * __builtin_bit_cast(unsigned short, (T)fill);
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int i = 0; i < WORDS; ++i) w[k][i] = k < count ? w[k][i] : bits;
+        }
+    }
     // All K steps where they are one piece of memory of K * N elements, from its lowest address, a multiple of 16 bytes.
-    __device__ __forceinline__ void load_dense(const T* __restrict__ p, unsigned off, int reverse) {
-        const unsigned* __restrict__ from = reinterpret_cast<const unsigned*>(lane_at(p, off));
+    __device__ __forceinline__ void load_dense(const T* __restrict__ p, int reverse) {
         constexpr int ALL = K * N * sizeof(T) / 4;
         unsigned word[ALL];
 #pragma unroll
         for (int i = 0; i < ALL; i += 4) {
-            const uint4 q = *reinterpret_cast<const uint4*>(from + i);
+            const uint4 q = *reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned*>(p) + i);
             word[i] = q.x; word[i + 1] = q.y; word[i + 2] = q.z; word[i + 3] = q.w;
         }
         const auto half = [&](int e) { return word[e / 2] >> (e & 1) * 16 & 0xffffu; };
@@ -309,8 +350,7 @@ struct Steps {
 
 // The K steps' outputs as one piece of memory.
 template <class T, int K, int N>
-__device__ __forceinline__ void store_dense(T* __restrict__ p, unsigned off, int reverse, const float (&v)[K][N]) {
-    unsigned* __restrict__ to = reinterpret_cast<unsigned*>(lane_at(p, off));
+__device__ __forceinline__ void store_dense(T* __restrict__ p, int reverse, const float (&v)[K][N]) {
     const auto value = [&](int e) { return (T)(reverse ? v[K - 1 - e / N][e % N] : v[e / N][e % N]); };
     constexpr int ALL = K * N * sizeof(T) / 4;
     unsigned word[ALL];
@@ -321,7 +361,7 @@ __device__ __forceinline__ void store_dense(T* __restrict__ p, unsigned off, int
     }
 #pragma unroll
     for (int i = 0; i < ALL; i += 4)
-        *reinterpret_cast<uint4*>(to + i) = uint4{word[i], word[i + 1], word[i + 2], word[i + 3]};
+        *reinterpret_cast<uint4*>(reinterpret_cast<unsigned*>(p) + i) = uint4{word[i], word[i + 1], word[i + 2], word[i + 3]};
 }
 
 // Everywhere below: A [GV], one product for all VEC columns of a lane where they share a gate (GV = 1), else one each.
@@ -448,7 +488,7 @@ __device__ __forceinline__ void scan_fold(const ScanArgs& p, const ScanPlace<VEC
 
 // APART: f(true_type) or f(false_type), one branch around a sweep over the steps; else f(blend != 0), a select per step --
 // two sweeps take registers, which is dear where a thread holds many values (backward kernel, float, four columns of a
-// shared gate: 183 against 148, 306 us against 269 for 65536 x 192 x 8; one column gains, 52 us against 41 for x 1).
+// shared gate: 306 us against 269 for 65536 x 192 x 8; one column gains, 52 us against 43 for x 1).
 template <bool APART, class F>
 __device__ __forceinline__ void by_blend(int blend, F&& f) {
     if (!APART) f(blend != 0);
@@ -631,9 +671,9 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_segments_kernel(ScanArgs p)
     const auto fetch = [&](int64_t n, Steps<GT, GV, K>& to_a, Steps<XT, VEC, K>& to_x) {
         const int64_t i0 = begin + (BACK ? rounds - 1 - n : n) * K;
         const int count = w.count(s, i0);
-        to_a.load(static_cast<const GT*>(p.gate) + w.gate_at(s, i0, p.reverse), 0u, gate_step, count, 1.0f);   // a stretch may be long: whole addresses
+        to_a.load(static_cast<const GT*>(p.gate) + w.gate_at(s, i0, p.reverse), gate_step, count, 1.0f);   // a stretch may be long: whole addresses
         if (BACK && !p.d_h) to_x.clear();
-        else to_x.load(static_cast<const XT*>(BACK ? p.d_h : p.x) + w.at(s, i0, p.reverse), 0u, x_step, count, 0.0f);
+        else to_x.load(static_cast<const XT*>(BACK ? p.d_h : p.x) + w.at(s, i0, p.reverse), x_step, count, 0.0f);
     };
     fetch(0, a_next, x_next);
     for (int64_t n = 0; n < rounds; ++n) {
@@ -674,9 +714,15 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_segments_kernel(ScanArgs p)
     }
 }
 
+// Whether a kernel reads through buffers: with four columns to a lane (16384 x 192 x 32 bfloat16, one gate a step, backward:
+// 164 us, by ordinary addresses 250).  With one column lanes without any still make their requests: 65536 x 192 x 5 float took
+// 245 us so against 198 forward and 429 against 377 backward, 65536 x 64 x 4 in dense pieces 50 against 47 backward.
+template <int VEC, bool DENSE>
+constexpr bool scan_buffers() { return VEC == 4 && !DENSE; }
+
 // DENSE: a lane has all channels of a sequence and its steps are one piece of memory (few channels, the rays of a picture):
-// they move 16 bytes at a time.  65536 rays x 192 x 3 float: 107 us step by step, 84 so; x 1: 69 and 29.  (Backward 139 and
-// 121, 106 and 47.)
+// they move 16 bytes at a time.  65536 rays x 192 x 3 float: 107 us step by step, 82 so; x 1: 69 and 27.  (Backward 139 and
+// 120, 106 and 43.)
 template <class GT, class XT, int VEC, int GV, int K, bool CHAIN, bool DENSE>
 __global__ __launch_bounds__(SCAN_THREADS, CHAIN ? 4 : 1) void scan_fwd_kernel(ScanArgs p) {
     __shared__ float s_a[2][4][SCAN_COLS], s_x[2][4][SCAN_COLS], s_part[CHAIN ? CHAIN_GROUP : 1][2][SCAN_COLS];
@@ -693,22 +739,28 @@ __global__ __launch_bounds__(SCAN_THREADS, CHAIN ? 4 : 1) void scan_fwd_kernel(S
     }
     if (!CHAIN) scan_fold<true, GV>(p, w, seg, s_a[~t_begin & 1], s_x[~t_begin & 1], carry);
     const int64_t x_step = p.reverse ? -(int64_t)s.C : s.C, gate_step = p.reverse ? -(int64_t)s.G : s.G;
-    const unsigned low = p.reverse ? K - 1 : 0;   // rows from a slice's first step to the one that lies first in memory
+    const int64_t low = p.reverse ? K - 1 : 0;   // rows from a slice's first step to the one that lies first in memory
     Steps<GT, GV, K> a, a_next;
     Steps<XT, VEC, K> x, x_next;
     const auto fetch = [&](int64_t tile, Steps<GT, GV, K>& to_a, Steps<XT, VEC, K>& to_x) {
         const int64_t i0 = tile * s.tile_steps + w.sl * K;
         const int count = tile < t_end ? w.count(s, i0) : 0;
-        const int64_t x0 = w.x0(s, tile, p.reverse), gate0 = w.gate0(s, tile, p.reverse);
-        if constexpr (DENSE) {
-            if (count == K) {
-                to_a.load_dense(static_cast<const GT*>(p.gate) + gate0, w.g_off - low * s.G, p.reverse);
-                to_x.load_dense(static_cast<const XT*>(p.x) + x0, w.x_off - low * s.C, p.reverse);
-                return;
+        if constexpr (scan_buffers<VEC, DENSE>()) {
+            to_a.load(buffer(static_cast<const GT*>(p.gate) + w.gate0(s, tile, p.reverse)), w.g_off * sizeof(GT), (unsigned)gate_step * sizeof(GT), count, 1.0f);
+            to_x.load(buffer(static_cast<const XT*>(p.x) + w.x0(s, tile, p.reverse)), w.x_off * sizeof(XT), (unsigned)x_step * sizeof(XT), count, 0.0f);
+        } else {
+            const GT* __restrict__ gate_from = static_cast<const GT*>(p.gate) + w.gate_at(s, i0, p.reverse);
+            const XT* __restrict__ x_from = static_cast<const XT*>(p.x) + w.at(s, i0, p.reverse);
+            if constexpr (DENSE) {
+                if (count == K) {
+                    to_a.load_dense(gate_from - low * s.G, p.reverse);
+                    to_x.load_dense(x_from - low * s.C, p.reverse);
+                    return;
+                }
             }
+            to_a.load(gate_from, gate_step, count, 1.0f);
+            to_x.load(x_from, x_step, count, 0.0f);
         }
-        to_a.load(static_cast<const GT*>(p.gate) + gate0, w.g_off, gate_step, count, 1.0f);
-        to_x.load(static_cast<const XT*>(p.x) + x0, w.x_off, x_step, count, 0.0f);
     };
     // the next tile is under way while this one is scanned -- where a thread holds few steps: with a shared gate it holds
     // twice as many, and the registers are worth more as a fourth workgroup on the compute unit
@@ -736,7 +788,7 @@ __global__ __launch_bounds__(SCAN_THREADS, CHAIN ? 4 : 1) void scan_fwd_kernel(S
         if (p.carry && count > 0 && i0 > 0 && (i0 & ((1 << p.l_carry) - 1)) == 0) store_run<VEC>(p.carry + ((i0 >> p.l_carry) - 1) * BC + w.bc, h);
         a.forget();
         x.forget();
-        XT* __restrict__ out = static_cast<XT*>(p.h) + w.x0(s, tile, p.reverse);
+        XT* __restrict__ out = static_cast<XT*>(p.h) + w.at(s, i0, p.reverse);
         float piece[DENSE ? K : 1][VEC];
         by_blend<(K < 16)>(p.blend, [&](auto blends) {
 #pragma unroll
@@ -746,16 +798,16 @@ __global__ __launch_bounds__(SCAN_THREADS, CHAIN ? 4 : 1) void scan_fwd_kernel(S
                     h[v] = scan_step(blends, a(k, v), h[v], x(k, v));
                     if (DENSE) piece[DENSE ? k : 0][v] = h[v];
                 }
-                if (!DENSE && k < count) store_run<VEC>(lane_at(out + k * x_step, w.x_off), h);
+                if (!DENSE && k < count) store_run<VEC>(out + k * x_step, h);
             }
         });
         if constexpr (DENSE) {
             if (count == K) {
-                store_dense(out, w.x_off - low * s.C, p.reverse, piece);
+                store_dense(out - low * s.C, p.reverse, piece);
             } else {
 #pragma unroll
                 for (int k = 0; k < K; ++k)
-                    if (k < count) store_run<VEC>(lane_at(out + k * x_step, w.x_off), piece[k]);
+                    if (k < count) store_run<VEC>(out + k * x_step, piece[k]);
             }
         }
     }
@@ -819,29 +871,41 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
     }
     scan_fold<false, GV>(p, w, seg, s_b[t_end & 1], s_r[t_end & 1], r_carry);
     const int64_t x_step = p.reverse ? -(int64_t)s.C : s.C, gate_step = p.reverse ? -(int64_t)s.G : s.G;
+    const int64_t low = p.reverse ? K - 1 : 0;
     // (the next tile under way as in the forward pass was slower here: 151 registers against 119, 240 us against 215 for a
     // bfloat16 sequence of 65536 x 1024)
     for (int64_t tile = t_end - 1; tile >= t_begin; --tile) {
-        const int64_t i0 = tile * s.tile_steps + w.sl * K, x0 = w.x0(s, tile, p.reverse), gate0 = w.gate0(s, tile, p.reverse);
+        const int64_t i0 = tile * s.tile_steps + w.sl * K, at = w.at(s, i0, p.reverse), gate_at = w.gate_at(s, i0, p.reverse);
         const int count = w.count(s, i0);
         Steps<GT, GV, K> a;
         Steps<XT, VEC, K> x, dh;
         float A[GV], X[VEC], h[VEC], r[VEC], carry[VEC];
-        const unsigned low = p.reverse ? K - 1 : 0, x_low = w.x_off - low * s.C, gate_low = w.g_off - low * s.G;
         const bool whole = DENSE && count == K;
-        if constexpr (DENSE) {
-            if (whole) {
-                a.load_dense(static_cast<const GT*>(p.gate) + gate0, gate_low, p.reverse);
-                x.load_dense(static_cast<const XT*>(p.x) + x0, x_low, p.reverse);
-                if (p.d_h) dh.load_dense(static_cast<const XT*>(p.d_h) + x0, x_low, p.reverse);
+        if constexpr (scan_buffers<VEC, DENSE>()) {
+            const int64_t x0 = w.x0(s, tile, p.reverse);
+            const unsigned x_next = (unsigned)x_step * sizeof(XT);
+            a.load(buffer(static_cast<const GT*>(p.gate) + w.gate0(s, tile, p.reverse)), w.g_off * sizeof(GT), (unsigned)gate_step * sizeof(GT), count, 1.0f);
+            x.load(buffer(static_cast<const XT*>(p.x) + x0), w.x_off * sizeof(XT), x_next, count, 0.0f);
+            if (p.d_h) dh.load(buffer(static_cast<const XT*>(p.d_h) + x0), w.x_off * sizeof(XT), x_next, count, 0.0f);
+            else dh.clear();
+        } else {
+            const GT* __restrict__ gate_from = static_cast<const GT*>(p.gate) + gate_at;
+            const XT* __restrict__ x_from = static_cast<const XT*>(p.x) + at;
+            const XT* __restrict__ dh_from = static_cast<const XT*>(p.d_h) + at;
+            if constexpr (DENSE) {
+                if (whole) {
+                    a.load_dense(gate_from - low * s.G, p.reverse);
+                    x.load_dense(x_from - low * s.C, p.reverse);
+                    if (p.d_h) dh.load_dense(dh_from - low * s.C, p.reverse);
+                    else dh.clear();
+                }
+            }
+            if (!whole) {
+                a.load(gate_from, gate_step, count, 1.0f);
+                x.load(x_from, x_step, count, 0.0f);
+                if (p.d_h) dh.load(dh_from, x_step, count, 0.0f);
                 else dh.clear();
             }
-        }
-        if (!whole) {
-            a.load(static_cast<const GT*>(p.gate) + gate0, w.g_off, gate_step, count, 1.0f);
-            x.load(static_cast<const XT*>(p.x) + x0, w.x_off, x_step, count, 0.0f);
-            if (p.d_h) dh.load(static_cast<const XT*>(p.d_h) + x0, w.x_off, x_step, count, 0.0f);
-            else dh.clear();
         }
 #pragma unroll
         for (int v = 0; v < VEC; ++v) carry[v] = 0.0f;
@@ -861,8 +925,8 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
         a.forget();
         x.forget();
         dh.forget();
-        XT* __restrict__ dx_out = static_cast<XT*>(p.d_x) + x0;
-        GT* __restrict__ da_out = static_cast<GT*>(p.d_gate) + gate0;
+        XT* __restrict__ dx_out = static_cast<XT*>(p.d_x) + at;
+        GT* __restrict__ da_out = static_cast<GT*>(p.d_gate) + gate_at;
         float dx_piece[DENSE ? K : 1][VEC], da_sum[K][1];
         by_blend<VEC == 1>(p.blend, [&](auto blends) {
             const bool blend = blends;
@@ -885,24 +949,24 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
                     r[v] = ak * g;
                     if (DENSE) dx_piece[DENSE ? k : 0][v] = dx[v];
                 }
-                if (!DENSE && p.d_x && k < count) store_run<VEC>(lane_at(dx_out + k * x_step, w.x_off), dx);
+                if (!DENSE && p.d_x && k < count) store_run<VEC>(dx_out + k * x_step, dx);
                 da_sum[k][0] = da[0];
                 if (GV == 1) {
 #pragma unroll
                     for (int v = 1; v < VEC; ++v) da_sum[k][0] += da[v];
                 } else if (p.d_gate && k < count) {
-                    store_run<VEC>(lane_at(da_out + k * gate_step, w.g_off), da);
+                    store_run<VEC>(da_out + k * gate_step, da);
                 }
             }
         });
         if constexpr (DENSE) {
             if (whole) {
-                if (p.d_x) store_dense(dx_out, x_low, p.reverse, dx_piece);
-                if (p.d_gate) store_dense(da_out, gate_low, p.reverse, da_sum);
+                if (p.d_x) store_dense(dx_out - low * s.C, p.reverse, dx_piece);
+                if (p.d_gate) store_dense(da_out - low * s.G, p.reverse, da_sum);
             } else {
 #pragma unroll
                 for (int k = 0; k < K; ++k)
-                    if (p.d_x && k < count) store_run<VEC>(lane_at(dx_out + k * x_step, w.x_off), dx_piece[k]);
+                    if (p.d_x && k < count) store_run<VEC>(dx_out + k * x_step, dx_piece[k]);
             }
         }
         if constexpr (GV == 1) {
@@ -910,9 +974,9 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
             if (!shared_gate) {
 #pragma unroll
                 for (int k = 0; k < K; ++k)
-                    if (k < count) *lane_at(da_out + k * gate_step, w.g_off) = (GT)da_sum[k][0];
+                    if (k < count) da_out[k * gate_step] = (GT)da_sum[k][0];
             } else {
-                scan_gate_sums(p, w, da_sum, w.count_in_unit(s, i0), lane_at(da_out, w.g_off), w.gate_at(s, i0, p.reverse), gate_step);   // lanes without columns write too
+                scan_gate_sums(p, w, da_sum, w.count_in_unit(s, i0), da_out, gate_at, gate_step);   // lanes without columns write too
             }
         }
     }
