@@ -90,6 +90,14 @@ class FusedAdam(torch.optim.Optimizer):
                        for k, st in sd["state"].items()}
         return sd
 
+    def __getstate__(self):   # copies and pickles; torch's own holds the defaults, the state and the groups
+        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm}
+
+    def __setstate__(self, state):   # (load_state_dict calls it too, on an optimiser that has these)
+        super().__setstate__(state)
+        for name, value in (("max_grad_norm", None), ("_norm", None), ("_dev_state", {}), ("_dev_lr", {})):
+            self.__dict__.setdefault(name, value)
+
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
         self._dev_state = {}   # rebuilt from the loaded step counts on the next step

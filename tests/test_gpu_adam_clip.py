@@ -232,6 +232,38 @@ def test_another_stream(dev):
     assert all(torch.equal(x, y) for x, y in zip(*got))
 
 
+def test_copies_and_pickles_keep_the_clipping():
+    """Without a step: no GPU needed."""
+    import pickle
+    from nerf_amd.optim import FusedAdam
+    for limit in (None, 0.5):
+        opt = FusedAdam([torch.nn.Parameter(torch.ones(3))], max_grad_norm=limit)
+        for twin in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+            assert twin.max_grad_norm == limit and twin.grad_norm is None
+            twin.load_state_dict(opt.state_dict())
+            assert twin.max_grad_norm == limit
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("limit", [None, 0.5])
+def test_a_copy_goes_on_like_the_original(dev, limit, capturable):
+    from nerf_amd.optim import FusedAdam
+    params = [torch.nn.Parameter(torch.arange(1.0, n + 1, device=dev)) for n in (5, 300)]
+    opt = FusedAdam(params, lr=1e-2, max_grad_norm=limit, capturable=capturable)
+    model = {"opt": opt, "params": params}
+    for step in range(4):
+        if step == 2:
+            twin = copy.deepcopy(model)
+        for m in (model, twin) if step >= 2 else (model,):
+            for p in m["params"]:
+                p.grad = torch.full_like(p, 0.1 * step + 0.1)
+            m["opt"].step()
+    for a, b in zip(params, twin["params"]):
+        assert a is not b and torch.equal(a, b)
+        assert float(opt.state[a]["step"]) == 4 == float(twin["opt"].state[b]["step"])
+
+
 def test_refusals():
     from nerf_amd._lib import NerfHipError
     from nerf_amd.optim import FusedAdam
