@@ -231,7 +231,7 @@ int nerf_gather_kept_by_slot(const float* d_rgb, const float* d_sigma, const int
  * infinity may turn into a NaN; no gate takes it back), and leaves other channels alone.  C <= 131072.
  * carry: nerf_linear_scan_carry_floats(B,T,C,G) floats that the backward pass needs (NULL: not
  * kept).  workspace: nerf_linear_scan_workspace_floats(B,T,C,G,backward) floats, NULL where that is
- * 0.  T >= 1; B = 0 or C = 0 is nothing to do.  Every pointer 16-byte aligned.
+ * 0.  T >= 1; B = 0 or C = 0 is nothing to do (no output is written).  Every pointer 16-byte aligned.
  * bwd: d_h [B,T,C] of x_type and d_last [B,C] (either may be NULL: zeros) -> d_gate (gate's type and
  * shape; the sum over the channels of a gate), d_x, d_state, all WRITTEN (any may be NULL); sums
  * have a fixed order.  h is recomputed from x, so h itself is not needed. */

@@ -489,6 +489,8 @@ def render_loss(rgb, target, rgb_fine=None, weights=None, reg: float = 0.0) -> t
 # ---------------------------------------------------- linear recurrence ----
 def _scan_fwd(gate, x, state, reverse, blend, want_last, keep):
     """Dense [B,T,G], [B,T,C], [B,C] | None -> h, last | None, carry | None (what the backward pass needs)."""
+    if x.numel() == 0:
+        return torch.empty_like(x), (None if not want_last else state.clone() if state is not None else x.new_zeros(x.shape[::2], dtype=torch.float32)), None
     lib = L.lib()
     B, T, C = x.shape
     G = gate.shape[2]
@@ -521,6 +523,9 @@ class _LinearScan(torch.autograd.Function):
         B, T, C = x.shape
         G = gate.shape[2]
         need_gate, need_x, need_state = ctx.needs_input_grad[:3]
+        if x.numel() == 0:   # the state passes through; a gate may have elements where there are no channels
+            d_state = None if not need_state else d_last.clone() if d_last is not None else torch.zeros_like(state)
+            return (*_once(torch.zeros_like(gate) if need_gate else None, torch.empty_like(x) if need_x else None, d_state), None, None, None)
         d_h, d_last = (None if t is None else L.dense(t.detach()) for t in (d_h, d_last))
         d_gate = torch.empty_like(gate) if need_gate else None   # (the saved tensors are dense)
         d_x = torch.empty_like(x) if need_x else None
@@ -567,11 +572,6 @@ def linear_scan(gate: torch.Tensor, x: torch.Tensor, state: Optional[torch.Tenso
         state = state.float()
     L.type_code(x, "x")
     L.same_device(gate, x, state)
-    if T == 0:
-        h = x.clone()
-        if not return_state:
-            return h
-        return h, (state.clone() if state is not None else torch.zeros(*lead, C, device=x.device))
     train = torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or (state is not None and state.requires_grad))
     shape = x.shape
     if len(shape) != 3:   # (a view of nothing new would still be a node of the graph)

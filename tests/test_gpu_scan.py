@@ -234,6 +234,15 @@ def test_empty_and_partial_gradients(dev):
         assert x.grad.shape == x.shape and (T > 0 or bool((state.grad == 1).all()))
         with torch.no_grad():
             ops.linear_scan(gate, x, None, return_state=True)
+        del h, last
+        for lead in ((), (2, 0), (1, 2)):     # memory that held something, a gate with elements where there are no channels
+            torch.full((4096,), 7.0, device=dev)
+            leaves = [torch.ones(*lead, T, n, device=dev, requires_grad=True) for n in (C or 3, C)]
+            y, end = ops.linear_scan(*leaves, return_state=True)
+            assert y.shape == (*lead, T, C) and end.shape == (*lead, C) and (T > 0 or not bool(end.any()))
+            if y.numel() == 0:
+                grads = torch.autograd.grad([y, end], leaves, [torch.ones_like(y), torch.ones_like(end)])
+                assert all(g.shape == t.shape and not bool(g.any()) for g, t in zip(grads, leaves))
     # only some of the inputs want gradients, only some of the outputs send any
     gate, x, s, d_h, d_last = make(2, 20, 8, 2, F32, F32, True, 9)
     want = ref_scan(gate, x, s, False, False, d_h, None)
