@@ -10,8 +10,8 @@
 //   - a wave adds up its chunk's rows, run by run.  A run that lies inside the chunk is finished and written; the
 //     stretches of runs that cross the chunk's borders are left as partial rows, at most two a chunk;
 //   - a second launch joins the partial rows of each run that crosses chunks.
-// The rows that no id names are zeros: the whole table is cleared by workgroups of the first sorting launch, which fill
-// the compute units that the sort leaves idle.
+// The rows that no id names are zeros: the whole table is cleared by workgroups of the sorting launches, which fill the
+// compute units that the sort leaves idle.
 // Sums are held in float, in an order that the ids alone decide, and rounded once.
 #include <algorithm>
 
@@ -25,35 +25,32 @@ constexpr int JOIN_CHUNKS = 64;      // most chunks whose crossing runs one work
 constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
 constexpr int SORT_ITEMS = 4, SORT_TILE = SORT_THREADS * SORT_ITEMS;   // keys that a workgroup ranks at once
 constexpr int SORT_BITS = 10, SORT_DIGITS = 1 << SORT_BITS;
-constexpr int SMALL_ITEMS = 16, SMALL_TILE = SORT_THREADS * SMALL_ITEMS;   // keys that one workgroup sorts by itself ...
-constexpr int SMALL_BITS = 8, SMALL_DIGITS = 1 << SMALL_BITS;              // ... in LDS, beside smaller counters
-constexpr int SORT_FEW_TILES = 32;
+// One tile is sorted by one workgroup in one launch.  More keys a workgroup (16384, 16 a thread) were slower than several
+// tiles from the second tile on: 6000 ids of 1000 rows 30 us against 24, 16384 36 against 25, of 50021 rows 46 against 40.
+// Up to so many tiles the scattering workgroups sum the counts of the tiles in front themselves.  Against a launch of its own
+// for that: 8 tiles 38 us and 42, 32 tiles 42 and 44, 48 tiles the same, 256 tiles 89 and 65.
+constexpr int SORT_FEW_TILES = 48;
 constexpr unsigned NO_KEY = 0xffffffffu;
 
 // ---- forward ---------------------------------------------------------------------------------------------------
-// A group of lanes per row, ROWS rows at a time: their ids, then their elements, are under way together.
-template <class T, int VEC, class ID, int ROWS>
+// A group of lanes per row, 16 bytes a lane where the row divides into them.  Bound by the reads of the rows and the writes
+// where those are long (65536 rows of 1024 bfloat16: 39 us, 6.8 TB/s, the rate of a fill, since rows come from the caches
+// again), by the lines that a row of a few bytes touches where they are short (2^20 rows of two floats out of 2^19: 9.8 us
+// for 24 MB of ids, rows and outputs).  Four rows a group at a time were no faster (1 % on either side of it).
+template <class T, int VEC, class ID>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(const T* __restrict__ table, int64_t V, int D, const ID* __restrict__ ids, int64_t N,
                                                             float scale, int l_lanes, T* __restrict__ out) {
     const int lanes = 1 << l_lanes, vectors = D / VEC, at_once = 256 >> l_lanes, first = (threadIdx.x & (lanes - 1)) + (int)blockIdx.y * lanes;
-    for (int64_t n0 = (int64_t)blockIdx.x * ROWS * at_once + (threadIdx.x >> l_lanes); n0 < N; n0 += (int64_t)gridDim.x * ROWS * at_once) {
-        int64_t id[ROWS];
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r) id[r] = n0 + r * at_once < N ? (int64_t)ids[n0 + r * at_once] : -1;
+    for (int64_t n = (int64_t)blockIdx.x * at_once + (threadIdx.x >> l_lanes); n < N; n += (int64_t)gridDim.x * at_once) {
+        const int64_t id = (int64_t)ids[n];
         for (int i = first; i < vectors; i += lanes * (int)gridDim.y) {
-            float v[ROWS][VEC];
+            float v[VEC];
 #pragma unroll
-            for (int r = 0; r < ROWS; ++r) {
+            for (int k = 0; k < VEC; ++k) v[k] = __builtin_nanf("");
+            if (id >= 0 && id < V) load_run<VEC>(table + id * D + (int64_t)i * VEC, v);
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) v[r][k] = __builtin_nanf("");
-                if (id[r] >= 0 && id[r] < V) load_run<VEC>(table + id[r] * D + (int64_t)i * VEC, v[r]);
-            }
-#pragma unroll
-            for (int r = 0; r < ROWS; ++r) {
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) v[r][k] *= scale;
-                if (n0 + r * at_once < N) store_run<VEC>(out + (n0 + r * at_once) * D + (int64_t)i * VEC, v[r]);
-            }
+            for (int k = 0; k < VEC; ++k) v[k] *= scale;
+            store_run<VEC>(out + n * D + (int64_t)i * VEC, v);
         }
     }
 }
@@ -157,7 +154,7 @@ __device__ __forceinline__ void clear_counts(unsigned (&count)[SORT_WAVES][DIGIT
         if ((int)threadIdx.x < digits) count[w][threadIdx.x] = 0u;
 }
 
-// Up to SMALL_TILE keys: every pass in one workgroup, the pairs changing places through LDS.
+// One tile: every pass in one workgroup, the pairs changing places through LDS.
 template <class ID, int ITEMS>
 __global__ __launch_bounds__(SORT_THREADS) void sort_small_kernel(const ID* __restrict__ ids, int n, int64_t V, int64_t padding, int passes, int bits,
                                                                   uint2* __restrict__ sorted, char* __restrict__ clear, int64_t clear_bytes) {
@@ -165,7 +162,7 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_small_kernel(const ID* __re
         clear_table(clear, clear_bytes, blockIdx.x - 1, gridDim.x - 1);
         return;
     }
-    __shared__ unsigned s_count[SORT_WAVES][SMALL_DIGITS];
+    __shared__ unsigned s_count[SORT_WAVES][SORT_DIGITS];
     __shared__ unsigned s_key[SORT_THREADS * ITEMS];
     __shared__ unsigned short s_val[SORT_THREADS * ITEMS];
     __shared__ unsigned s_wave[SORT_WAVES];
@@ -221,7 +218,7 @@ template <class ID, bool FIRST>
 __global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const ID* __restrict__ ids, const uint2* __restrict__ from, int64_t n, int64_t V,
                                                                   int64_t padding, int shift, int bits, int tiles, unsigned* __restrict__ table,
                                                                   char* __restrict__ clear, int64_t clear_bytes) {
-    if (FIRST && (int)blockIdx.x >= tiles) {
+    if ((int)blockIdx.x >= tiles) {
         clear_table(clear, clear_bytes, blockIdx.x - tiles, gridDim.x - tiles);
         return;
     }
@@ -272,7 +269,11 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_prefix_kernel(unsigned* __r
 template <class ID, bool FIRST>
 __global__ __launch_bounds__(SORT_THREADS) void sort_scatter_kernel(const ID* __restrict__ ids, const uint2* __restrict__ from, int64_t n, int64_t V, int64_t padding,
                                                                     int shift, int bits, const unsigned* __restrict__ table, int tiles, bool summed,
-                                                                    uint2* __restrict__ to) {
+                                                                    uint2* __restrict__ to, char* __restrict__ clear, int64_t clear_bytes) {
+    if ((int)blockIdx.x >= tiles) {
+        clear_table(clear, clear_bytes, blockIdx.x - tiles, gridDim.x - tiles);
+        return;
+    }
     __shared__ unsigned s_count[SORT_WAVES][SORT_DIGITS];
     __shared__ unsigned s_to[SORT_DIGITS];   // what a rank in the sorted tile lacks to its place in the output, per digit
     __shared__ unsigned s_wave[SORT_WAVES];
@@ -444,7 +445,7 @@ __global__ __launch_bounds__(256) void embedding_sums_kernel(EmbSums p, const T*
 // group of lanes each, longer ones by the whole workgroup.
 template <class T, int VEC>
 __global__ __launch_bounds__(JOIN_THREADS) void embedding_join_kernel(EmbSums p, T* __restrict__ d_table) {
-    constexpr int FEW = 8;
+    constexpr int FEW = 16;   // against 8: runs over 8 to 15 chunks 39 us and 52 (262144 ids of 1000 rows), shorter ones 0.7 us more
     __shared__ int s_over[JOIN_CHUNKS];       // chunks that the run goes on over, FEW: at least so many; 0: none starts here
     __shared__ unsigned s_key[JOIN_CHUNKS];
     __shared__ int s_count[JOIN_THREADS / 64];
@@ -556,16 +557,23 @@ struct EmbWork {                       // the workspace, cut into arrays that st
     size_t pairs[2], table, part, bytes;
 };
 
-// log2 of the positions of a chunk: at least four rounds of a wave; long enough that the two partial rows of a chunk
-// (8 bytes an element, written and read) stay a small part of its rows' bytes
-static int chunk_log2(int l_lanes) { return std::max(5, 8 - l_lanes); }
+// log2 of the positions of a chunk: 32 positions or four rounds of a wave, whichever is more, which keeps the two partial
+// rows of a chunk (8 bytes an element, written and read) a small part of its rows' bytes; down to 8 or four rounds while that
+// leaves too few waves to hide the reads.  50021 rows of 1024 bfloat16: 4096 ids 28 us with 8 positions, 33 with 16, 42 with
+// 32; 16384 ids 49, 52 and 59, or where a few ids are most of them 65, 60 and 63; 65536 ids 90, 76 and 72.
+constexpr int SUM_WAVES = 2048;
+static int chunk_log2(int64_t N, int l_lanes, int col_tiles) {
+    int l = std::max(5, 8 - l_lanes);
+    while (l > std::max(3, 8 - l_lanes) && ceil_div(N, 1ll << l) * col_tiles < SUM_WAVES) --l;
+    return l;
+}
 
 static EmbWork embedding_work(int64_t N, int64_t V, int D) {
     EmbWork w;
     int bits = 1;
     while ((1ll << bits) < V + 1) ++bits;
-    const bool small = N <= SMALL_TILE;
-    w.passes = (int)ceil_div(bits, small ? SMALL_BITS : SORT_BITS);
+    const bool small = N <= SORT_TILE;
+    w.passes = (int)ceil_div(bits, SORT_BITS);
     w.bits = (int)ceil_div(bits, w.passes);
     w.tiles = small ? 1 : ceil_div(N, SORT_TILE);
     size_t at = 0;
@@ -577,7 +585,8 @@ static EmbWork embedding_work(int64_t N, int64_t V, int D) {
     w.pairs[0] = take(8 * N);
     w.pairs[1] = take(small ? 0 : 8 * N);
     w.table = take(small ? 0 : 4ull * (w.tiles + 1) << w.bits);
-    w.part = take(N > 32 ? 8ull * D * (size_t)ceil_div(N, 32) : 0);   // chunks hold 32 positions or more
+    // chunks hold 32 positions or more, or 8 or more while they are fewer than twice SUM_WAVES
+    w.part = take(N > 8 ? 8ull * D * (size_t)std::max(ceil_div(N, 32), std::min<int64_t>(ceil_div(N, 8), 2 * SUM_WAVES)) : 0);
     w.bytes = at;
     return w;
 }
@@ -597,16 +606,11 @@ static int embedding_fwd_typed(const T* table, int64_t V, int D, const ID* ids, 
     return with_vector<T>(D, [&](auto vec) {
         constexpr int VEC = decltype(vec)::value;
         const int l = lanes_log2(D / VEC);
-        const auto launch = [&](auto rows) {
-            constexpr int ROWS = decltype(rows)::value;
-            const int64_t blocks = std::min<int64_t>(ceil_div(N, (256 >> l) * ROWS), 1 << 20);   // a launch holds fewer than 2^32 threads
-            // few rows: their columns are spread over workgroups too
-            const int wide = (int)std::min<int64_t>(ceil_div(D / VEC, 1 << l), std::max<int64_t>(1, ceil_div(1024, blocks)));
-            hipLaunchKernelGGL((embedding_fwd_kernel<T, VEC, ID, ROWS>), dim3((unsigned)blocks, wide), dim3(256), 0, stream, table, V, D, ids, N, scale, l, out);
-            return check_launch("nerf_embedding_fwd");
-        };
-        // four rows a group once that still leaves four workgroups to a compute unit
-        return N >= 4 * 1024ll * (256 >> l) ? launch(std::integral_constant<int, 4>{}) : launch(std::integral_constant<int, 1>{});
+        const int64_t blocks = std::min<int64_t>(ceil_div(N, 256 >> l), 1 << 20);   // a launch holds fewer than 2^32 threads
+        // few rows: their columns are spread over workgroups too
+        const int wide = (int)std::min<int64_t>(ceil_div(D / VEC, 1 << l), std::max<int64_t>(1, ceil_div(1024, blocks)));
+        hipLaunchKernelGGL((embedding_fwd_kernel<T, VEC, ID>), dim3((unsigned)blocks, wide), dim3(256), 0, stream, table, V, D, ids, N, scale, l, out);
+        return check_launch("nerf_embedding_fwd");
     });
 }
 
@@ -614,39 +618,48 @@ template <class ID>
 static int embedding_sort(const ID* ids, int64_t N, int64_t V, int64_t padding, const EmbWork& w, char* work, char* clear, int64_t clear_bytes,
                           const uint2** sorted, hipStream_t stream) {
     // workgroups that clear: 16 KB each while that leaves them one to a compute unit or fewer, then more
-    const int clearing = (int)std::min<int64_t>(1024, ceil_div(clear_bytes, 16384));
+    const auto clearing = [](int64_t bytes) { return (unsigned)std::min<int64_t>(1024, ceil_div(bytes, 16384)); };
     uint2* pairs[2] = {reinterpret_cast<uint2*>(work + w.pairs[0]), reinterpret_cast<uint2*>(work + w.pairs[1])};
     if (w.tiles <= 1) {
         const auto launch = [&](auto items) {
-            hipLaunchKernelGGL((sort_small_kernel<ID, decltype(items)::value>), dim3(1 + clearing), dim3(SORT_THREADS), 0, stream, ids, (int)N, V, padding, w.passes,
+            hipLaunchKernelGGL((sort_small_kernel<ID, decltype(items)::value>), dim3(1 + clearing(clear_bytes)), dim3(SORT_THREADS), 0, stream, ids, (int)N, V, padding, w.passes,
                                w.bits, pairs[0], clear, clear_bytes);
         };
         if (N <= SORT_THREADS) launch(std::integral_constant<int, 1>{});
-        else if (N <= 4 * SORT_THREADS) launch(std::integral_constant<int, 4>{});
-        else launch(std::integral_constant<int, SMALL_ITEMS>{});
+        else launch(std::integral_constant<int, SORT_ITEMS>{});
         *sorted = pairs[0];
         return check_launch("nerf_embedding_bwd(sort)");
     }
     unsigned* table = reinterpret_cast<unsigned*>(work + w.table);
+    // The launches share the clearing of a large table, by the time that they take for themselves: a count one part, a scatter
+    // two.  (50021 rows of 1024 bfloat16, 102 MB, 16384 ids, two passes: 38 us with all of it beside the first count, 35 so.)
+    const int64_t part = std::max<int64_t>((ceil_div(clear_bytes, 3 * w.passes) + 15) / 16 * 16, 8 << 20);
+    int64_t cleared = 0;
+    const auto share = [&](int parts) {   // the next bytes to clear
+        const int64_t bytes = std::min(parts * part, clear_bytes - cleared);
+        cleared += bytes;
+        return bytes;
+    };
     int from = 0;
     for (int p = 0; p < w.passes; ++p) {
         const int to = p == 0 ? 0 : 1 - from, shift = p * w.bits;
-        const dim3 grid((unsigned)w.tiles), block(SORT_THREADS);
-        if (p == 0)
-            hipLaunchKernelGGL((sort_count_kernel<ID, true>), dim3((unsigned)(w.tiles + clearing)), block, 0, stream, ids, (const uint2*)nullptr, N, V, padding, shift, w.bits,
-                               (int)w.tiles, table, clear, clear_bytes);
-        else
-            hipLaunchKernelGGL((sort_count_kernel<ID, false>), grid, block, 0, stream, ids, (const uint2*)pairs[from], N, V, padding, shift, w.bits,
-                               (int)w.tiles, table, (char*)nullptr, int64_t(0));
+        const dim3 block(SORT_THREADS);
         const bool summed = w.tiles > SORT_FEW_TILES;
-        if (summed)
-            hipLaunchKernelGGL(sort_prefix_kernel, dim3((unsigned)ceil_div(1 << w.bits, 64)), block, 0, stream, table, (int)w.tiles, 1 << w.bits);
-        if (p == 0)
-            hipLaunchKernelGGL((sort_scatter_kernel<ID, true>), grid, block, 0, stream, ids, (const uint2*)nullptr, N, V, padding, shift, w.bits, table, (int)w.tiles,
-                               summed, pairs[to]);
-        else
-            hipLaunchKernelGGL((sort_scatter_kernel<ID, false>), grid, block, 0, stream, ids, (const uint2*)pairs[from], N, V, padding, shift, w.bits, table,
-                               (int)w.tiles, summed, pairs[to]);
+        const auto pass = [&](auto first) {
+            constexpr bool FIRST = decltype(first)::value;
+            char* at = clear + cleared;
+            int64_t bytes = share(1);
+            hipLaunchKernelGGL((sort_count_kernel<ID, FIRST>), dim3((unsigned)w.tiles + clearing(bytes)), block, 0, stream, ids, (const uint2*)pairs[from], N, V, padding,
+                               shift, w.bits, (int)w.tiles, table, at, bytes);
+            if (summed)
+                hipLaunchKernelGGL(sort_prefix_kernel, dim3((unsigned)ceil_div(1 << w.bits, 64)), block, 0, stream, table, (int)w.tiles, 1 << w.bits);
+            at = clear + cleared;
+            bytes = share(2);
+            hipLaunchKernelGGL((sort_scatter_kernel<ID, FIRST>), dim3((unsigned)w.tiles + clearing(bytes)), block, 0, stream, ids, (const uint2*)pairs[from], N, V, padding,
+                               shift, w.bits, table, (int)w.tiles, summed, pairs[to], at, bytes);
+        };
+        if (p == 0) pass(std::true_type{});
+        else pass(std::false_type{});
         if (int rc = check_launch("nerf_embedding_bwd(sort)")) return rc;
         from = to;
     }
@@ -662,8 +675,8 @@ static int embedding_sums(const T* d_out, int64_t N, int64_t V, int D, const uin
         EmbSums p;
         p.sorted = sorted; p.N = N; p.V = V; p.D = D; p.scale = scale;
         p.l_lanes = lanes_log2(D / VEC);
-        p.l_chunk = chunk_log2(p.l_lanes);
         p.col_tiles = (int)ceil_div(D / VEC, 1 << p.l_lanes);
+        p.l_chunk = chunk_log2(N, p.l_lanes, p.col_tiles);
         p.chunks = ceil_div(N, 1 << p.l_chunk);
         p.join_chunks = std::min(JOIN_CHUNKS, 2 * (JOIN_THREADS >> p.l_lanes));
         p.part = reinterpret_cast<float*>(work + w.part);
