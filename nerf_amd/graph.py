@@ -12,6 +12,10 @@ them), draws random numbers with ``torch.rand(..., device=...)`` only, does noth
 step count and the learning rate on the device (``FusedAdam(capturable=True)``).  The reference has no counterpart
 (its loops are eager PyTorch); a captured step computes what the eager step computes -- including under a learning-rate
 scheduler (src/train_nerf.py:87,204; src/train_nerf_ngp.py:57-62), whose rate reaches the device in front of each replay.
+
+While the step is captured no autograd graph of an eager call over the same parameters may be alive (a loss that was kept,
+an output that still requires its gradient): the captured backward pass would meet the gradient accumulators that the eager
+graph made on another stream, which ends the process.  Drop or detach such results first.
 """
 from __future__ import annotations
 
