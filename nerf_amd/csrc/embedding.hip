@@ -12,6 +12,7 @@
 //   - a second launch joins the partial rows of each run that crosses chunks.
 // The rows that no id names are zeros: the whole table is cleared by workgroups of the sorting launches, which fill the
 // compute units that the sort leaves idle.
+// Rows of one vector (a hash grid's two features) are moved instead of sorted: see the buckets below.
 // Sums are held in float, in an order that the ids alone decide, and rounded once.
 #include <algorithm>
 
@@ -76,8 +77,8 @@ __device__ __forceinline__ unsigned sort_key(ID id, int64_t V, int64_t padding) 
 // digit find each other by ballots, take their ranks from the old count, and the last of them writes the new one.
 // On return rank[r] is the key's place within its wave and digit, and after digit_starts() count[w][d] is where the
 // wave's keys of digit d start in the sorted tile.
-template <int ITEMS, int DIGITS>
-__device__ __forceinline__ void rank_in_wave(const unsigned (&key)[ITEMS], const bool (&on)[ITEMS], int shift, int bits, unsigned (&count)[SORT_WAVES][DIGITS],
+template <int ITEMS, int WAVES, int DIGITS>
+__device__ __forceinline__ void rank_in_wave(const unsigned (&key)[ITEMS], const bool (&on)[ITEMS], int shift, int bits, unsigned (&count)[WAVES][DIGITS],
                                              unsigned (&rank)[ITEMS]) {
     const unsigned mask = (1u << bits) - 1u;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -107,8 +108,9 @@ __device__ __forceinline__ void rank_in_wave(const unsigned (&key)[ITEMS], const
     }
 }
 
-// Exclusive sum over the workgroup's 1024 threads.
-__device__ __forceinline__ unsigned block_exclusive(unsigned v, unsigned (&s_wave)[SORT_WAVES]) {
+// Exclusive sum over the workgroup's threads.
+template <int WAVES>
+__device__ __forceinline__ unsigned block_exclusive(unsigned v, unsigned (&s_wave)[WAVES]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     unsigned inc = v;
 #pragma unroll
@@ -120,7 +122,7 @@ __device__ __forceinline__ unsigned block_exclusive(unsigned v, unsigned (&s_wav
     __syncthreads();
     unsigned base = 0;
 #pragma unroll
-    for (int w = 0; w < SORT_WAVES; ++w) base += w < wave ? s_wave[w] : 0u;
+    for (int w = 0; w < WAVES; ++w) base += w < wave ? s_wave[w] : 0u;
     __syncthreads();
     return base + inc - v;
 }
@@ -216,7 +218,7 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_small_kernel(const ID* __re
 // counts themselves (`summed` false): a launch less.
 template <class ID, bool FIRST>
 __global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const ID* __restrict__ ids, const uint2* __restrict__ from, int64_t n, int64_t V,
-                                                                  int64_t padding, int shift, int bits, int tiles, unsigned* __restrict__ table,
+                                                                  int64_t padding, int shift, int bits, unsigned limit, int tiles, unsigned* __restrict__ table,
                                                                   char* __restrict__ clear, int64_t clear_bytes) {
     if ((int)blockIdx.x >= tiles) {
         clear_table(clear, clear_bytes, blockIdx.x - tiles, gridDim.x - tiles);
@@ -231,7 +233,7 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const ID* __re
         const int64_t i = base + r * SORT_THREADS + threadIdx.x;
         if (i < n) {
             const unsigned key = FIRST ? sort_key(ids[i], V, padding) : from[i].x;
-            atomicAdd(&s_count[(key >> shift) & (digits - 1)], 1u);   // whole numbers: the order does not matter
+            if (key < limit) atomicAdd(&s_count[(key >> shift) & (digits - 1)], 1u);   // whole numbers: the order does not matter
         }
     }
     __syncthreads();
@@ -538,6 +540,280 @@ __global__ __launch_bounds__(JOIN_THREADS) void embedding_join_kernel(EmbSums p,
     }
 }
 
+// ---- narrow rows -------------------------------------------------------------------------------------------------------
+// Rows of up to 16 bytes.  Sorted whole, each position costs two moves of a pair and then a read of its row from anywhere
+// (2^20 rows of 8 bytes: 19 us of 70 for that alone).  Here the rows themselves are moved, once and as they are read, in order
+// of their ids' upper bits: a bucket holds the rows of 2^low neighbouring ids, in the order of their positions.  A workgroup
+// then puts up to BUCKET_SEG rows of a bucket in order in LDS and adds up each id's run; it writes all of its bucket's part of
+// the table, so that nothing is cleared.  A bucket of more rows -- ids are often far from even -- is cut into segments, whose
+// sums a last launch adds in order.  2^20 positions over 2^19 rows of two floats: 38 us, sorted whole 66; 16384: 27 and 38;
+// most of them a few ids: 51 and 77.  (Up to 1023 rows one pass sorts them, and the two ways take the same time.)
+constexpr int BUCKETS = 1024, BUCKET_BITS = 10, BUCKET_LOW = 5;   // 2^5 ids to a bucket at least
+constexpr int BUCKET_WAVES = 4, BUCKET_THREADS = 64 * BUCKET_WAVES, BUCKET_ITEMS = 8, BUCKET_SEG = BUCKET_THREADS * BUCKET_ITEMS;
+constexpr int BUCKET_MOST_BITS = 20;
+constexpr unsigned BUCKET_RUN = 128;   // rows of one id that a lane adds up by itself; of more, a wave
+
+template <class T, int VEC>
+constexpr int row_words() { return (int)(sizeof(T) * VEC + 3) / 4; }
+
+// A row as it lies in memory, in words, and back.
+template <class T, int VEC>
+__device__ __forceinline__ void row_load(const T* __restrict__ p, unsigned (&w)[row_words<T, VEC>()]) {
+    const Run<T, VEC> r = *reinterpret_cast<const Run<T, VEC>*>(p);
+    if constexpr (sizeof(T) * VEC == 2) w[0] = __builtin_bit_cast(unsigned short, r.v[0]);
+    else __builtin_memcpy(w, &r, sizeof(r));
+}
+template <class T, int VEC>
+__device__ __forceinline__ float row_value(const unsigned* w, int k) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[k]);
+    else return (float)__builtin_bit_cast(T, (unsigned short)(w[k / 2] >> (k & 1) * 16));
+}
+
+template <class T, int VEC, class ID>
+__global__ __launch_bounds__(SORT_THREADS) void bucket_scatter_kernel(const ID* __restrict__ ids, int64_t n, int64_t V, int64_t padding, int low,
+                                                                      const unsigned* __restrict__ table, int tiles, const T* __restrict__ d_out,
+                                                                      unsigned* __restrict__ to) {
+    constexpr int W = row_words<T, VEC>(), ITEM = 1 + W;
+    __shared__ unsigned s_count[SORT_WAVES][BUCKETS];
+    __shared__ unsigned s_to[BUCKETS];   // as in sort_scatter_kernel
+    __shared__ unsigned s_wave[SORT_WAVES];
+    __shared__ unsigned s_item[SORT_TILE * ITEM];
+    __shared__ int s_held;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t tile = (int64_t)blockIdx.x * SORT_TILE;
+    unsigned key[SORT_ITEMS], rank[SORT_ITEMS], row[SORT_ITEMS][W];
+    bool on[SORT_ITEMS];
+    if (threadIdx.x == 0) s_held = 0;
+#pragma unroll
+    for (int r = 0; r < SORT_ITEMS; ++r) {
+        const int64_t i = tile + (wave * SORT_ITEMS + r) * 64 + lane;
+        key[r] = i < n ? sort_key(ids[i], V, padding) : (unsigned)V;
+        on[r] = key[r] < (unsigned)V;
+#pragma unroll
+        for (int k = 0; k < W; ++k) row[r][k] = 0u;
+        if (i < n) row_load<T, VEC>(d_out + i * VEC, row[r]);
+    }
+    const unsigned total = table[(int64_t)tiles * BUCKETS + threadIdx.x], front = table[(int64_t)blockIdx.x * BUCKETS + threadIdx.x];
+    clear_counts(s_count, BUCKETS);
+    __syncthreads();
+    rank_in_wave(key, on, low, BUCKET_BITS, s_count, rank);
+#pragma unroll
+    for (int r = 0; r < SORT_ITEMS; ++r) {
+        const int held = __popcll(__ballot(on[r]));
+        if (lane == 0) atomicAdd(&s_held, held);
+    }
+    __syncthreads();
+    unsigned start;
+    digit_starts(s_count, s_wave, BUCKETS, start);
+    const unsigned first = block_exclusive(total, s_wave);
+    s_to[threadIdx.x] = first + front - start;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < SORT_ITEMS; ++r) {
+        if (on[r]) {
+            unsigned* const at = s_item + (s_count[wave][key[r] >> low] + rank[r]) * ITEM;
+            at[0] = key[r];
+#pragma unroll
+            for (int k = 0; k < W; ++k) at[1 + k] = row[r][k];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < SORT_ITEMS; ++r) {
+        const int i = r * SORT_THREADS + (int)threadIdx.x;
+        if (i < s_held) {
+            const unsigned* const from = s_item + i * ITEM;
+            unsigned* const at = to + (int64_t)((unsigned)i + s_to[from[0] >> low]) * ITEM;
+#pragma unroll
+            for (int k = 0; k < ITEM; ++k) at[k] = from[k];
+        }
+    }
+}
+
+struct BucketSums {
+    const unsigned* total;   // [BUCKETS] rows
+    const unsigned* items;
+    float* part;             // [segments][2^low][D]
+    int64_t V;
+    int low, buckets;
+    float scale;
+};
+__device__ __forceinline__ unsigned bucket_segments(const BucketSums& p, int q, unsigned rows) {
+    return q < p.buckets ? max(1u, (rows + BUCKET_SEG - 1) / BUCKET_SEG) : 0u;
+}
+
+// A workgroup: one segment.
+template <class T, int VEC>
+__global__ __launch_bounds__(BUCKET_THREADS) void bucket_sums_kernel(BucketSums p, T* __restrict__ d_table) {
+    constexpr int W = row_words<T, VEC>(), ITEM = 1 + W, PER = BUCKETS / BUCKET_THREADS;
+    __shared__ unsigned s_count[BUCKET_WAVES][BUCKETS];
+    __shared__ unsigned s_row[BUCKET_SEG * W];
+    __shared__ unsigned s_start[BUCKETS + 1];
+    __shared__ unsigned s_wave[BUCKET_WAVES];
+    __shared__ unsigned s_bucket, s_segment, s_first, s_rows;
+    __shared__ unsigned s_long[BUCKET_SEG / BUCKET_RUN], s_longs;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    // which segment of which bucket: buckets hold their segments one after the other
+    if (threadIdx.x == 0) {
+        s_bucket = NO_KEY;
+        s_longs = 0;
+    }
+    unsigned rows[PER], segments[PER], all_rows = 0, all_segments = 0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int q = (int)threadIdx.x * PER + k;
+        rows[k] = p.total[q];
+        segments[k] = bucket_segments(p, q, rows[k]);
+        all_rows += rows[k];
+        all_segments += segments[k];
+    }
+    unsigned first = block_exclusive(all_rows, s_wave), segment = block_exclusive(all_segments, s_wave);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        if (blockIdx.x >= segment && blockIdx.x < segment + segments[k]) {
+            s_bucket = threadIdx.x * PER + k;
+            s_segment = blockIdx.x - segment;
+            s_first = first;
+            s_rows = rows[k];
+        }
+        first += rows[k];
+        segment += segments[k];
+    }
+    for (int i = threadIdx.x; i < BUCKET_WAVES * BUCKETS; i += BUCKET_THREADS) s_count[0][i] = 0u;
+    __syncthreads();
+    if (s_bucket == NO_KEY) return;   // more workgroups than segments
+    const int skip = (int)s_segment * BUCKET_SEG, n = min(BUCKET_SEG, (int)s_rows - skip), ids = 1 << p.low;
+    const bool whole = s_rows <= BUCKET_SEG;
+    const unsigned* const items = p.items + ((int64_t)s_first + skip) * ITEM;
+    const int rounds = (n + BUCKET_THREADS - 1) / BUCKET_THREADS;   // in use: the rows are packed to the front of every wave
+    unsigned key[BUCKET_ITEMS], rank[BUCKET_ITEMS], row[BUCKET_ITEMS][W];
+    bool on[BUCKET_ITEMS];
+#pragma unroll
+    for (int r = 0; r < BUCKET_ITEMS; ++r) {
+        const int i = wave * 64 * rounds + r * 64 + lane;
+        on[r] = r < rounds && i < n;
+        key[r] = 0u;
+#pragma unroll
+        for (int k = 0; k < W; ++k) row[r][k] = 0u;
+        if (on[r]) {
+            key[r] = items[(int64_t)i * ITEM] & (unsigned)(ids - 1);
+#pragma unroll
+            for (int k = 0; k < W; ++k) row[r][k] = items[(int64_t)i * ITEM + 1 + k];
+        }
+    }
+    rank_in_wave(key, on, 0, p.low, s_count, rank);
+    __syncthreads();
+    unsigned held = 0, c[PER][BUCKET_WAVES];
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+#pragma unroll
+        for (int w = 0; w < BUCKET_WAVES; ++w) {
+            c[k][w] = s_count[w][threadIdx.x * PER + k];
+            held += c[k][w];
+        }
+    unsigned at = block_exclusive(held, s_wave);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        s_start[threadIdx.x * PER + k] = at;
+#pragma unroll
+        for (int w = 0; w < BUCKET_WAVES; ++w) {
+            s_count[w][threadIdx.x * PER + k] = at;
+            at += c[k][w];
+        }
+    }
+    if (threadIdx.x == BUCKET_THREADS - 1) s_start[BUCKETS] = at;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < BUCKET_ITEMS; ++r) {
+        if (on[r]) {
+#pragma unroll
+            for (int k = 0; k < W; ++k) s_row[(s_count[wave][key[r]] + rank[r]) * W + k] = row[r][k];
+        }
+    }
+    __syncthreads();
+    const auto finish = [&](unsigned id, float (&sum)[VEC]) {
+        if (whole) {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) sum[k] *= p.scale;
+            store_run<VEC>(d_table + (((int64_t)s_bucket << p.low) + id) * VEC, sum);
+        } else {
+            store_run<VEC>(p.part + ((int64_t)blockIdx.x * ids + id) * VEC, sum);
+        }
+    };
+    const int here = (int)min((int64_t)ids, p.V - ((int64_t)s_bucket << p.low));   // ids that are rows of the table
+    for (int id = threadIdx.x; id < here; id += BUCKET_THREADS) {
+        const unsigned begin = s_start[id], end = s_start[id + 1];
+        if (end - begin > BUCKET_RUN) {
+            s_long[atomicAdd(&s_longs, 1u)] = id;   // each is added up by itself: their order does not matter
+            continue;
+        }
+        float sum[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) sum[k] = 0.0f;
+#pragma unroll 4
+        for (unsigned i = begin; i < end; ++i)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) sum[k] += row_value<T, VEC>(s_row + i * W, k);
+        finish(id, sum);
+    }
+    __syncthreads();
+    for (unsigned q = wave; q < s_longs; q += BUCKET_WAVES) {
+        const unsigned id = s_long[q], end = s_start[id + 1];
+        float sum[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) sum[k] = 0.0f;
+        for (unsigned i = s_start[id] + lane; i < end; i += 64)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) sum[k] += row_value<T, VEC>(s_row + i * W, k);
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) sum[k] += __shfl_xor(sum[k], d, 64);
+        if (lane == 0) finish(id, sum);
+    }
+}
+
+// The buckets of several segments: JOIN_IDS ids a workgroup, JOIN_PARTS stretches of the segments side by side.
+constexpr int JOIN_IDS = 256, JOIN_PARTS = 1024 / JOIN_IDS;
+template <class T, int VEC>
+__global__ __launch_bounds__(1024) void bucket_join_kernel(BucketSums p, T* __restrict__ d_table) {
+    __shared__ unsigned s_wave[SORT_WAVES];
+    __shared__ unsigned s_first;
+    __shared__ float s_sum[JOIN_PARTS][JOIN_IDS][VEC];
+    const unsigned q = blockIdx.x;
+    const unsigned mine = bucket_segments(p, (int)q, p.total[q]);
+    if (mine == 1) return;
+    const unsigned first = block_exclusive(bucket_segments(p, (int)threadIdx.x, p.total[threadIdx.x]), s_wave);
+    if (threadIdx.x == q) s_first = first;
+    __syncthreads();
+    const int slot = threadIdx.x & (JOIN_IDS - 1), stretch = threadIdx.x / JOIN_IDS, ids = 1 << p.low, id = (int)blockIdx.y * JOIN_IDS + slot;
+    const int64_t v = ((int64_t)q << p.low) + id;
+    const bool on = id < ids && v < p.V;
+    const unsigned per = (mine + JOIN_PARTS - 1) / JOIN_PARTS, begin = min(stretch * per, mine), end = min(begin + per, mine);
+    float sum[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) sum[k] = 0.0f;
+    if (on) {
+#pragma unroll 8
+        for (unsigned i = begin; i < end; ++i) {
+            float x[VEC];
+            load_run<VEC>(p.part + ((int64_t)(s_first + i) * ids + id) * VEC, x);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) sum[k] += x[k];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) s_sum[stretch][slot][k] = sum[k];
+    __syncthreads();
+    if (stretch > 0 || !on) return;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+        for (int j = 1; j < JOIN_PARTS; ++j) sum[k] += s_sum[j][slot][k];
+        sum[k] *= p.scale;
+    }
+    store_run<VEC>(d_table + v * VEC, sum);
+}
+
 // ---- host ------------------------------------------------------------------------------------------------------------
 static int vector_of(int D, int size) {   // elements per lane: the widest power of two that divides a row, 16 bytes at most
     int v = 16 / size;
@@ -588,6 +864,28 @@ static EmbWork embedding_work(int64_t N, int64_t V, int D) {
     // chunks hold 32 positions or more, or 8 or more while they are fewer than twice SUM_WAVES
     w.part = take(N > 8 ? 8ull * D * (size_t)std::max(ceil_div(N, 32), std::min<int64_t>(ceil_div(N, 8), 2 * SUM_WAVES)) : 0);
     w.bytes = at;
+    return w;
+}
+
+// Narrow rows: one vector each, more ids than one workgroup sorts, more rows than one pass sorts by, few enough for the buckets.
+static bool embedding_narrow(int64_t N, int64_t V, int D, int size) { return N > SORT_TILE && V >= SORT_DIGITS && V <= 1ll << BUCKET_MOST_BITS && vector_of(D, size) == D; }
+
+struct NarrowWork {
+    int low, buckets;
+    int64_t tiles, segments;   // segments: at most
+    size_t table, items, part, bytes;
+};
+static NarrowWork narrow_work(int64_t N, int64_t V, int D) {   // for elements of any size
+    NarrowWork w;
+    w.low = BUCKET_LOW;
+    while (BUCKETS << w.low < V) ++w.low;
+    w.buckets = (int)ceil_div(V, 1 << w.low);
+    w.tiles = ceil_div(N, SORT_TILE);
+    w.segments = w.buckets + N / BUCKET_SEG;
+    w.table = 0;
+    w.items = 4ull * (w.tiles + 1) * BUCKETS;
+    w.part = w.items + (4ull * (1 + std::min(D, 4)) * N + 255) / 256 * 256;   // a row of more than four elements has 16-bit ones
+    w.bytes = w.part + (4ull * D * w.segments << w.low);
     return w;
 }
 
@@ -650,7 +948,7 @@ static int embedding_sort(const ID* ids, int64_t N, int64_t V, int64_t padding, 
             char* at = clear + cleared;
             int64_t bytes = share(1);
             hipLaunchKernelGGL((sort_count_kernel<ID, FIRST>), dim3((unsigned)w.tiles + clearing(bytes)), block, 0, stream, ids, (const uint2*)pairs[from], N, V, padding,
-                               shift, w.bits, (int)w.tiles, table, at, bytes);
+                               shift, w.bits, NO_KEY, (int)w.tiles, table, at, bytes);
             if (summed)
                 hipLaunchKernelGGL(sort_prefix_kernel, dim3((unsigned)ceil_div(1 << w.bits, 64)), block, 0, stream, table, (int)w.tiles, 1 << w.bits);
             at = clear + cleared;
@@ -692,6 +990,26 @@ static int embedding_sums(const T* d_out, int64_t N, int64_t V, int D, const uin
     });
 }
 
+template <class T, class ID>
+static int embedding_narrow_bwd(const T* d_out, const ID* ids, int64_t N, int64_t V, int D, float scale, int64_t padding, char* work, T* d_table, hipStream_t stream) {
+    return with_vector<T>(D, [&](auto vec) {
+        constexpr int VEC = decltype(vec)::value;
+        const NarrowWork w = narrow_work(N, V, D);
+        unsigned* const table = reinterpret_cast<unsigned*>(work + w.table);
+        unsigned* const items = reinterpret_cast<unsigned*>(work + w.items);
+        const BucketSums p{table + w.tiles * BUCKETS, items, reinterpret_cast<float*>(work + w.part), V, w.low, w.buckets, scale};
+        const dim3 tiles((unsigned)w.tiles), block(SORT_THREADS);
+        hipLaunchKernelGGL((sort_count_kernel<ID, true>), tiles, block, 0, stream, ids, (const uint2*)nullptr, N, V, padding, w.low, BUCKET_BITS, (unsigned)V, (int)w.tiles,
+                           table, (char*)nullptr, int64_t(0));
+        hipLaunchKernelGGL(sort_prefix_kernel, dim3(BUCKETS / 64), block, 0, stream, table, (int)w.tiles, BUCKETS);
+        hipLaunchKernelGGL((bucket_scatter_kernel<T, VEC, ID>), tiles, block, 0, stream, ids, N, V, padding, w.low, (const unsigned*)table, (int)w.tiles, d_out, items);
+        if (int rc = check_launch("nerf_embedding_bwd(buckets)")) return rc;
+        hipLaunchKernelGGL((bucket_sums_kernel<T, VEC>), dim3((unsigned)w.segments), dim3(BUCKET_THREADS), 0, stream, p, d_table);
+        hipLaunchKernelGGL((bucket_join_kernel<T, VEC>), dim3((unsigned)w.buckets, (unsigned)ceil_div(1 << w.low, JOIN_IDS)), dim3(1024), 0, stream, p, d_table);
+        return check_launch("nerf_embedding_bwd(bucket sums)");
+    });
+}
+
 static int embedding_check(const char* who, int64_t V, int D, int type, int64_t N, const void* ids, int ids_bytes) {
     NERF_REQUIRE(V >= 0 && D >= 0 && N >= 0, "%s: V=%lld D=%d N=%lld", who, (long long)V, D, (long long)N);
     NERF_REQUIRE(V < 0x7fffffffll && N < 0x7fffffffll, "%s: at most 2^31 - 2 rows and ids", who);
@@ -724,7 +1042,8 @@ extern "C" int nerf_embedding_fwd(const void* table, int type, int64_t V, int D,
 
 extern "C" size_t nerf_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int D) {
     if (N <= 0 || V <= 0 || D <= 0) return 0;
-    return embedding_work(N, V, D).bytes;
+    const size_t bytes = embedding_work(N, V, D).bytes;
+    return embedding_narrow(N, V, D, 4) || embedding_narrow(N, V, D, 2) ? std::max(bytes, narrow_work(N, V, D).bytes) : bytes;
 }
 
 extern "C" int nerf_embedding_bwd(const void* d_out, int type, const void* ids, int ids_bytes, int64_t N, int64_t V, int D, float scale, int64_t padding_idx,
@@ -742,8 +1061,16 @@ extern "C" int nerf_embedding_bwd(const void* d_out, int type, const void* ids, 
                            static_cast<char*>(d_table), clear_bytes);
         return check_launch(who);
     }
-    const EmbWork w = embedding_work(N, V, D);
     char* const work = static_cast<char*>(workspace);
+    if (embedding_narrow(N, V, D, type == NERF_F32 ? 4 : 2)) {
+        return with_type(type, [&](auto t) {
+            using T = decltype(t);
+            if (ids_bytes == 8)
+                return embedding_narrow_bwd(static_cast<const T*>(d_out), static_cast<const int64_t*>(ids), N, V, D, scale, padding_idx, work, static_cast<T*>(d_table), (hipStream_t)stream);
+            return embedding_narrow_bwd(static_cast<const T*>(d_out), static_cast<const int32_t*>(ids), N, V, D, scale, padding_idx, work, static_cast<T*>(d_table), (hipStream_t)stream);
+        });
+    }
+    const EmbWork w = embedding_work(N, V, D);
     char* const clear = static_cast<char*>(d_table);
     const uint2* sorted = nullptr;
     const int rc = ids_bytes == 8 ? embedding_sort(static_cast<const int64_t*>(ids), N, V, padding_idx, w, work, clear, clear_bytes, &sorted, (hipStream_t)stream)

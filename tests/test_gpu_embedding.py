@@ -38,7 +38,10 @@ def want_grad(ids, d_out, V, scale, pad):
     (1100000, 100003, 2, "uniform"), (1100000, 9000, 1, "skewed"), (300, 30000, 65, "runs"), (3, 200000, 6, "one"), (524288, 262144, 2, "skewed"),
     (50, 5000, 1024, "skewed"), (100, 777, 2056, "uniform"), (2049, 16384, 24, "one"), (300000, 65, 7, "uniform"),
     (700, 1024, 12, "skewed"), (700, 1025, 12, "skewed"), (90, 4096, 40, "uniform"), (90, 4097, 40, "uniform"), (70001, 16385, 3, "skewed"), (8, 16385, 260, "runs"),
-    (60, 28000, 2, "borders"), (60, 28000, 16, "borders"), (60, 28000, 48, "borders"), (30, 12000, 512, "borders"), (40, 16500, 1, "borders")])
+    (60, 28000, 2, "borders"), (60, 28000, 16, "borders"), (60, 28000, 48, "borders"), (30, 12000, 512, "borders"), (40, 16500, 1, "borders"),
+    # rows of one vector: the smallest and the largest tables in buckets, one row more, buckets of no, one and many segments
+    (1, 5000, 2, "one"), (2, 500000, 1, "one"), (33, 9000, 8, "uniform"), (5, 100003, 4, "skewed"), (1023, 70000, 4, "skewed"), (32768, 65536, 2, "uniform"),
+    (32769, 66000, 8, "skewed"), (100000, 262145, 4, "runs"), (1048576, 20000, 4, "uniform"), (1048577, 20000, 4, "uniform"), (1048576, 400000, 2, "skewed")])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_rows_and_exact_sums(dev, V, N, D, kind, dtype):
     from nerf_amd import ops
@@ -59,7 +62,8 @@ def test_rows_and_exact_sums(dev, V, N, D, kind, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("V,N,D,kind", [(40, 20000, 32, "uniform"), (5000, 9000, 96, "skewed"), (11, 5000, 7, "one"), (100, 100, 300, "uniform")])
+@pytest.mark.parametrize("V,N,D,kind", [(40, 20000, 32, "uniform"), (5000, 9000, 96, "skewed"), (11, 5000, 7, "one"), (100, 100, 300, "uniform"), (3000, 50000, 4, "skewed"),
+                                        (60, 9000, 2, "borders")])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_random_gradients(dev, V, N, D, kind, dtype):
     from nerf_amd import ops
@@ -113,9 +117,16 @@ def test_ids_out_of_range(dev):
     assert torch.equal(g.cpu(), torch.bincount(ids[good], minlength=V).float()[:, None].expand(V, D))
     out32 = ops.embedding(torch.tensor([-2147483648, 2147483647, 1], dtype=torch.int32, device=dev), table.detach())
     assert bool(out32[:2].isnan().all()) and torch.equal(out32[2], table.detach()[1])
-    none = ops.embedding(torch.full((500,), -5, device=dev), table)
-    (g,) = torch.autograd.grad(none, table, torch.ones_like(none))
-    assert bool((g == 0).all())
+    for n, width in ((500, D), (5000, D), (5000, 2)):     # none of them names a row
+        table = torch.randn(V, width, device=dev, requires_grad=True)
+        none = ops.embedding(torch.full((n,), -5, device=dev), table)
+        (g,) = torch.autograd.grad(none, table, torch.full_like(none, float("nan")))
+        assert bool((g == 0).all())
+    table, many = torch.randn(V, 2, device=dev, requires_grad=True), ids.repeat(40)     # rows of one vector
+    d = torch.ones(len(many), 2, device=dev)
+    d[~good.repeat(40).to(dev)] = float("nan")
+    (g,) = torch.autograd.grad(ops.embedding(many.to(dev), table), table, d)
+    assert torch.equal(g.cpu(), 40 * torch.bincount(ids[good], minlength=V).float()[:, None].expand(V, 2))
 
 
 @pytest.mark.gpu
