@@ -28,6 +28,9 @@ constexpr int SORT_ITEMS = 4, SORT_TILE = SORT_THREADS * SORT_ITEMS;   // keys t
 constexpr int SORT_BITS = 10, SORT_DIGITS = 1 << SORT_BITS;
 // One tile is sorted by one workgroup in one launch.  More keys a workgroup (16384, 16 a thread) were slower than several
 // tiles from the second tile on: 6000 ids of 1000 rows 30 us against 24, 16384 36 against 25, of 50021 rows 46 against 40.
+// Up to so many tiles the scattering workgroups count all tiles' digits themselves, a launch a pass less: 2 tiles 34 us and 37
+// (8192 ids of 50021 rows; most of them a few ids: 39 and 40), 4 tiles the same (50 and 43), 8 tiles 47 and 39.
+constexpr int SORT_OWN_TILES = 2;
 // Up to so many tiles the scattering workgroups sum the counts of the tiles in front themselves.  Against a launch of its own
 // for that: 8 tiles 38 us and 42, 32 tiles 42 and 44, 48 tiles the same, 256 tiles 89 and 65.
 constexpr int SORT_FEW_TILES = 48;
@@ -214,8 +217,8 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_small_kernel(const ID* __re
 }
 
 // More keys: per pass, the digits of every tile are counted, the counts summed over the tiles in front, and the tiles
-// ranked and scattered.  table: [tiles][digits], then [digits] totals.  With few tiles the scattering workgroups sum the
-// counts themselves (`summed` false): a launch less.
+// ranked and scattered.  table: [tiles][digits], then [digits] totals.  With few tiles the scattering workgroups count
+// or sum themselves: a launch or two less.
 template <class ID, bool FIRST>
 __global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const ID* __restrict__ ids, const uint2* __restrict__ from, int64_t n, int64_t V,
                                                                   int64_t padding, int shift, int bits, unsigned limit, int tiles, unsigned* __restrict__ table,
@@ -267,10 +270,54 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_prefix_kernel(unsigned* __r
     }
 }
 
+// How many keys of digit threadIdx.x there are in all (total) and in the tiles in front of this one (front).  With the sums of
+// sort_prefix_kernel (SUMMED), with the tiles' counts (COUNTED), or from the keys themselves: key_at(i), NO_KEY where there is
+// none, counted in s_total and s_front [digits].
+enum { SORT_SUMMED, SORT_COUNTED, SORT_UNCOUNTED };
+template <class F>
+__device__ __forceinline__ void digit_counts(int mode, const unsigned* __restrict__ table, int tiles, int digits, int shift, unsigned (&s_total)[SORT_DIGITS],
+                                             unsigned (&s_front)[SORT_DIGITS], const F& key_at, unsigned& total, unsigned& front) {
+    const int d = threadIdx.x;
+    total = front = 0;
+    if (mode == SORT_UNCOUNTED) {
+        s_total[d] = s_front[d] = 0u;
+        __syncthreads();
+        for (int t = 0; t < tiles; ++t) {
+            unsigned key[SORT_ITEMS];
+#pragma unroll
+            for (int r = 0; r < SORT_ITEMS; ++r) key[r] = key_at((int64_t)t * SORT_TILE + r * SORT_THREADS + d);
+#pragma unroll
+            for (int r = 0; r < SORT_ITEMS; ++r) {
+                if (key[r] == NO_KEY) continue;
+                const unsigned digit = (key[r] >> shift) & (unsigned)(digits - 1);
+                atomicAdd(&s_total[digit], 1u);   // whole numbers: the order does not matter
+                if (t < (int)blockIdx.x) atomicAdd(&s_front[digit], 1u);
+            }
+        }
+        __syncthreads();
+        if (d < digits) {
+            total = s_total[d];
+            front = s_front[d];
+        }
+    } else if (d < digits) {
+        if (mode == SORT_SUMMED) {
+            total = table[(int64_t)tiles * digits + d];
+            front = table[(int64_t)blockIdx.x * digits + d];
+        } else {
+#pragma unroll 8
+            for (int t = 0; t < tiles; ++t) {
+                const unsigned n_t = table[(int64_t)t * digits + d];
+                total += n_t;
+                front += t < (int)blockIdx.x ? n_t : 0u;
+            }
+        }
+    }
+}
+
 // The tile is put in order in LDS first, so that neighbouring lanes write neighbouring places of the output.
 template <class ID, bool FIRST>
 __global__ __launch_bounds__(SORT_THREADS) void sort_scatter_kernel(const ID* __restrict__ ids, const uint2* __restrict__ from, int64_t n, int64_t V, int64_t padding,
-                                                                    int shift, int bits, const unsigned* __restrict__ table, int tiles, bool summed,
+                                                                    int shift, int bits, const unsigned* __restrict__ table, int tiles, int mode,
                                                                     uint2* __restrict__ to, char* __restrict__ clear, int64_t clear_bytes) {
     if ((int)blockIdx.x >= tiles) {
         clear_table(clear, clear_bytes, blockIdx.x - tiles, gridDim.x - tiles);
@@ -300,21 +347,9 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_scatter_kernel(const ID* __
             }
         }
     }
-    // where the digit starts in the whole output, and what the tiles in front hold of it
-    unsigned total = 0, front = 0;
-    if ((int)threadIdx.x < digits) {
-        if (summed) {
-            total = table[(int64_t)tiles * digits + threadIdx.x];
-            front = table[(int64_t)blockIdx.x * digits + threadIdx.x];
-        } else {
-#pragma unroll 8
-            for (int t = 0; t < tiles; ++t) {
-                const unsigned n_t = table[(int64_t)t * digits + threadIdx.x];
-                total += n_t;
-                front += t < (int)blockIdx.x ? n_t : 0u;
-            }
-        }
-    }
+    unsigned total, front;
+    digit_counts(mode, table, tiles, digits, shift, s_to, s_count[0], [&](int64_t i) { return i >= n ? NO_KEY : FIRST ? sort_key(ids[i], V, padding) : from[i].x; }, total, front);
+    __syncthreads();
     clear_counts(s_count, digits);
     __syncthreads();
     rank_in_wave(key, on, shift, bits, s_count, rank);
@@ -571,7 +606,7 @@ __device__ __forceinline__ float row_value(const unsigned* w, int k) {
 
 template <class T, int VEC, class ID>
 __global__ __launch_bounds__(SORT_THREADS) void bucket_scatter_kernel(const ID* __restrict__ ids, int64_t n, int64_t V, int64_t padding, int low,
-                                                                      const unsigned* __restrict__ table, int tiles, const T* __restrict__ d_out,
+                                                                      unsigned* __restrict__ table, int tiles, int mode, const T* __restrict__ d_out,
                                                                       unsigned* __restrict__ to) {
     constexpr int W = row_words<T, VEC>(), ITEM = 1 + W;
     __shared__ unsigned s_count[SORT_WAVES][BUCKETS];
@@ -593,7 +628,14 @@ __global__ __launch_bounds__(SORT_THREADS) void bucket_scatter_kernel(const ID* 
         for (int k = 0; k < W; ++k) row[r][k] = 0u;
         if (i < n) row_load<T, VEC>(d_out + i * VEC, row[r]);
     }
-    const unsigned total = table[(int64_t)tiles * BUCKETS + threadIdx.x], front = table[(int64_t)blockIdx.x * BUCKETS + threadIdx.x];
+    unsigned total, front;
+    const auto key_at = [&](int64_t i) {
+        const unsigned k = i < n ? sort_key(ids[i], V, padding) : (unsigned)V;
+        return k < (unsigned)V ? k : NO_KEY;
+    };
+    digit_counts(mode, table, tiles, BUCKETS, low, s_to, s_count[0], key_at, total, front);
+    if (mode != SORT_SUMMED && blockIdx.x == 0) table[(int64_t)tiles * BUCKETS + threadIdx.x] = total;   // for the sums
+    __syncthreads();
     clear_counts(s_count, BUCKETS);
     __syncthreads();
     rank_in_wave(key, on, low, BUCKET_BITS, s_count, rank);
@@ -912,6 +954,8 @@ static int embedding_fwd_typed(const T* table, int64_t V, int D, const ID* ids, 
     });
 }
 
+static int sort_mode(int64_t tiles) { return tiles > SORT_FEW_TILES ? SORT_SUMMED : tiles > SORT_OWN_TILES ? SORT_COUNTED : SORT_UNCOUNTED; }
+
 template <class ID>
 static int embedding_sort(const ID* ids, int64_t N, int64_t V, int64_t padding, const EmbWork& w, char* work, char* clear, int64_t clear_bytes,
                           const uint2** sorted, hipStream_t stream) {
@@ -929,12 +973,14 @@ static int embedding_sort(const ID* ids, int64_t N, int64_t V, int64_t padding, 
         return check_launch("nerf_embedding_bwd(sort)");
     }
     unsigned* table = reinterpret_cast<unsigned*>(work + w.table);
+    const int mode = sort_mode(w.tiles);
     // The launches share the clearing of a large table, by the time that they take for themselves: a count one part, a scatter
-    // two.  (50021 rows of 1024 bfloat16, 102 MB, 16384 ids, two passes: 38 us with all of it beside the first count, 35 so.)
-    const int64_t part = std::max<int64_t>((ceil_div(clear_bytes, 3 * w.passes) + 15) / 16 * 16, 8 << 20);
+    // two.  (50021 rows of 1024 bfloat16, 102 MB, 16384 ids, two passes: 38 us with all of it beside the first launch, 35 so.)
+    const int parts = (mode == SORT_UNCOUNTED ? 2 : 3) * w.passes;
+    const int64_t part = std::max<int64_t>((ceil_div(clear_bytes, parts) + 15) / 16 * 16, 8 << 20);
     int64_t cleared = 0;
-    const auto share = [&](int parts) {   // the next bytes to clear
-        const int64_t bytes = std::min(parts * part, clear_bytes - cleared);
+    const auto share = [&](int n) {   // the next n parts to clear
+        const int64_t bytes = std::min(n * part, clear_bytes - cleared);
         cleared += bytes;
         return bytes;
     };
@@ -942,19 +988,19 @@ static int embedding_sort(const ID* ids, int64_t N, int64_t V, int64_t padding, 
     for (int p = 0; p < w.passes; ++p) {
         const int to = p == 0 ? 0 : 1 - from, shift = p * w.bits;
         const dim3 block(SORT_THREADS);
-        const bool summed = w.tiles > SORT_FEW_TILES;
         const auto pass = [&](auto first) {
             constexpr bool FIRST = decltype(first)::value;
             char* at = clear + cleared;
-            int64_t bytes = share(1);
-            hipLaunchKernelGGL((sort_count_kernel<ID, FIRST>), dim3((unsigned)w.tiles + clearing(bytes)), block, 0, stream, ids, (const uint2*)pairs[from], N, V, padding,
-                               shift, w.bits, NO_KEY, (int)w.tiles, table, at, bytes);
-            if (summed)
+            int64_t bytes = mode == SORT_UNCOUNTED ? 0 : share(1);
+            if (mode != SORT_UNCOUNTED)
+                hipLaunchKernelGGL((sort_count_kernel<ID, FIRST>), dim3((unsigned)w.tiles + clearing(bytes)), block, 0, stream, ids, (const uint2*)pairs[from], N, V, padding,
+                                   shift, w.bits, NO_KEY, (int)w.tiles, table, at, bytes);
+            if (mode == SORT_SUMMED)
                 hipLaunchKernelGGL(sort_prefix_kernel, dim3((unsigned)ceil_div(1 << w.bits, 64)), block, 0, stream, table, (int)w.tiles, 1 << w.bits);
             at = clear + cleared;
             bytes = share(2);
             hipLaunchKernelGGL((sort_scatter_kernel<ID, FIRST>), dim3((unsigned)w.tiles + clearing(bytes)), block, 0, stream, ids, (const uint2*)pairs[from], N, V, padding,
-                               shift, w.bits, table, (int)w.tiles, summed, pairs[to], at, bytes);
+                               shift, w.bits, table, (int)w.tiles, mode, pairs[to], at, bytes);
         };
         if (p == 0) pass(std::true_type{});
         else pass(std::false_type{});
@@ -999,10 +1045,13 @@ static int embedding_narrow_bwd(const T* d_out, const ID* ids, int64_t N, int64_
         unsigned* const items = reinterpret_cast<unsigned*>(work + w.items);
         const BucketSums p{table + w.tiles * BUCKETS, items, reinterpret_cast<float*>(work + w.part), V, w.low, w.buckets, scale};
         const dim3 tiles((unsigned)w.tiles), block(SORT_THREADS);
-        hipLaunchKernelGGL((sort_count_kernel<ID, true>), tiles, block, 0, stream, ids, (const uint2*)nullptr, N, V, padding, w.low, BUCKET_BITS, (unsigned)V, (int)w.tiles,
-                           table, (char*)nullptr, int64_t(0));
-        hipLaunchKernelGGL(sort_prefix_kernel, dim3(BUCKETS / 64), block, 0, stream, table, (int)w.tiles, BUCKETS);
-        hipLaunchKernelGGL((bucket_scatter_kernel<T, VEC, ID>), tiles, block, 0, stream, ids, N, V, padding, w.low, (const unsigned*)table, (int)w.tiles, d_out, items);
+        const int mode = sort_mode(w.tiles);
+        if (mode != SORT_UNCOUNTED)
+            hipLaunchKernelGGL((sort_count_kernel<ID, true>), tiles, block, 0, stream, ids, (const uint2*)nullptr, N, V, padding, w.low, BUCKET_BITS, (unsigned)V, (int)w.tiles,
+                               table, (char*)nullptr, int64_t(0));
+        if (mode == SORT_SUMMED)
+            hipLaunchKernelGGL(sort_prefix_kernel, dim3(BUCKETS / 64), block, 0, stream, table, (int)w.tiles, BUCKETS);
+        hipLaunchKernelGGL((bucket_scatter_kernel<T, VEC, ID>), tiles, block, 0, stream, ids, N, V, padding, w.low, table, (int)w.tiles, mode, d_out, items);
         if (int rc = check_launch("nerf_embedding_bwd(buckets)")) return rc;
         hipLaunchKernelGGL((bucket_sums_kernel<T, VEC>), dim3((unsigned)w.segments), dim3(BUCKET_THREADS), 0, stream, p, d_table);
         hipLaunchKernelGGL((bucket_join_kernel<T, VEC>), dim3((unsigned)w.buckets, (unsigned)ceil_div(1 << w.low, JOIN_IDS)), dim3(1024), 0, stream, p, d_table);
