@@ -162,8 +162,9 @@ def launch(name: str, t: torch.Tensor, *args) -> None:
     """Call an entry point on the current stream of ``t``'s device, which need not be the current device."""
     index = t.get_device()
     fn = getattr(_lib or lib(), name)
-    # the stream's handle itself: a torch.cuda.Stream object costs a microsecond, a fifth of what a small call takes
-    if index == torch.cuda.current_device():
+    # the device's and the stream's handles themselves (``t`` is on a GPU: the runtime is up): a torch.cuda.Stream object
+    # costs a microsecond, a fifth of what a small call takes
+    if index == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
@@ -172,7 +173,15 @@ def launch(name: str, t: torch.Tensor, *args) -> None:
         check(rc, name)
 
 
-def same_device(*tensors: torch.Tensor) -> None:
+def same_device(first: torch.Tensor, *others: torch.Tensor) -> None:
+    index = first.get_device()   # -1: on the CPU
+    for t in others:
+        if t is not None and t.get_device() != index:
+            break
+    else:
+        if index >= 0:
+            return
+    tensors = (first, *others)
     indices = {t.get_device() for t in tensors if t is not None}   # -1: on the CPU
     if len(indices) > 1 or -1 in indices:
         need_gpu(*tensors)

@@ -5,6 +5,7 @@ all arithmetic happens in the HIP kernels.
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Sequence
 
 import torch
@@ -217,10 +218,13 @@ def _once(*formed):
 
 
 # ----------------------------------------------------------- embedding ----
+_ID_TYPES = {torch.int64: 8, torch.int32: 4}
+
+
 def _embedding_fwd(ids, table, scale):
     V, D = table.shape
-    out = torch.empty(*ids.shape, D, device=table.device, dtype=table.dtype)
-    L.launch("nerf_embedding_fwd", table, L.ptr(table), L.TYPES[table.dtype], V, D, L.ptr(ids), ids.element_size(), ids.numel(), scale, L.ptr(out))
+    out = table.new_empty((*ids.shape, D))
+    L.launch("nerf_embedding_fwd", table, table.data_ptr(), L.TYPES[table.dtype], V, D, ids.data_ptr(), _ID_TYPES[ids.dtype], ids.numel(), scale, out.data_ptr())
     return out
 
 
@@ -228,9 +232,9 @@ def _embedding_bwd(ids, d_out, V, D, scale, padding_idx):
     """The table's gradient for dense ids and d_out."""
     N = ids.numel()
     nbytes = L.lib().nerf_embedding_bwd_workspace_bytes(N, V, D)
-    work = torch.empty(nbytes, device=d_out.device, dtype=torch.uint8) if nbytes else None
-    d_table = torch.empty(V, D, device=d_out.device, dtype=d_out.dtype)
-    L.launch("nerf_embedding_bwd", d_out, d_out.data_ptr(), L.TYPES[d_out.dtype], ids.data_ptr(), ids.element_size(), N, V, D, scale, padding_idx,
+    work = d_out.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    d_table = d_out.new_empty((V, D))
+    L.launch("nerf_embedding_bwd", d_out, d_out.data_ptr(), L.TYPES[d_out.dtype], ids.data_ptr(), _ID_TYPES[ids.dtype], N, V, D, scale, padding_idx,
              d_table.data_ptr(), L.ptr(work), nbytes)
     return d_table
 
@@ -258,25 +262,25 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, paddin
     gradient (negative: counted from the end), as in ``torch.nn.functional.embedding``.  The gradient of the table is
     dense, formed by sorting the ids -- the same bits for the same inputs, whatever ids repeat -- and summed in float32.
     Differentiable once in ``table``."""
-    if table.dim() != 2:
-        raise ValueError(f"table must be [V, D], got {tuple(table.shape)}")
-    if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
+    shape = table.shape
+    if len(shape) != 2:
+        raise ValueError(f"table must be [V, D], got {tuple(shape)}")
+    if ids.dtype not in _ID_TYPES and (ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool):
         raise ValueError(f"ids must be integers, got {ids.dtype}")
-    V = table.shape[0]
     if padding_idx is None:
         padding_idx = -1
-    elif -V <= padding_idx < V:
-        padding_idx = int(padding_idx) % V
+    elif -shape[0] <= padding_idx < shape[0]:
+        padding_idx = int(padding_idx) % shape[0]
     else:
-        raise ValueError(f"padding_idx {padding_idx} is outside the {V} rows")
+        raise ValueError(f"padding_idx {padding_idx} is outside the {shape[0]} rows")
     L.type_code(table, "table")
     L.same_device(ids, table)
-    if ids.dtype not in (torch.int64, torch.int32):
+    if ids.dtype not in _ID_TYPES:
         ids = ids.long()
     ids = ids.contiguous()
-    if torch.is_grad_enabled() and table.requires_grad:
+    if table.requires_grad and torch.is_grad_enabled():
         return _Embedding.apply(table, ids, float(scale), padding_idx)
-    return _embedding_fwd(ids, L.dense(table.detach()), float(scale))
+    return _embedding_fwd(ids, L.dense(table), float(scale))
 
 
 # ----------------------------------------------------------- composite ----
@@ -495,11 +499,11 @@ def _scan_fwd(gate, x, state, reverse, blend, want_last, keep):
     B, T, C = x.shape
     G = gate.shape[2]
     h = torch.empty_like(x)
-    last = torch.empty(B, C, device=x.device) if want_last else None
+    last = x.new_empty((B, C), dtype=torch.float32) if want_last else None
     n = lib.nerf_linear_scan_carry_floats(B, T, C, G) if keep else 0
-    carry = torch.empty(n, device=x.device) if n else None
+    carry = x.new_empty(n, dtype=torch.float32) if n else None
     n = lib.nerf_linear_scan_workspace_floats(B, T, C, G, 0)
-    work = torch.empty(n, device=x.device) if n else None
+    work = x.new_empty(n, dtype=torch.float32) if n else None
     L.launch("nerf_linear_scan_fwd", x, L.ptr(gate), L.TYPES[gate.dtype], L.ptr(x), L.TYPES[x.dtype], L.ptr(state), B, T, C, G,
              reverse, blend, L.ptr(h), L.ptr(last), L.ptr(carry), L.ptr(work))
     return h, last, carry
@@ -531,7 +535,7 @@ class _LinearScan(torch.autograd.Function):
         d_x = torch.empty_like(x) if need_x else None
         d_state = torch.empty_like(state) if need_state else None
         n = L.lib().nerf_linear_scan_workspace_floats(B, T, C, G, 1)
-        work = torch.empty(n, device=x.device) if n else None
+        work = x.new_empty(n, dtype=torch.float32) if n else None
         L.launch("nerf_linear_scan_bwd", x, L.ptr(gate), L.TYPES[gate.dtype], L.ptr(x), L.TYPES[x.dtype], L.ptr(state), L.ptr(carry),
                  L.ptr(d_h), L.ptr(d_last), B, T, C, G, *ctx.meta, L.ptr(d_gate), L.ptr(d_x), L.ptr(d_state), L.ptr(work))
         return (*_once(d_gate, d_x, d_state), None, None, None)
@@ -552,39 +556,38 @@ def linear_scan(gate: torch.Tensor, x: torch.Tensor, state: Optional[torch.Tenso
     takes as ``state`` (a long sequence in parts, or one step at a time with T = 1).
     Differentiable once in ``gate``, ``x`` and ``state``."""
     # (the texts of these checks are only put together where one fails: a call may take a few microseconds in all)
-    if x.dim() < 2:
-        raise ValueError(f"x must be [..., T, C], got {tuple(x.shape)}")
-    lead, T, C = x.shape[:-2], x.shape[-2], x.shape[-1]
-    if gate.shape[:-1] != x.shape[:-1]:
-        raise ValueError(f"gate must be {[*x.shape[:-1]]} + [G], got {tuple(gate.shape)}")
-    G = gate.shape[-1]
+    shape, gates = tuple(x.shape), tuple(gate.shape)
+    if len(shape) < 2:
+        raise ValueError(f"x must be [..., T, C], got {shape}")
+    if gates[:-1] != shape[:-1]:
+        raise ValueError(f"gate must be {[*shape[:-1]]} + [G], got {gates}")
+    T, C, G = shape[-2], shape[-1], gates[-1]
     if C != 0 and (G == 0 or C % G != 0):
         raise ValueError(f"{G} gates do not divide {C} channels")
-    if not gate.is_floating_point():
-        raise ValueError(f"gate must be floating point, got {gate.dtype}")
     if gate.dtype != x.dtype and gate.dtype != torch.float32:
+        if not gate.is_floating_point():
+            raise ValueError(f"gate must be floating point, got {gate.dtype}")
         gate = gate.float()
     if state is not None:
-        if state.shape != (*lead, C):
-            raise ValueError(f"state must be {[*lead, C]}, got {tuple(state.shape)}")
-        if not state.is_floating_point():
-            raise ValueError(f"state must be floating point, got {state.dtype}")
-        state = state.float()
+        if tuple(state.shape) != (*shape[:-2], C):
+            raise ValueError(f"state must be {[*shape[:-2], C]}, got {tuple(state.shape)}")
+        if state.dtype != torch.float32:
+            if not state.is_floating_point():
+                raise ValueError(f"state must be floating point, got {state.dtype}")
+            state = state.float()
     L.type_code(x, "x")
     L.same_device(gate, x, state)
     train = torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or (state is not None and state.requires_grad))
-    shape = x.shape
     if len(shape) != 3:   # (a view of nothing new would still be a node of the graph)
-        B = lead.numel()
+        B = math.prod(shape[:-2])
         gate, x = gate.reshape(B, T, G), x.reshape(B, T, C)
         state = state.reshape(B, C) if state is not None else None
     if train:
         h, last = _LinearScan.apply(gate, x, state, bool(reverse), bool(blend), bool(return_state))
     else:
-        h, last, _ = _scan_fwd(L.dense(gate.detach()), L.dense(x.detach()), None if state is None else L.dense(state.detach()), bool(reverse),
-                               bool(blend), bool(return_state), False)
+        h, last, _ = _scan_fwd(L.dense(gate), L.dense(x), None if state is None else L.dense(state), bool(reverse), bool(blend), bool(return_state), False)
     if len(shape) != 3:
-        h, last = h.view(shape), last.view(*lead, C) if return_state else None
+        h, last = h.view(shape), last.view(*shape[:-2], C) if return_state else None
     return (h, last) if return_state else h
 
 
