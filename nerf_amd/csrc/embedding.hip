@@ -314,7 +314,8 @@ __device__ __forceinline__ void digit_counts(int mode, const unsigned* __restric
     }
 }
 
-// The tile is put in order in LDS first, so that neighbouring lanes write neighbouring places of the output.
+// The tile is put in order in LDS first, so that neighbouring lanes write neighbouring places of the output.  Bound by the
+// chain of loads, ballots and barriers of one workgroup a tile: 8 us up to 256 tiles (2^20 keys 12 us, 16 MB moved).
 template <class ID, bool FIRST>
 __global__ __launch_bounds__(SORT_THREADS) void sort_scatter_kernel(const ID* __restrict__ ids, const uint2* __restrict__ from, int64_t n, int64_t V, int64_t padding,
                                                                     int shift, int bits, const unsigned* __restrict__ table, int tiles, int mode,
@@ -388,7 +389,8 @@ struct EmbSums {
 
 // A wave holds 64 / lanes sorted positions at a time, one per group of lanes, and adds them up by a scan that stops where
 // the id changes; what the last group holds is carried into the next round.  The rows of ROUNDS rounds are under way at
-// once.  WHOLE: all 64 lanes on one row -- the id is the wave's, and nothing changes lanes.
+// once.  WHOLE: all 64 lanes on one row -- the id is the wave's, and nothing changes lanes.  Bound by the reads of the rows,
+// and by their latency where there are few: 131072 rows of 32 float 6 us (17 MB), 16384 of 1024 bfloat16 14 us (34 MB).
 template <class T, int VEC, bool WHOLE>
 __global__ __launch_bounds__(256) void embedding_sums_kernel(EmbSums p, const T* __restrict__ d_out, T* __restrict__ d_table) {
     constexpr int ROUNDS = 8;
@@ -479,7 +481,8 @@ __global__ __launch_bounds__(256) void embedding_sums_kernel(EmbSums p, const T*
 }
 
 // The runs that cross chunks: a run belongs to the chunk that it starts in.  Those over a few chunks are joined by a
-// group of lanes each, longer ones by the whole workgroup.
+// group of lanes each, longer ones by the whole workgroup.  A few dependent reads long whatever there is to join: 7 us where
+// there is little, 13 for 40 runs over a hundred chunks each.
 template <class T, int VEC>
 __global__ __launch_bounds__(JOIN_THREADS) void embedding_join_kernel(EmbSums p, T* __restrict__ d_table) {
     constexpr int FEW = 16;   // against 8: runs over 8 to 15 chunks 39 us and 52 (262144 ids of 1000 rows), shorter ones 0.7 us more

@@ -258,6 +258,8 @@ static int clip_run(int count, float* const* grads, const int64_t* numel, long l
 // Squares and sums in double: a gradient of 1e30 has a norm, and the result does not depend on how the tensors are cut.
 // One partial sum per workgroup, which takes a contiguous stretch of 4096-element chunks (the tensor of its first
 // chunk is searched for once); the partials are folded in a fixed order.
+// Bound by the reads: 134 M elements 150 us (3.6 TB/s; reading alone reaches 4.4 here) + 5 for the coefficient, Adam behind
+// it 712 us for 28 bytes an element (5.3 TB/s); 10.4 M elements, whose gradients Adam finds in the last-level cache, 12 + 45.
 // ---------------------------------------------------------------------------
 constexpr int NORM_MAX_TENSORS = 160;   // 20 bytes of kernel arguments each
 constexpr int NORM_BLOCKS = 2048;       // workgroups of a launch, at most

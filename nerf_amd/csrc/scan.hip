@@ -22,7 +22,8 @@
 // Layout: x [B,T,C], gate [B,T,G]; the C/G = P channels of a gate are neighbours.  G = C: one "unit" of C columns per
 // batch entry; G < C: one unit of P columns per (batch entry, gate).  A workgroup of 256 threads is cut into groups of
 // CL x S threads: CL lanes side by side on the columns of a unit (VEC each), S slices of K steps.  Both passes are
-// bound by memory: the forward pass moves gate + x + h once, the backward pass gate, x, dh in and d_gate, d_x out.
+// bound by memory: the forward pass moves gate + x + h once, the backward pass gate, x, dh in and d_gate, d_x out.  16384 rays
+// x 192 x 32 float, one gate a step: 141 us for 818 MB and 233 for 1.23 GB, 5.8 and 5.3 TB/s, against 5.1 for a large copy.
 #include <algorithm>
 
 #include "typed.h"
@@ -34,6 +35,8 @@ constexpr int scan_steps(int gates) { return gates > 1 ? 4 : 8; }
 constexpr int SCAN_THREADS = 256;
 constexpr int SCAN_COLS = 64;      // most columns of a unit that one workgroup takes side by side
 constexpr int SCAN_CHANNELS = 1 << 17;   // most channels
+// Workgroups to aim for along the time axis.  65536 x 64 float: 28 us, with 512 21, with 2048 27; x 128 bfloat16 28, 28 and 46;
+// backward 8 x 2048 x 1024 bfloat16 55, 51 and 57, 16384 x 1024 59, 65 and 61, 256 x 2048 x 5 float 21, 25 and 23.
 constexpr int SCAN_WANT_BLOCKS = 1024;
 constexpr int CHAIN_GROUP = 32;    // tiles of the chain between two published states
 constexpr int CHAIN_BLOCKS = 8;    // fewest chains side by side
@@ -63,7 +66,9 @@ static ScanShape scan_shape(int64_t B, int64_t T, int C, int G, int steps = 0) {
     s.B = B; s.T = T; s.C = C; s.G = G;
     s.units_per_b = G == C ? 1 : G;
     s.P = C / s.units_per_b;
-    s.vec = s.P % 4 == 0 ? 4 : G != C && s.P <= 3 ? s.P : 1;   // colours: a lane takes all channels of its steps
+    // Two or three channels of a gate: a lane takes them all (65536 x 192 x 3 float, one gate a step: 77 us, a lane a channel 112,
+    // backward 111 and 157; x 2 49 and 105).
+    s.vec = s.P % 4 == 0 ? 4 : G != C && s.P <= 3 ? s.P : 1;
     s.steps = steps ? steps : scan_steps(G == C ? s.vec : 1);
     s.lcl = log2_up(std::min<int64_t>(ceil_div(s.P, s.vec), SCAN_COLS / s.vec));
     s.ls = std::min(log2_up(ceil_div(T, s.steps)), 8 - s.lcl);
@@ -81,12 +86,13 @@ static ScanShape scan_shape(int64_t B, int64_t T, int C, int G, int steps = 0) {
 }
 
 // Steps per thread of the forward pass in a chain: long tiles, as many steps as the registers hold beside four workgroups on
-// a compute unit.
+// a compute unit -- 16 of 16 bits (65536 x 1024 bfloat16 111 us, with 8 129; 8 x 2048 x 1024 24 and 28; 65536 x 1024 with
+// eight gates in float 68 and 89).
 constexpr int CHAIN_STEPS = 8, CHAIN_STEPS_16BIT = 16;
 // Whether the tiles of the forward pass form chains: a workgroup holds one tile of one chain, there are enough chains (a
 // chain advances by a group of tiles in about 4 us), and they are long enough to be worth clearing their words first.
-// 65536 steps of bfloat16 with float32 gates, chain against segments: 1024 channels (16 chains) 143 against 178 us, 512 (8)
-// 74 against 80, 256 (4) 68 against 47; 2048 of float32 359 against 526; 8 x 2048 x 1024 of bfloat16 25 against 35.
+// 65536 steps of bfloat16 with float32 gates, chain against segments: 1024 channels (16 chains) 141 against 179 us, 512 (8)
+// 73 against 78, 256 (4) 66 against 43; 2048 of float32 351 against 526; 8 x 2048 x 1024 of bfloat16 24 against 32.
 static bool scan_chained(const ScanShape& s, int steps = CHAIN_STEPS) {
     return s.segments > 1 && s.lcl + s.ls == 8 && s.blocks >= CHAIN_BLOCKS && s.T >= 4ll * ((int64_t)steps << s.ls);
 }
