@@ -325,6 +325,33 @@ def test_streams_and_graph(dev):
 
 
 @pytest.mark.gpu
+def test_two_streams_at_once(dev):
+    """Calls that share the compute units, chained tiles and segments among them: each as if it were alone."""
+    from nerf_amd import ops
+    shapes = [(1, 9000, 640, 640), (2, 4000, 520, 520), (1, 20000, 4, 4), (700, 192, 3, 1)]
+    data = [[t.to(dev) for t in make(*shape, F32, F32, True, k)[:4]] for k, shape in enumerate(shapes)]
+
+    def step(gate, x, s, d_h):
+        leaves = [t.detach().requires_grad_(True) for t in (gate, x, s)]
+        h = ops.linear_scan(*leaves, blend=True)
+        return [h.detach(), *torch.autograd.grad(h, leaves, d_h)]
+
+    alone = [step(*d) for d in data]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in data]
+    for stream in streams:
+        stream.wait_stream(torch.cuda.current_stream())
+    together = [None] * len(data)
+    for _ in range(5):
+        for k, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                together[k] = step(*data[k])
+    torch.cuda.synchronize()
+    for one, other in zip(alone, together):
+        assert all(torch.equal(a, b) for a, b in zip(one, other))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [3, 900])
 @pytest.mark.parametrize("G", [32768, 131072, 1])
 def test_most_channels(dev, T, G):
