@@ -15,9 +15,9 @@
 // with (kept in float by the forward pass): x costs the bytes that a saved h would, and h is not rounded on the way.
 //
 // Where there are few sequences and many steps the time axis is spread over workgroups as well, in one of two ways:
-// segments, whose (A, X) a pass of its own finds first; or, in the forward pass and with enough columns for it to keep the
-// memory busy, tiles in a chain, each of which finds the state it is entered with from what the tiles in front of it have
-// published: one pass over the data.
+// segments, whose (A, X) a pass of its own finds first; or, with enough columns for it to keep the memory busy, tiles in a
+// chain, each of which finds the state it is entered with from what the tiles in front of it (in the backward pass: behind
+// it) have published: one pass over the data.
 //
 // Layout: x [B,T,C], gate [B,T,G]; the C/G = P channels of a gate are neighbours.  G = C: one "unit" of C columns per
 // batch entry; G < C: one unit of P columns per (batch entry, gate).  A workgroup of 256 threads is cut into groups of
@@ -89,10 +89,11 @@ static ScanShape scan_shape(int64_t B, int64_t T, int C, int G, int steps = 0) {
 // a compute unit -- 16 of 16 bits (65536 x 1024 bfloat16 111 us, with 8 129; 8 x 2048 x 1024 24 and 28; 65536 x 1024 with
 // eight gates in float 68 and 89).
 constexpr int CHAIN_STEPS = 8, CHAIN_STEPS_16BIT = 16;
-// Whether the tiles of the forward pass form chains: a workgroup holds one tile of one chain, there are enough chains (a
-// chain advances by a group of tiles in about 4 us), and they are long enough to be worth clearing their words first.
+// Whether the tiles of a pass form chains: a workgroup holds one tile of one chain, there are enough chains (a chain advances
+// by a group of tiles in 2 to 4 us), and they are long enough to be worth clearing their words first.
 // 65536 steps of bfloat16 with float32 gates, chain against segments: 1024 channels (16 chains) 141 against 179 us, 512 (8)
-// 73 against 78, 256 (4) 66 against 43; 2048 of float32 351 against 526; 8 x 2048 x 1024 of bfloat16 24 against 32.
+// 70 against 78, 256 (4) 42 against 43; 2048 of float32 347 against 526; 8 x 2048 x 1024 of bfloat16 24 against 32.  Backward
+// (see there) 512 channels 133 against 131, 256 73 against 62.
 static bool scan_chained(const ScanShape& s, int steps = CHAIN_STEPS) {
     return s.segments > 1 && s.lcl + s.ls == 8 && s.blocks >= CHAIN_BLOCKS && s.T >= 4ll * ((int64_t)steps << s.ls);
 }
@@ -589,13 +590,14 @@ struct ChainPlace {
 };
 
 // Publishes the (A, X) of the order-th tile of the chain.  The waves' have been exchanged through s_a and s_x.
-template <int GV, int VEC>
+template <int GV, bool UP, int VEC>
 __device__ __forceinline__ void chain_publish(const ScanArgs& p, const ScanPlace<VEC>& w, int64_t chain, int64_t order, float (*s_a)[SCAN_COLS], float (*s_x)[SCAN_COLS]) {
     const ChainPlace<VEC> at(p, w, chain, order);
     if (w.sl != 0 || at.k == CHAIN_GROUP - 1) return;
     float A[GV], X[VEC];
     scan_identity(A, X);
-    for (int n = 0; n < w.NW; ++n) {
+    for (int i = 0; i < w.NW; ++i) {
+        const int n = UP ? i : w.NW - 1 - i;
         float A_n[GV], X_n[VEC];
 #pragma unroll
         for (int g = 0; g < GV; ++g) A_n[g] = s_a[n][w.c * VEC + g];
@@ -611,12 +613,14 @@ __device__ __forceinline__ void chain_publish(const ScanArgs& p, const ScanPlace
 }
 
 // `state`: what the recurrence starts from -> what this tile is entered with.  s_part is [CHAIN_GROUP][2][SCAN_COLS].
-template <int GV, int VEC>
+// Everything that can be composed without the group's state is composed before it is waited for, and the last tile of a
+// group hands the next group's state on as soon as it has its own: between two groups lie a read, a product and a write.
+template <int GV, bool UP, int VEC>
 __device__ __forceinline__ void chain_state(const ScanArgs& p, const ScanPlace<VEC>& w, int64_t chain, int64_t order, float (*s_a)[SCAN_COLS], float (*s_x)[SCAN_COLS],
                                             float (*s_part)[2][SCAN_COLS], float (&state)[VEC]) {
     const ChainPlace<VEC> at(p, w, chain, order);
     const int k = at.k, col = w.c * VEC;
-    const int64_t group = at.group;
+    const bool hands_on = w.sl == w.S - 1 && k == CHAIN_GROUP - 1 && order + 1 < p.s.tiles;
 #pragma unroll 1
     for (int q = w.sl; q < k; q += w.S) {
         float ax[GV + VEC];
@@ -626,34 +630,52 @@ __device__ __forceinline__ void chain_state(const ScanArgs& p, const ScanPlace<V
 #pragma unroll
         for (int v = 0; v < VEC; ++v) s_part[q][1][col + v] = ax[GV + v];
     }
-    if (group > 0 && w.sl == w.S - 1) {   // the slice that has the fewest tiles to wait for
-        float h[VEC];
-        if (w.c == 0) {   // one lane waits
-            float first[1];
-            chain_get<1, 4>(at.states, 0, first);
-        }
-        chain_get<VEC, 4>(at.states, w.CL, h);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) s_part[CHAIN_GROUP - 1][0][col + v] = h[v];
-    }
     __syncthreads();
-    if (group > 0) {
+    float A[GV], X[VEC];
+    const auto append = [&](const float* a_n, const float* x_n) {
+        float A_n[GV], X_n[VEC];
+#pragma unroll
+        for (int g = 0; g < GV; ++g) A_n[g] = a_n[col + g];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) X_n[v] = x_n[col + v];
+        scan_append(A, X, A_n, X_n);
+    };
+    scan_identity(A, X);
+#pragma unroll 2
+    for (int q = 0; q < k; ++q) append(s_part[q][0], s_part[q][1]);
+    float A_in[GV], X_in[VEC];
+#pragma unroll
+    for (int g = 0; g < GV; ++g) A_in[g] = A[g];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) X_in[v] = X[v];
+    if (hands_on) {   // this tile too
+#pragma unroll 1
+        for (int i = 0; i < w.NW; ++i) append(s_a[UP ? i : w.NW - 1 - i], s_x[UP ? i : w.NW - 1 - i]);
+    }
+    const auto hand_on = [&](const float (&h)[VEC]) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) chain_put(at.states + SCAN_COLS + v * w.CL, scan_apply(A[scan_gate<GV>(v)], h[v], X[v]));
+    };
+    if (at.group > 0) {
+        if (w.sl == w.S - 1) {   // the slice that has the fewest tiles to wait for
+            float h[VEC];
+            if (!hands_on && w.c == 0) {   // one lane waits
+                float first[1];
+                chain_get<1, 4>(at.states, 0, first);
+            }
+            chain_get<VEC, 1>(at.states, w.CL, h);
+            if (hands_on) hand_on(h);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) s_part[CHAIN_GROUP - 1][0][col + v] = h[v];
+        }
+        __syncthreads();
 #pragma unroll
         for (int v = 0; v < VEC; ++v) state[v] = s_part[CHAIN_GROUP - 1][0][col + v];
+    } else if (hands_on) {
+        hand_on(state);
     }
-#pragma unroll 2
-    for (int q = 0; q < k; ++q)
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) state[v] = scan_apply(s_part[q][0][col + scan_gate<GV>(v)], state[v], s_part[q][1][col + v]);
-    if (w.sl == 0 && k == CHAIN_GROUP - 1 && order + 1 < p.s.tiles) {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            float h = state[v];
-#pragma unroll 1
-            for (int n = 0; n < w.NW; ++n) h = scan_apply(s_a[n][col + scan_gate<GV>(v)], h, s_x[n][col + v]);
-            chain_put(at.states + SCAN_COLS + v * w.CL, h);
-        }
-    }
+    for (int v = 0; v < VEC; ++v) state[v] = scan_apply(A_in[scan_gate<GV>(v)], state[v], X_in[v]);
 }
 
 // (A, X) of whole segments -- all but the last one -- or, BACK, (A, R) of all but the first.  Nothing is written per step,
@@ -787,8 +809,8 @@ __global__ __launch_bounds__(SCAN_THREADS, CHAIN ? 4 : 1) void scan_fwd_kernel(S
         scan_wave<true>(w, A, X);
         scan_exchange<true>(w, A, X, s_a[tile & 1], s_x[tile & 1]);
         if (CHAIN) {
-            chain_publish<GV>(p, w, block, tile, s_a[tile & 1], s_x[tile & 1]);
-            chain_state<GV>(p, w, block, tile, s_a[tile & 1], s_x[tile & 1], s_part, carry);
+            chain_publish<GV, true>(p, w, block, tile, s_a[tile & 1], s_x[tile & 1]);
+            chain_state<GV, true>(p, w, block, tile, s_a[tile & 1], s_x[tile & 1], s_part, carry);
         }
         scan_carry<true>(w, A, X, carry, h, s_a[tile & 1], s_x[tile & 1]);
         if (p.carry && count > 0 && i0 > 0 && (i0 & ((1 << p.l_carry) - 1)) == 0) store_run<VEC>(p.carry + ((i0 >> p.l_carry) - 1) * BC + w.bc, h);
@@ -857,17 +879,19 @@ __device__ __forceinline__ void scan_gate_sums(const ScanArgs& p, const ScanPlac
     }
 }
 
-// The time axis is spread by segments here.  (As a chain -- 16 KB of LDS, 168 registers, three workgroups on a compute unit
-// against four -- it took 340 us for 65536 x 1024 bfloat16 with float32 gates, the two kernels 303.)
-template <class GT, class XT, int VEC, int GV, bool DENSE>
-__global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
+// CHAIN: the stretch from the other end is formed and published before the states from the front are scanned, which then
+// goes on while the other tiles' stretches arrive (published behind it: 283 us against 246 for 65536 x 1024 bfloat16 with
+// float32 gates, 281 in segments; 2048 of float32 622, 576 and 772; 8 x 16384 x 512 bfloat16, eight gates, 127, 124 and 142).
+template <class GT, class XT, int VEC, int GV, bool CHAIN, bool DENSE>
+__global__ __launch_bounds__(SCAN_THREADS, CHAIN ? 4 : 1) void scan_bwd_kernel(ScanArgs p) {
     constexpr int K = scan_steps(GV);
-    __shared__ float s_a[2][4][SCAN_COLS], s_x[2][4][SCAN_COLS], s_b[2][4][SCAN_COLS], s_r[2][4][SCAN_COLS];
+    __shared__ float s_a[2][4][SCAN_COLS], s_x[2][4][SCAN_COLS], s_b[2][4][SCAN_COLS], s_r[2][4][SCAN_COLS],
+        s_part[CHAIN ? CHAIN_GROUP : 1][2][SCAN_COLS];
     const ScanShape& s = p.s;
     unsigned block;
-    const int64_t seg = scan_segment(s, block), BC = s.B * s.C;
+    const int64_t BC = s.B * s.C, segment = scan_segment(s, block), order = CHAIN ? chain_ticket(p, block) : 0, seg = CHAIN ? s.tiles - 1 - order : segment;
     const ScanPlace<VEC> w(s, block, p.reverse);
-    const int64_t t_begin = seg * s.seg_tiles, t_end = min(t_begin + s.seg_tiles, s.tiles);
+    const int64_t t_begin = CHAIN ? seg : seg * s.seg_tiles, t_end = CHAIN ? seg + 1 : min(t_begin + s.seg_tiles, s.tiles);
     const bool shared_gate = s.G != s.C;
     float r_carry[VEC];
 #pragma unroll
@@ -875,7 +899,7 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
     if (w.on) {
         if (p.d_last) load_run<VEC>(p.d_last + w.bc, r_carry);
     }
-    scan_fold<false, GV>(p, w, seg, s_b[t_end & 1], s_r[t_end & 1], r_carry);
+    if (!CHAIN) scan_fold<false, GV>(p, w, seg, s_b[t_end & 1], s_r[t_end & 1], r_carry);
     const int64_t x_step = p.reverse ? -(int64_t)s.C : s.C, gate_step = p.reverse ? -(int64_t)s.G : s.G;
     const int64_t low = p.reverse ? K - 1 : 0;
     // (the next tile under way as in the forward pass was slower here: 151 registers against 119, 240 us against 215 for a
@@ -919,15 +943,25 @@ __global__ __launch_bounds__(SCAN_THREADS) void scan_bwd_kernel(ScanArgs p) {
             if (tile > 0) load_run<VEC>(p.carry + (tile - 1) * BC + w.bc, carry);
             else if (p.state) load_run<VEC>(p.state + w.bc, carry);
         }
+        const auto back = [&](float (&A_b)[GV], float (&R)[VEC]) {   // the tile's stretch from the other end
+            scan_local_back(a, dh, A_b, R);
+            scan_wave<false>(w, A_b, R);
+            scan_exchange<false>(w, A_b, R, s_b[tile & 1], s_r[tile & 1]);
+        };
+        float A_b[GV], R[VEC];
+        if (CHAIN) {   // others wait for it: first of all
+            back(A_b, R);
+            chain_publish<GV, false>(p, w, block, order, s_b[tile & 1], s_r[tile & 1]);
+            a.forget();
+        }
         scan_local(a, x, p.blend, A, X);
         scan_wave<true>(w, A, X);
         scan_exchange<true>(w, A, X, s_a[tile & 1], s_x[tile & 1]);
         scan_carry<true>(w, A, X, carry, h, s_a[tile & 1], s_x[tile & 1]);
         a.forget();
-        scan_local_back(a, dh, A, X);
-        scan_wave<false>(w, A, X);
-        scan_exchange<false>(w, A, X, s_b[tile & 1], s_r[tile & 1]);
-        scan_carry<false>(w, A, X, r_carry, r, s_b[tile & 1], s_r[tile & 1]);
+        if (CHAIN) chain_state<GV, false>(p, w, block, order, s_b[tile & 1], s_r[tile & 1], s_part, r_carry);
+        else back(A_b, R);
+        scan_carry<false>(w, A_b, R, r_carry, r, s_b[tile & 1], s_r[tile & 1]);
         a.forget();
         x.forget();
         dh.forget();
@@ -1005,7 +1039,7 @@ __global__ __launch_bounds__(256) void chain_clear_kernel(uint4* __restrict__ p,
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = uint4{0u, 0u, 0u, 0u};
 }
 
-template <class GT, class XT, int VEC, int GV, int K>
+template <class GT, class XT, int VEC, int GV, int K, bool BACK = false>
 static int scan_chain_launch(ScanArgs p, const char* who, hipStream_t stream) {
     p.s = scan_shape(p.s.B, p.s.T, p.s.C, p.s.G, K);
     const ChainWork work = chain_work(p.s);
@@ -1016,7 +1050,20 @@ static int scan_chain_launch(ScanArgs p, const char* who, hipStream_t stream) {
     hipLaunchKernelGGL(chain_clear_kernel, dim3((unsigned)std::min<int64_t>(2048, ceil_div(work.bytes, 4096))), dim3(256), 0, stream,
                        reinterpret_cast<uint4*>(at), work.bytes / 16);
     if (int rc = check_launch(who)) return rc;
-    hipLaunchKernelGGL((scan_fwd_kernel<GT, XT, VEC, GV, K, true, false>), dim3((unsigned)(p.s.blocks * p.s.tiles)), dim3(SCAN_THREADS), 0, stream, p);
+    if constexpr (BACK)
+        hipLaunchKernelGGL((scan_bwd_kernel<GT, XT, VEC, GV, true, false>), dim3((unsigned)(p.s.blocks * p.s.tiles)), dim3(SCAN_THREADS), 0, stream, p);
+    else
+        hipLaunchKernelGGL((scan_fwd_kernel<GT, XT, VEC, GV, K, true, false>), dim3((unsigned)(p.s.blocks * p.s.tiles)), dim3(SCAN_THREADS), 0, stream, p);
+    return check_launch(who);
+}
+
+// Where a gate's channels take several column tiles: the tiles' sums.
+template <class GT>
+static int scan_gate_total(const ScanArgs& p, const char* who, hipStream_t stream) {
+    const ScanShape& s = p.s;
+    if (!p.d_gate || s.G == s.C || s.col_tiles == 1) return NERF_OK;
+    const int64_t n = s.B * s.T * s.G;
+    hipLaunchKernelGGL((scan_gate_sum_kernel<GT>), dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, stream, p.d_gate_part, s.col_tiles, n, static_cast<GT*>(p.d_gate));
     return check_launch(who);
 }
 
@@ -1029,6 +1076,10 @@ static int scan_launch(const ScanArgs& p, int dir, const char* who, hipStream_t 
         return scan_chain_launch<GT, XT, VEC, GV, CHAIN_STEPS>(p, who, stream);
     }
     const ScanShape& s = p.s;
+    if (dir == SCAN_BWD && scan_chained(s, scan_steps(GV))) {
+        if (int rc = scan_chain_launch<GT, XT, VEC, GV, scan_steps(GV), true>(p, who, stream)) return rc;
+        return scan_gate_total<GT>(p, who, stream);
+    }
     if (s.segments > 1) {
         const dim3 grid((unsigned)(s.blocks * (s.segments - 1)));
         if (dir == SCAN_FWD) hipLaunchKernelGGL((scan_segments_kernel<GT, XT, VEC, GV, false>), grid, dim3(SCAN_THREADS), 0, stream, p);
@@ -1040,18 +1091,12 @@ static int scan_launch(const ScanArgs& p, int dir, const char* who, hipStream_t 
     if constexpr (GV == 1) {
         dense = s.C == VEC && s.G == 1 && s.T * VEC * sizeof(XT) % 16 == 0 && s.T * sizeof(GT) % 16 == 0;
         if (dense && dir == SCAN_FWD) hipLaunchKernelGGL((scan_fwd_kernel<GT, XT, VEC, 1, scan_steps(1), false, true>), grid, dim3(SCAN_THREADS), 0, stream, p);
-        else if (dense) hipLaunchKernelGGL((scan_bwd_kernel<GT, XT, VEC, 1, true>), grid, dim3(SCAN_THREADS), 0, stream, p);
+        else if (dense) hipLaunchKernelGGL((scan_bwd_kernel<GT, XT, VEC, 1, false, true>), grid, dim3(SCAN_THREADS), 0, stream, p);
     }
     if (!dense && dir == SCAN_FWD) hipLaunchKernelGGL((scan_fwd_kernel<GT, XT, VEC, GV, scan_steps(GV), false, false>), grid, dim3(SCAN_THREADS), 0, stream, p);
-    else if (!dense) hipLaunchKernelGGL((scan_bwd_kernel<GT, XT, VEC, GV, false>), grid, dim3(SCAN_THREADS), 0, stream, p);
+    else if (!dense) hipLaunchKernelGGL((scan_bwd_kernel<GT, XT, VEC, GV, false, false>), grid, dim3(SCAN_THREADS), 0, stream, p);
     if (int rc = check_launch(who)) return rc;
-    if (dir == SCAN_BWD && p.d_gate && s.G != s.C && s.col_tiles > 1) {
-        const int64_t n = s.B * s.T * s.G;
-        hipLaunchKernelGGL((scan_gate_sum_kernel<GT>), dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, stream, p.d_gate_part, s.col_tiles, n,
-                           static_cast<GT*>(p.d_gate));
-        return check_launch(who);
-    }
-    return NERF_OK;
+    return dir == SCAN_BWD ? scan_gate_total<GT>(p, who, stream) : NERF_OK;
 }
 
 template <class GT, class XT>
@@ -1071,7 +1116,7 @@ static int scan_run(const ScanArgs& p, int gate_type, int x_type, int dir, const
 
 // Floats of the workspace that hold what the workgroups along the time axis tell each other (a multiple of 4).
 static size_t scan_states_floats(const ScanShape& s, bool backward) {
-    if (!backward && scan_chained(s)) return (size_t)chain_work(scan_shape(s.B, s.T, s.C, s.G, CHAIN_STEPS)).bytes / 4;
+    if (scan_chained(s, backward ? s.steps : CHAIN_STEPS)) return (size_t)chain_work(backward ? s : scan_shape(s.B, s.T, s.C, s.G, CHAIN_STEPS)).bytes / 4;
     return s.segments > 1 ? (size_t)(2 * s.segments * ceil_div(s.B * s.C, 4) * 4) : 0;
 }
 
