@@ -106,6 +106,23 @@ def lib() -> C.CDLL:
     return _lib
 
 
+_native = None
+
+
+def native():
+    """The operators that enter autograd's graph from C++ (csrc/autograd.cpp), on this binding's library."""
+    global _native
+    if _native is None:
+        try:
+            from . import _autograd
+        except ImportError as e:
+            raise NerfHipError(f"{os.path.join(_HERE, '_autograd.so')} is missing or does not fit this torch ({e}): build it with "
+                               "`make -C nerf_amd/csrc` (or __graft_entry__.build()); nerf_amd has no fallback path") from e
+        _autograd.bind({name: C.cast(getattr(lib(), name), C.c_void_p).value for name in _autograd.entries}, NerfHipError)
+        _native = _autograd
+    return _native
+
+
 def check(rc: int, what: str) -> None:
     if rc != 0:
         msg = lib().nerf_last_error()
@@ -141,21 +158,12 @@ def f32c(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous()
 
 
-# the element types of the operators that take more than float32 (NERF_F32, NERF_BF16, NERF_F16)
-TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+TYPES = (torch.float32, torch.bfloat16, torch.float16)   # of the operators that take more than float32
 
 
-def type_code(t: torch.Tensor, what: str) -> int:
-    code = TYPES.get(t.dtype)
-    if code is None:
+def need_type(t: torch.Tensor, what: str) -> None:
+    if t.dtype not in TYPES:
         raise NerfHipError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
-    return code
-
-
-def dense(t: torch.Tensor) -> torch.Tensor:
-    """Dense view/copy that starts on a 16-byte boundary, of the tensor's own type."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def launch(name: str, t: torch.Tensor, *args) -> None:

@@ -1,0 +1,203 @@
+// The two operators that enter autograd's graph from C++: ops.embedding and ops.linear_scan.  A backward pass written in
+// Python costs a small call more than its kernels -- autograd's thread has to take the interpreter's lock and run cold
+// code -- so allocation, launch and graph node are here; ops.py checks the arguments.  Host code only: every kernel is
+// reached through the C ABI, whose functions ops.py's binding hands over (bind), so that both use one library.
+// A training call of a lookup of 2^20 ids: 58 us (its kernels 53), with the node in Python 86; of 4096 rays x 192 x 3 55, 84.
+#include <torch/extension.h>
+
+#include <c10/hip/HIPStream.h>
+
+#include "../../include/nerf_hip.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptionalTensor = std::optional<Tensor>;
+
+#define NERF_ENTRIES(X) \
+    X(nerf_last_error) X(nerf_embedding_fwd) X(nerf_embedding_bwd_workspace_bytes) X(nerf_embedding_bwd) X(nerf_linear_scan_carry_floats) \
+    X(nerf_linear_scan_workspace_floats) X(nerf_linear_scan_fwd) X(nerf_linear_scan_bwd)
+
+struct Entries {
+#define X(name) decltype(&::name) name = nullptr;
+    NERF_ENTRIES(X)
+#undef X
+} entry;
+
+PyObject* error_class = PyExc_RuntimeError;   // kept to the process's end
+struct EntryError : std::runtime_error {
+    using std::runtime_error::runtime_error;
+};
+void check(int rc, const char* name) {
+    if (rc != 0) throw EntryError(std::string(name) + " failed (" + std::to_string(rc) + "): " + entry.nerf_last_error());
+}
+
+int type_code(const Tensor& t) { return t.scalar_type() == at::kFloat ? NERF_F32 : t.scalar_type() == at::kBFloat16 ? NERF_BF16 : NERF_F16; }
+void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+void* ptr(const OptionalTensor& t) { return t && t->numel() ? t->data_ptr() : nullptr; }
+// Dense view or copy that starts on a 16-byte boundary.
+Tensor dense(const Tensor& t) {
+    Tensor c = t.contiguous();
+    return (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15) == 0 ? c : c.clone();
+}
+OptionalTensor floats(const Tensor& like, size_t n) {
+    return n ? OptionalTensor(at::empty({(int64_t)n}, like.options().dtype(at::kFloat))) : std::nullopt;
+}
+
+// A gradient that a kernel formed.  Where a graph of the gradients is asked for, differentiating it raises, whatever it
+// depends on; otherwise this does nothing.
+struct Once : torch::autograd::Function<Once> {
+    static Tensor forward(AutogradContext*, const Tensor& anchor, const Tensor& formed) { return formed.detach(); }
+    static variable_list backward(AutogradContext*, variable_list) {
+        throw std::runtime_error("this operator of nerf_amd is differentiable once: its gradients have no gradient");
+    }
+};
+Tensor once(const Tensor& formed) {
+    if (!formed.defined() || !at::GradMode::is_enabled()) return formed;
+    return Once::apply(at::empty({0}, formed.options()).set_requires_grad(true), formed);
+}
+
+// ---- embedding ----
+Tensor embedding_fwd(const Tensor& table, const Tensor& ids, double scale) {
+    auto shape = ids.sizes().vec();
+    shape.push_back(table.size(1));
+    Tensor out = at::empty(shape, table.options());
+    check(entry.nerf_embedding_fwd(table.data_ptr(), type_code(table), table.size(0), (int)table.size(1), ids.data_ptr(), (int)ids.element_size(), ids.numel(),
+                                   (float)scale, out.data_ptr(), stream_of(table)),
+          "nerf_embedding_fwd");
+    return out;
+}
+
+struct Embedding : torch::autograd::Function<Embedding> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& table, const Tensor& ids, double scale, int64_t padding) {
+        ctx->save_for_backward({ids});
+        ctx->saved_data["meta"] = std::vector<int64_t>{table.size(0), table.size(1), padding};
+        ctx->saved_data["scale"] = scale;
+        return embedding_fwd(dense(table), ids, scale);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const Tensor ids = ctx->get_saved_variables()[0];
+        const auto meta = ctx->saved_data["meta"].toIntVector();
+        const float scale = (float)ctx->saved_data["scale"].toDouble();
+        c10::DeviceGuard guard(ids.device());
+        const Tensor d_out = dense(grads[0].detach());
+        const int64_t N = ids.numel(), V = meta[0], D = meta[1];
+        const size_t bytes = entry.nerf_embedding_bwd_workspace_bytes(N, V, (int)D);
+        OptionalTensor work;
+        if (bytes) work = at::empty({(int64_t)bytes}, d_out.options().dtype(at::kByte));
+        Tensor d_table = at::empty({V, D}, d_out.options());
+        check(entry.nerf_embedding_bwd(d_out.data_ptr(), type_code(d_out), ids.data_ptr(), (int)ids.element_size(), N, V, (int)D, scale, meta[2], d_table.data_ptr(),
+                                       ptr(work), bytes, stream_of(d_out)),
+              "nerf_embedding_bwd");
+        return {once(d_table), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// ids dense, of 32 or 64 bits, on the table's device
+Tensor embedding(const Tensor& ids, const Tensor& table, double scale, int64_t padding) {
+    c10::DeviceGuard guard(table.device());
+    if (at::GradMode::is_enabled() && table.requires_grad()) return Embedding::apply(table, ids, scale, padding);
+    return embedding_fwd(dense(table), ids, scale);
+}
+
+// ---- linear recurrence ----
+struct Scanned {
+    Tensor h;
+    OptionalTensor last, carry;
+};
+// gate [B,T,G], x [B,T,C], state [B,C]: dense.  keep: with what the backward pass needs.
+Scanned scan_fwd(const Tensor& gate, const Tensor& x, const OptionalTensor& state, bool reverse, bool blend, bool want_last, bool keep) {
+    Scanned r;
+    r.h = at::empty_like(x);
+    const int64_t B = x.size(0), T = x.size(1);
+    const int C = (int)x.size(2), G = (int)gate.size(2);
+    if (x.numel() == 0) {   // the state passes through
+        if (want_last) r.last = state ? state->detach().clone() : at::zeros({B, C}, x.options().dtype(at::kFloat));
+        return r;
+    }
+    if (want_last) r.last = at::empty({B, C}, x.options().dtype(at::kFloat));
+    if (keep) r.carry = floats(r.h, entry.nerf_linear_scan_carry_floats(B, T, C, G));
+    const OptionalTensor work = floats(r.h, entry.nerf_linear_scan_workspace_floats(B, T, C, G, 0));
+    check(entry.nerf_linear_scan_fwd(gate.data_ptr(), type_code(gate), x.data_ptr(), type_code(x), static_cast<const float*>(ptr(state)), B, T, C, G, reverse, blend,
+                                     r.h.data_ptr(), static_cast<float*>(ptr(r.last)), static_cast<float*>(ptr(r.carry)), static_cast<float*>(ptr(work)), stream_of(x)),
+          "nerf_linear_scan_fwd");
+    return r;
+}
+
+struct LinearScan : torch::autograd::Function<LinearScan> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& gate_in, const Tensor& x_in, const OptionalTensor& state_in, bool reverse, bool blend, bool want_last) {
+        const Tensor gate = dense(gate_in), x = dense(x_in);
+        const OptionalTensor state = state_in ? OptionalTensor(dense(*state_in)) : std::nullopt;
+        Scanned r = scan_fwd(gate, x, state, reverse, blend, want_last, true);
+        ctx->save_for_backward({gate, x, state.value_or(Tensor()), r.carry.value_or(Tensor())});
+        ctx->saved_data["flags"] = (int64_t)(reverse | blend << 1);
+        ctx->set_materialize_grads(false);
+        return want_last ? variable_list{r.h, *r.last} : variable_list{r.h};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &gate = saved[0], &x = saved[1], &state = saved[2], &carry = saved[3];
+        const int64_t flags = ctx->saved_data["flags"].toInt();
+        c10::DeviceGuard guard(x.device());
+        const auto option = [](const Tensor& t) { return t.defined() ? OptionalTensor(t) : std::nullopt; };
+        const auto like = [](const Tensor& t, bool wanted) { return wanted ? OptionalTensor(at::empty_like(t)) : std::nullopt; };
+        const OptionalTensor d_h = grads[0].defined() ? OptionalTensor(dense(grads[0].detach())) : std::nullopt,
+                             d_last = grads.size() > 1 && grads[1].defined() ? OptionalTensor(dense(grads[1].detach())) : std::nullopt;
+        const bool needs_state = state.defined() && ctx->needs_input_grad(2);
+        OptionalTensor d_gate = like(gate, ctx->needs_input_grad(0)), d_x = like(x, ctx->needs_input_grad(1)), d_state = like(state, needs_state);
+        if (x.numel() == 0) {   // the state passes through; a gate may have elements where there are no channels
+            if (d_gate) d_gate->zero_();
+            if (d_state) d_last ? (void)d_state->copy_(*d_last) : (void)d_state->zero_();
+        } else {
+            const int64_t B = x.size(0), T = x.size(1);
+            const int C = (int)x.size(2), G = (int)gate.size(2);
+            const OptionalTensor work = floats(x.detach(), entry.nerf_linear_scan_workspace_floats(B, T, C, G, 1));
+            check(entry.nerf_linear_scan_bwd(gate.data_ptr(), type_code(gate), x.data_ptr(), type_code(x), static_cast<const float*>(ptr(option(state))),
+                                             static_cast<const float*>(ptr(option(carry))), ptr(d_h), static_cast<const float*>(ptr(d_last)), B, T, C, G, flags & 1,
+                                             flags >> 1, ptr(d_gate), ptr(d_x), static_cast<float*>(ptr(d_state)), static_cast<float*>(ptr(work)), stream_of(x)),
+                  "nerf_linear_scan_bwd");
+        }
+        return {once(d_gate.value_or(Tensor())), once(d_x.value_or(Tensor())), once(d_state.value_or(Tensor())), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// gate [B,T,G], x [B,T,C], state [B,C] float32 on one device -> h, last (None unless want_last)
+std::pair<Tensor, OptionalTensor> linear_scan(const Tensor& gate, const Tensor& x, const OptionalTensor& state, bool reverse, bool blend, bool want_last) {
+    c10::DeviceGuard guard(x.device());
+    if (at::GradMode::is_enabled() && (gate.requires_grad() || x.requires_grad() || (state && state->requires_grad()))) {
+        auto out = LinearScan::apply(gate, x, state, reverse, blend, want_last);
+        return {out[0], want_last ? OptionalTensor(out[1]) : std::nullopt};
+    }
+    Scanned r = scan_fwd(dense(gate), dense(x), state ? OptionalTensor(dense(*state)) : std::nullopt, reverse, blend, want_last, false);
+    return {r.h, r.last};
+}
+
+// addresses: of the C ABI's functions, by name; error: what a failing entry point raises
+void bind(const std::map<std::string, uintptr_t>& addresses, py::object error) {
+#define X(name) entry.name = reinterpret_cast<decltype(entry.name)>(addresses.at(#name));
+    NERF_ENTRIES(X)
+#undef X
+    error_class = error.release().ptr();
+}
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    py::register_exception_translator([](std::exception_ptr p) {
+        try {
+            if (p) std::rethrow_exception(p);
+        } catch (const EntryError& e) {
+            PyErr_SetString(error_class, e.what());
+        }
+    });
+    m.def("bind", &bind);
+    m.def("embedding", &embedding, py::call_guard<py::gil_scoped_release>());
+    m.def("linear_scan", &linear_scan, py::call_guard<py::gil_scoped_release>());
+    m.attr("entries") = std::vector<std::string>{
+#define X(name) #name,
+        NERF_ENTRIES(X)
+#undef X
+    };
+}

@@ -192,67 +192,8 @@ def hashgrid_debug(x: torch.Tensor, tables: Sequence[torch.Tensor], res: Sequenc
     return out, idx, w
 
 
-class _Once(torch.autograd.Function):
-    """Gradients that a kernel formed, as tensors whose own gradient nobody can ask for."""
-
-    @staticmethod
-    def forward(ctx, anchor, *formed):
-        return tuple(t.view_as(t) for t in formed)
-
-    @staticmethod
-    def backward(ctx, *_):
-        raise RuntimeError("this operator of nerf_amd is differentiable once: its gradients have no gradient")
-
-
-def _once(*formed):
-    """The gradients of an operator that is differentiable once.  Where a graph of them is asked for (``create_graph``),
-    differentiating them raises, whatever they depend on; otherwise this does nothing."""
-    if not torch.is_grad_enabled():
-        return formed
-    there = [i for i, t in enumerate(formed) if t is not None]
-    if not there:
-        return formed
-    anchor = torch.empty(0, device=formed[there[0]].device, requires_grad=True)
-    tied = dict(zip(there, _Once.apply(anchor, *(formed[i] for i in there))))
-    return tuple(tied.get(i) for i in range(len(formed)))
-
-
 # ----------------------------------------------------------- embedding ----
-_ID_TYPES = {torch.int64: 8, torch.int32: 4}
-
-
-def _embedding_fwd(ids, table, scale):
-    V, D = table.shape
-    out = table.new_empty((*ids.shape, D))
-    L.launch("nerf_embedding_fwd", table, table.data_ptr(), L.TYPES[table.dtype], V, D, ids.data_ptr(), _ID_TYPES[ids.dtype], ids.numel(), scale, out.data_ptr())
-    return out
-
-
-def _embedding_bwd(ids, d_out, V, D, scale, padding_idx):
-    """The table's gradient for dense ids and d_out."""
-    N = ids.numel()
-    nbytes = L.lib().nerf_embedding_bwd_workspace_bytes(N, V, D)
-    work = d_out.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    d_table = d_out.new_empty((V, D))
-    L.launch("nerf_embedding_bwd", d_out, d_out.data_ptr(), L.TYPES[d_out.dtype], ids.data_ptr(), _ID_TYPES[ids.dtype], N, V, D, scale, padding_idx,
-             d_table.data_ptr(), L.ptr(work), nbytes)
-    return d_table
-
-
-class _Embedding(torch.autograd.Function):
-    """(table [V,D], ids [...]) -> [..., D]."""
-
-    @staticmethod
-    def forward(ctx, table, ids, scale, padding_idx):
-        out = _embedding_fwd(ids, L.dense(table), scale)
-        ctx.save_for_backward(ids)
-        ctx.meta = (table.shape[0], table.shape[1], scale, padding_idx)
-        return out
-
-    @staticmethod
-    def backward(ctx, d_out):
-        (ids,) = ctx.saved_tensors
-        return (*_once(_embedding_bwd(ids, L.dense(d_out.detach()), *ctx.meta)), None, None, None)
+_ID_TYPES = (torch.int64, torch.int32)
 
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
@@ -273,14 +214,11 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, paddin
         padding_idx = int(padding_idx) % shape[0]
     else:
         raise ValueError(f"padding_idx {padding_idx} is outside the {shape[0]} rows")
-    L.type_code(table, "table")
+    L.need_type(table, "table")
     L.same_device(ids, table)
     if ids.dtype not in _ID_TYPES:
         ids = ids.long()
-    ids = ids.contiguous()
-    if table.requires_grad and torch.is_grad_enabled():
-        return _Embedding.apply(table, ids, float(scale), padding_idx)
-    return _embedding_fwd(ids, L.dense(table), float(scale))
+    return (L._native or L.native()).embedding(ids.contiguous(), table, scale, padding_idx)
 
 
 # ----------------------------------------------------------- composite ----
@@ -491,56 +429,6 @@ def render_loss(rgb, target, rgb_fine=None, weights=None, reg: float = 0.0) -> t
 
 
 # ---------------------------------------------------- linear recurrence ----
-def _scan_fwd(gate, x, state, reverse, blend, want_last, keep):
-    """Dense [B,T,G], [B,T,C], [B,C] | None -> h, last | None, carry | None (what the backward pass needs)."""
-    if x.numel() == 0:
-        return torch.empty_like(x), (None if not want_last else state.clone() if state is not None else x.new_zeros(x.shape[::2], dtype=torch.float32)), None
-    lib = L.lib()
-    B, T, C = x.shape
-    G = gate.shape[2]
-    h = torch.empty_like(x)
-    last = x.new_empty((B, C), dtype=torch.float32) if want_last else None
-    n = lib.nerf_linear_scan_carry_floats(B, T, C, G) if keep else 0
-    carry = x.new_empty(n, dtype=torch.float32) if n else None
-    n = lib.nerf_linear_scan_workspace_floats(B, T, C, G, 0)
-    work = x.new_empty(n, dtype=torch.float32) if n else None
-    L.launch("nerf_linear_scan_fwd", x, L.ptr(gate), L.TYPES[gate.dtype], L.ptr(x), L.TYPES[x.dtype], L.ptr(state), B, T, C, G,
-             reverse, blend, L.ptr(h), L.ptr(last), L.ptr(carry), L.ptr(work))
-    return h, last, carry
-
-
-class _LinearScan(torch.autograd.Function):
-    """(gate [B,T,G], x [B,T,C], state [B,C] | None) -> (h [B,T,C], last [B,C] | None)."""
-
-    @staticmethod
-    def forward(ctx, gate, x, state, reverse, blend, want_last):
-        gate, x, state = (None if t is None else L.dense(t) for t in (gate, x, state))
-        h, last, carry = _scan_fwd(gate, x, state, reverse, blend, want_last, True)
-        ctx.save_for_backward(gate, x, state, carry)
-        ctx.meta = (reverse, blend)
-        ctx.set_materialize_grads(False)
-        return h, last
-
-    @staticmethod
-    def backward(ctx, d_h, d_last):
-        gate, x, state, carry = ctx.saved_tensors
-        B, T, C = x.shape
-        G = gate.shape[2]
-        need_gate, need_x, need_state = ctx.needs_input_grad[:3]
-        if x.numel() == 0:   # the state passes through; a gate may have elements where there are no channels
-            d_state = None if not need_state else d_last.clone() if d_last is not None else torch.zeros_like(state)
-            return (*_once(torch.zeros_like(gate) if need_gate else None, torch.empty_like(x) if need_x else None, d_state), None, None, None)
-        d_h, d_last = (None if t is None else L.dense(t.detach()) for t in (d_h, d_last))
-        d_gate = torch.empty_like(gate) if need_gate else None   # (the saved tensors are dense)
-        d_x = torch.empty_like(x) if need_x else None
-        d_state = torch.empty_like(state) if need_state else None
-        n = L.lib().nerf_linear_scan_workspace_floats(B, T, C, G, 1)
-        work = x.new_empty(n, dtype=torch.float32) if n else None
-        L.launch("nerf_linear_scan_bwd", x, L.ptr(gate), L.TYPES[gate.dtype], L.ptr(x), L.TYPES[x.dtype], L.ptr(state), L.ptr(carry),
-                 L.ptr(d_h), L.ptr(d_last), B, T, C, G, *ctx.meta, L.ptr(d_gate), L.ptr(d_x), L.ptr(d_state), L.ptr(work))
-        return (*_once(d_gate, d_x, d_state), None, None, None)
-
-
 def linear_scan(gate: torch.Tensor, x: torch.Tensor, state: Optional[torch.Tensor] = None, reverse: bool = False, blend: bool = False,
                 return_state: bool = False):
     """Gated linear recurrence over the second to last axis, ``h_t = a_t h_{t-1} + x_t``, or with ``blend``
@@ -575,17 +463,13 @@ def linear_scan(gate: torch.Tensor, x: torch.Tensor, state: Optional[torch.Tenso
             if not state.is_floating_point():
                 raise ValueError(f"state must be floating point, got {state.dtype}")
             state = state.float()
-    L.type_code(x, "x")
+    L.need_type(x, "x")
     L.same_device(gate, x, state)
-    train = torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or (state is not None and state.requires_grad))
     if len(shape) != 3:   # (a view of nothing new would still be a node of the graph)
         B = math.prod(shape[:-2])
         gate, x = gate.reshape(B, T, G), x.reshape(B, T, C)
         state = state.reshape(B, C) if state is not None else None
-    if train:
-        h, last = _LinearScan.apply(gate, x, state, bool(reverse), bool(blend), bool(return_state))
-    else:
-        h, last, _ = _scan_fwd(L.dense(gate), L.dense(x), None if state is None else L.dense(state), bool(reverse), bool(blend), bool(return_state), False)
+    h, last = (L._native or L.native()).linear_scan(gate, x, state, reverse, blend, return_state)
     if len(shape) != 3:
         h, last = h.view(shape), last.view(*shape[:-2], C) if return_state else None
     return (h, last) if return_state else h
