@@ -35,8 +35,8 @@ constexpr int scan_steps(int gates) { return gates > 1 ? 4 : 8; }
 constexpr int SCAN_THREADS = 256;
 constexpr int SCAN_COLS = 64;      // most columns of a unit that one workgroup takes side by side
 constexpr int SCAN_CHANNELS = 1 << 17;   // most channels
-// Workgroups to aim for along the time axis.  65536 x 64 float: 28 us, with 512 21, with 2048 27; x 128 bfloat16 28, 28 and 46;
-// backward 8 x 2048 x 1024 bfloat16 55, 51 and 57, 16384 x 1024 59, 65 and 61, 256 x 2048 x 5 float 21, 25 and 23.
+// Workgroups to aim for along the time axis, in segments.  65536 x 64 float: 28 us, with 512 21, with 2048 27; x 128 bfloat16
+// 28, 28 and 46, backward 37, 38 and 51; x 256 backward 62, 67 and 66.
 constexpr int SCAN_WANT_BLOCKS = 1024;
 constexpr int CHAIN_GROUP = 32;    // tiles of the chain between two published states
 constexpr int CHAIN_BLOCKS = 8;    // fewest chains side by side

@@ -247,6 +247,14 @@ def test_offsets_past_32_bits(dev):
     assert bool((g == 1).all())
 
 
+def test_nodes_bind_to_the_library():
+    """The C++ nodes call the entry points that the binding names: no GPU needed."""
+    from nerf_amd import _lib as L
+    native = L.native()
+    assert native is L.native() and set(native.entries) <= set(L.SIGNATURES)
+    assert {"nerf_embedding_bwd", "nerf_linear_scan_bwd", "nerf_last_error"} <= set(native.entries)
+
+
 def test_refusals():
     from nerf_amd import ops
     from nerf_amd._lib import NerfHipError

@@ -395,6 +395,16 @@ def test_more_than_two_to_the_31_elements(dev):
         assert float((err - allow).max()) <= 0.0
 
 
+@pytest.mark.gpu
+def test_entry_points_errors_reach_python(dev):
+    from nerf_amd import ops
+    from nerf_amd._lib import NerfHipError
+    x = torch.zeros(1, 1, 131074, device=dev)
+    for leaf in (x, x.clone().requires_grad_(True)):
+        with pytest.raises(NerfHipError, match="131074 channels, at most 131072"):
+            ops.linear_scan(leaf, leaf)
+
+
 def test_refusals():
     from nerf_amd import ops
     from nerf_amd._lib import NerfHipError
