@@ -5,6 +5,7 @@
 // A training call of a lookup of 2^20 ids: 58 us (its kernels 53), with the node in Python 86; of 4096 rays x 192 x 3 55, 84.
 #include <torch/extension.h>
 
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
 #include "../../include/nerf_hip.h"
@@ -45,6 +46,18 @@ Tensor dense(const Tensor& t) {
 OptionalTensor floats(const Tensor& like, size_t n) {
     return n ? OptionalTensor(at::empty({(int64_t)n}, like.options().dtype(at::kFloat))) : std::nullopt;
 }
+
+// A leaf's gradient is accumulated on the stream where the first graph over it that is still alive was made.  While a stream
+// is captured that has to be the captured one: another stream would be drawn into the capture, which ends the process.
+void refuse_foreign_graph(const Tensor& t) {
+    if (!t.is_leaf() || !t.requires_grad()) return;
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!accumulator || !accumulator->stream()) return;
+    const c10::Stream here = c10::hip::getCurrentHIPStream(t.get_device()).unwrap();
+    if (accumulator->stream()->id() != here.id())
+        throw EntryError("a graph over this tensor that was made outside the capture is still alive: drop or detach its outputs before capturing");
+}
+bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
 
 // A gradient that a kernel formed.  Where a graph of the gradients is asked for, differentiating it raises, whatever it
 // depends on; otherwise this does nothing.
@@ -98,7 +111,10 @@ struct Embedding : torch::autograd::Function<Embedding> {
 // ids dense, of 32 or 64 bits, on the table's device
 Tensor embedding(const Tensor& ids, const Tensor& table, double scale, int64_t padding) {
     c10::DeviceGuard guard(table.device());
-    if (at::GradMode::is_enabled() && table.requires_grad()) return Embedding::apply(table, ids, scale, padding);
+    if (at::GradMode::is_enabled() && table.requires_grad()) {
+        if (capturing()) refuse_foreign_graph(table);
+        return Embedding::apply(table, ids, scale, padding);
+    }
     return embedding_fwd(dense(table), ids, scale);
 }
 
@@ -167,6 +183,11 @@ struct LinearScan : torch::autograd::Function<LinearScan> {
 std::pair<Tensor, OptionalTensor> linear_scan(const Tensor& gate, const Tensor& x, const OptionalTensor& state, bool reverse, bool blend, bool want_last) {
     c10::DeviceGuard guard(x.device());
     if (at::GradMode::is_enabled() && (gate.requires_grad() || x.requires_grad() || (state && state->requires_grad()))) {
+        if (capturing()) {
+            refuse_foreign_graph(gate);
+            refuse_foreign_graph(x);
+            if (state) refuse_foreign_graph(*state);
+        }
         auto out = LinearScan::apply(gate, x, state, reverse, blend, want_last);
         return {out[0], want_last ? OptionalTensor(out[1]) : std::nullopt};
     }

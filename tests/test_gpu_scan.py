@@ -325,6 +325,35 @@ def test_streams_and_graph(dev):
 
 
 @pytest.mark.gpu
+def test_capture_refuses_a_live_eager_graph(dev):
+    """Nothing of the refused call is captured; without the eager graph it is, and replays."""
+    from nerf_amd import ops
+    from nerf_amd._lib import NerfHipError
+    gate, x, _, d_h, _ = (t.to(dev) if t is not None else None for t in make(3, 70, 8, 2, F32, F32, False, 3))
+    table, ids = torch.randn(9, 8, device=dev, requires_grad=True), torch.arange(70, device=dev).expand(3, 70) % 9
+    leaf = x.clone().requires_grad_(True)
+    calls = {"scan": lambda: ops.linear_scan(gate, leaf), "lookup": lambda: ops.embedding(ids, table)}
+    for name, of in (("scan", leaf), ("lookup", table)):
+        call = calls[name]
+        kept = call()
+        want = torch.autograd.grad(kept, of, d_h, retain_graph=True)[0]
+        torch.cuda.synchronize()
+        with pytest.raises(NerfHipError, match="still alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+        del kept
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = torch.autograd.grad(call(), of, d_h)[0]
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want), name
+
+
+@pytest.mark.gpu
 def test_two_streams_at_once(dev):
     """Calls that share the compute units, chained tiles and segments among them: each as if it were alone."""
     from nerf_amd import ops
