@@ -166,21 +166,6 @@ def need_type(t: torch.Tensor, what: str) -> None:
         raise NerfHipError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
 
 
-def launch(name: str, t: torch.Tensor, *args) -> None:
-    """Call an entry point on the current stream of ``t``'s device, which need not be the current device."""
-    index = t.get_device()
-    fn = getattr(_lib or lib(), name)
-    # the device's and the stream's handles themselves (``t`` is on a GPU: the runtime is up): a torch.cuda.Stream object
-    # costs a microsecond, a fifth of what a small call takes
-    if index == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if rc != 0:
-        check(rc, name)
-
-
 def same_device(first: torch.Tensor, *others: torch.Tensor) -> None:
     index = first.get_device()   # -1: on the CPU
     for t in others:

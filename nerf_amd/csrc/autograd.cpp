@@ -1,4 +1,5 @@
-// The two operators that enter autograd's graph from C++: ops.embedding and ops.linear_scan.  A backward pass written in
+// What of the package's host side is in C++: the two operators that enter autograd's graph from here, ops.embedding and
+// ops.linear_scan, and the pointer lists of the clipped optimiser step.  A backward pass written in
 // Python costs a small call more than its kernels -- autograd's thread has to take the interpreter's lock and run cold
 // code -- so allocation, launch and graph node are here; ops.py checks the arguments.  Host code only: every kernel is
 // reached through the C ABI, whose functions ops.py's binding hands over (bind), so that both use one library.
@@ -19,7 +20,8 @@ using OptionalTensor = std::optional<Tensor>;
 
 #define NERF_ENTRIES(X) \
     X(nerf_last_error) X(nerf_embedding_fwd) X(nerf_embedding_bwd_workspace_bytes) X(nerf_embedding_bwd) X(nerf_linear_scan_carry_floats) \
-    X(nerf_linear_scan_workspace_floats) X(nerf_linear_scan_fwd) X(nerf_linear_scan_bwd)
+    X(nerf_linear_scan_workspace_floats) X(nerf_linear_scan_fwd) X(nerf_linear_scan_bwd) X(nerf_grad_norm_workspace_doubles) X(nerf_grad_norm) \
+    X(nerf_adam_step_scaled)
 
 struct Entries {
 #define X(name) decltype(&::name) name = nullptr;
@@ -195,6 +197,57 @@ std::pair<Tensor, OptionalTensor> linear_scan(const Tensor& gate, const Tensor& 
     return {r.h, r.last};
 }
 
+// ---- clipped Adam (FusedAdam) ----
+using Tensors = std::vector<Tensor>;
+template <class T>
+std::vector<T*> pointers(const Tensors& list) {
+    std::vector<T*> out;
+    for (const Tensor& t : list) out.push_back(static_cast<T*>(t.data_ptr()));
+    return out;
+}
+std::vector<int64_t> counts(const Tensors& list) {
+    std::vector<int64_t> out;
+    for (const Tensor& t : list) out.push_back(t.numel());
+    return out;
+}
+
+// The norm of grads and the coefficient that it leads to -> norm[0], norm[1].  Returns the gradients as the optimiser's
+// kernels take them if they are not so already.
+std::optional<Tensors> grad_norm(const Tensors& params, Tensors grads, double max_norm, const Tensor& norm) {
+    bool changed = false;
+    for (size_t i = 0; i < params.size(); ++i) {
+        const Tensor& p = params[i];
+        Tensor& g = grads[i];
+        if (g.layout() != at::kStrided) throw EntryError("FusedAdam does not take sparse gradients");
+        if (p.scalar_type() != at::kFloat || !p.is_contiguous()) throw EntryError("FusedAdam needs contiguous float32 parameters");
+        if (!p.is_cuda()) throw EntryError("nerf_amd ops run on the GPU only: got a tensor on " + p.device().str());
+        if (p.device() != norm.device() || g.device() != norm.device()) throw EntryError("FusedAdam: all parameters and gradients must be on one device");
+        if (g.scalar_type() == at::kFloat && g.is_contiguous()) continue;
+        g = g.to(at::kFloat).contiguous();
+        changed = true;
+    }
+    c10::DeviceGuard guard(norm.device());
+    const auto n = counts(grads);
+    const auto at = pointers<const float>(grads);
+    const Tensor partials = at::empty({(int64_t)entry.nerf_grad_norm_workspace_doubles((int)n.size(), n.data())}, norm.options().dtype(at::kDouble));
+    check(entry.nerf_grad_norm((int)n.size(), at.data(), n.data(), (float)max_norm, static_cast<double*>(partials.data_ptr()), static_cast<float*>(norm.data_ptr()),
+                               stream_of(norm)),
+          "nerf_grad_norm");
+    return changed ? std::optional<Tensors>(std::move(grads)) : std::nullopt;
+}
+
+// One update with the gradients times norm[1]; `state`: of a group whose count and rate are in device memory.
+void adam_step(const Tensors& params, const Tensors& grads, const Tensors& m, const Tensors& v, int64_t step, const OptionalTensor& state, double lr, double beta1,
+               double beta2, double eps, double weight_decay, const Tensor& norm) {
+    c10::DeviceGuard guard(norm.device());
+    const auto n = counts(params);
+    const auto p_at = pointers<float>(params), m_at = pointers<float>(m), v_at = pointers<float>(v);
+    const auto g_at = pointers<const float>(grads);
+    check(entry.nerf_adam_step_scaled((int)n.size(), p_at.data(), g_at.data(), m_at.data(), v_at.data(), n.data(), step, static_cast<float*>(ptr(state)), (float)lr,
+                                      beta1, beta2, (float)eps, (float)weight_decay, static_cast<const float*>(norm.data_ptr()) + 1, stream_of(norm)),
+          "nerf_adam_step_scaled");
+}
+
 // addresses: of the C ABI's functions, by name; error: what a failing entry point raises
 void bind(const std::map<std::string, uintptr_t>& addresses, py::object error) {
 #define X(name) entry.name = reinterpret_cast<decltype(entry.name)>(addresses.at(#name));
@@ -216,6 +269,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("bind", &bind);
     m.def("embedding", &embedding, py::call_guard<py::gil_scoped_release>());
     m.def("linear_scan", &linear_scan, py::call_guard<py::gil_scoped_release>());
+    m.def("grad_norm", &grad_norm, py::call_guard<py::gil_scoped_release>());
+    m.def("adam_step", &adam_step, py::call_guard<py::gil_scoped_release>());
     m.attr("entries") = std::vector<std::string>{
 #define X(name) #name,
         NERF_ENTRIES(X)

@@ -110,35 +110,25 @@ class FusedAdam(torch.optim.Optimizer):
         return None if self._norm is None else self._norm[0]
 
     def _step_clipped(self) -> None:
-        lib = L.lib()
-        work = []   # per group: its index, the group, parameters, gradients, states
+        native = L.native()
+        work = []   # per group: its index, the group, parameters, gradients
         for gi, group in enumerate(self.param_groups):
             ps = [p for p in group["params"] if p.grad is not None]
-            if not ps:
-                continue
-            grads = [p.grad for p in ps]
-            if any(g.is_sparse for g in grads):
-                raise L.NerfHipError("FusedAdam does not take sparse gradients")
-            if not all(p.dtype == torch.float32 and p.is_contiguous() for p in ps):
-                raise L.NerfHipError("FusedAdam needs contiguous float32 parameters")
-            work.append((gi, group, ps, [g if g.dtype == torch.float32 and g.is_contiguous() else L.f32c(g) for g in grads]))
+            if ps:
+                work.append((gi, group, ps, [p.grad for p in ps]))
         if not work:
             if self._norm is not None:
                 self._norm[0] = 0.0
             return
-        every = work[0][3] if len(work) == 1 else [g for _, _, _, grads in work for g in grads]
-        devices = {t.get_device() for _, _, ps, grads in work for ts in (ps, grads) for t in ts}
-        if len(devices) > 1 or -1 in devices:
-            L.same_device(*[p for _, _, ps, _ in work for p in ps], *every)
-        if self._norm is None or self._norm.device != every[0].device:
-            self._norm = torch.zeros(2, device=every[0].device)
-        n = len(every)
-        numel = (C.c_int64 * n)(*[g.numel() for g in every])
-        pointers = (C.c_void_p * n)(*[g.data_ptr() for g in every])
-        partials = torch.empty(lib.nerf_grad_norm_workspace_doubles(n, numel), device=every[0].device, dtype=torch.float64)
-        L.launch("nerf_grad_norm", every[0], n, pointers, numel, float(self.max_grad_norm), L.ptr(partials), L.ptr(self._norm))
-        coef = self._norm.data_ptr() + 4
-        for gi, group, ps, grads in work:
+        every_p = work[0][2] if len(work) == 1 else [p for _, _, ps, _ in work for p in ps]
+        every_g = work[0][3] if len(work) == 1 else [g for _, _, _, grads in work for g in grads]
+        if self._norm is None or self._norm.device != every_p[0].device:
+            self._norm = torch.zeros(2, device=every_p[0].device)
+        every_g = native.grad_norm(every_p, every_g, self.max_grad_norm, self._norm) or every_g   # (as the kernels take them)
+        first = 0
+        for gi, group, ps, _ in work:
+            grads = every_g if len(work) == 1 else every_g[first:first + len(ps)]
+            first += len(ps)
             states = [self.state[p] for p in ps]
             for p, st in zip(ps, states):
                 if not st:
@@ -152,16 +142,10 @@ class FusedAdam(torch.optim.Optimizer):
             else:
                 dev, parts = None, self._shared_steps(states)
             beta1, beta2 = group["betas"]
+            ms, vs = [st["exp_avg"] for st in states], [st["exp_avg_sq"] for st in states]
             for step0, step, part in parts:
-                m = len(part)
-                ms, vs = [states[i]["exp_avg"].data_ptr() for i in part], [states[i]["exp_avg_sq"].data_ptr() for i in part]
-                if m == n:   # the one list of the one group: as the norm had it
-                    gp, counts, pp = pointers, numel, [p.data_ptr() for p in ps]
-                else:
-                    gp = (C.c_void_p * m)(*[grads[i].data_ptr() for i in part])
-                    counts, pp = (C.c_int64 * m)(*[ps[i].numel() for i in part]), [ps[i].data_ptr() for i in part]
-                L.launch("nerf_adam_step_scaled", ps[0], m, (C.c_void_p * m)(*pp), gp, (C.c_void_p * m)(*ms), (C.c_void_p * m)(*vs), counts,
-                         step0 + 1, L.ptr(dev), group["lr"], beta1, beta2, group["eps"], group["weight_decay"], coef)
+                lists = (ps, grads, ms, vs) if len(part) == len(ps) else tuple([ts[i] for i in part] for ts in (ps, grads, ms, vs))
+                native.adam_step(*lists, step0 + 1, dev, group["lr"], beta1, beta2, group["eps"], group["weight_decay"], self._norm)
                 if step is not None:
                     step = step + 1   # a new tensor: a parameter without a gradient in this step keeps the old one
                     for i in part:
@@ -173,6 +157,9 @@ class FusedAdam(torch.optim.Optimizer):
         states were loaded piecemeal or a parameter had no gradient in some step.  The members of a part are left with
         one step tensor between them, which is never written, so that counting a step is one operation and not one per
         parameter (``state_dict`` hands out a copy for each)."""
+        first = states[0]["step"]
+        if all([st["step"] is first for st in states]):
+            return [(int(first.item()), first, range(len(states)))]
         by_tensor = {}
         for i, st in enumerate(states):
             by_tensor.setdefault(id(st["step"]), []).append(i)
