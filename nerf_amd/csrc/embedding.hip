@@ -24,15 +24,20 @@ constexpr int JOIN_THREADS = 512;
 constexpr int JOIN_CHUNKS = 64;      // most chunks whose crossing runs one workgroup joins
 
 constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
-constexpr int SORT_ITEMS = 4, SORT_TILE = SORT_THREADS * SORT_ITEMS;   // keys that a workgroup ranks at once
+// Keys that a workgroup ranks at once: 4 a thread with more than SORT_MANY of them, else 1, so that more workgroups share the
+// ranking.  16384 ids of 50021 rows of 64 float: 37 us with 4, 34 with 1 (most of them a few ids: 42 and 37); 2^17 49 and 48;
+// 2^20 121 and 142.
+constexpr int SORT_ITEMS = 4, SORT_TILE = SORT_THREADS * SORT_ITEMS;
+constexpr int64_t SORT_MANY = 1 << 17;
+constexpr int sort_items(int64_t n) { return n > SORT_MANY ? SORT_ITEMS : 1; }
 constexpr int SORT_BITS = 10, SORT_DIGITS = 1 << SORT_BITS;
-// One tile is sorted by one workgroup in one launch.  More keys a workgroup (16384, 16 a thread) were slower than several
-// tiles from the second tile on: 6000 ids of 1000 rows 30 us against 24, 16384 36 against 25, of 50021 rows 46 against 40.
-// Up to so many tiles the scattering workgroups count all tiles' digits themselves, a launch a pass less: 2 tiles 34 us and 37
-// (8192 ids of 50021 rows; most of them a few ids: 39 and 40), 4 tiles the same (50 and 43), 8 tiles 47 and 39.
-constexpr int SORT_OWN_TILES = 2;
-// Up to so many tiles the scattering workgroups sum the counts of the tiles in front themselves.  Against a launch of its own
-// for that: 8 tiles 38 us and 42, 32 tiles 42 and 44, 48 tiles the same, 256 tiles 89 and 65.
+// Up to SORT_TILE keys are sorted by one workgroup in one launch.  More keys a workgroup (16384, 16 a thread) were slower than
+// several tiles: 6000 ids of 1000 rows 30 us against 24, 16384 36 against 25, of 50021 rows 46 against 40.
+// Up to so many tiles the scattering workgroups count all tiles' digits themselves, a launch a pass less (4 us for the host):
+// 8 tiles 19.7 us against 21.5 (8192 ids of 2^19 rows of two floats), 21 and 22 (of 40 rows; 28 and 24 where a few ids are most).
+constexpr int SORT_OWN_TILES = 8;
+// Up to so many tiles they sum the counts of the tiles in front themselves.  Against a launch of its own for that: 64 tiles 42
+// us and 44 (65536 ids of 50021 rows of 64 float), 27 and 25 (of 2^19 rows of two floats), 128 tiles 54 and 47, 36 and 25.
 constexpr int SORT_FEW_TILES = 48;
 constexpr unsigned NO_KEY = 0xffffffffu;
 
@@ -219,7 +224,7 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_small_kernel(const ID* __re
 // More keys: per pass, the digits of every tile are counted, the counts summed over the tiles in front, and the tiles
 // ranked and scattered.  table: [tiles][digits], then [digits] totals.  With few tiles the scattering workgroups count
 // or sum themselves: a launch or two less.
-template <class ID, bool FIRST>
+template <class ID, bool FIRST, int ITEMS>
 __global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const ID* __restrict__ ids, const uint2* __restrict__ from, int64_t n, int64_t V,
                                                                   int64_t padding, int shift, int bits, unsigned limit, int tiles, unsigned* __restrict__ table,
                                                                   char* __restrict__ clear, int64_t clear_bytes) {
@@ -231,8 +236,8 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(const ID* __re
     const int digits = 1 << bits;
     for (int i = threadIdx.x; i < digits; i += SORT_THREADS) s_count[i] = 0u;
     __syncthreads();
-    const int64_t base = (int64_t)blockIdx.x * SORT_TILE;
-    for (int r = 0; r < SORT_ITEMS; ++r) {
+    const int64_t base = (int64_t)blockIdx.x * (SORT_THREADS * ITEMS);
+    for (int r = 0; r < ITEMS; ++r) {
         const int64_t i = base + r * SORT_THREADS + threadIdx.x;
         if (i < n) {
             const unsigned key = FIRST ? sort_key(ids[i], V, padding) : from[i].x;
@@ -274,7 +279,7 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_prefix_kernel(unsigned* __r
 // sort_prefix_kernel (SUMMED), with the tiles' counts (COUNTED), or from the keys themselves: key_at(i), NO_KEY where there is
 // none, counted in s_total and s_front [digits].
 enum { SORT_SUMMED, SORT_COUNTED, SORT_UNCOUNTED };
-template <class F>
+template <int ITEMS, class F>
 __device__ __forceinline__ void digit_counts(int mode, const unsigned* __restrict__ table, int tiles, int digits, int shift, unsigned (&s_total)[SORT_DIGITS],
                                              unsigned (&s_front)[SORT_DIGITS], const F& key_at, unsigned& total, unsigned& front) {
     const int d = threadIdx.x;
@@ -283,11 +288,11 @@ __device__ __forceinline__ void digit_counts(int mode, const unsigned* __restric
         s_total[d] = s_front[d] = 0u;
         __syncthreads();
         for (int t = 0; t < tiles; ++t) {
-            unsigned key[SORT_ITEMS];
+            unsigned key[ITEMS];
 #pragma unroll
-            for (int r = 0; r < SORT_ITEMS; ++r) key[r] = key_at((int64_t)t * SORT_TILE + r * SORT_THREADS + d);
+            for (int r = 0; r < ITEMS; ++r) key[r] = key_at((int64_t)t * (SORT_THREADS * ITEMS) + r * SORT_THREADS + d);
 #pragma unroll
-            for (int r = 0; r < SORT_ITEMS; ++r) {
+            for (int r = 0; r < ITEMS; ++r) {
                 if (key[r] == NO_KEY) continue;
                 const unsigned digit = (key[r] >> shift) & (unsigned)(digits - 1);
                 atomicAdd(&s_total[digit], 1u);   // whole numbers: the order does not matter
@@ -316,7 +321,7 @@ __device__ __forceinline__ void digit_counts(int mode, const unsigned* __restric
 
 // The tile is put in order in LDS first, so that neighbouring lanes write neighbouring places of the output.  Bound by the
 // chain of loads, ballots and barriers of one workgroup a tile: 8 us up to 256 tiles (2^20 keys 12 us, 16 MB moved).
-template <class ID, bool FIRST>
+template <class ID, bool FIRST, int ITEMS>
 __global__ __launch_bounds__(SORT_THREADS) void sort_scatter_kernel(const ID* __restrict__ ids, const uint2* __restrict__ from, int64_t n, int64_t V, int64_t padding,
                                                                     int shift, int bits, const unsigned* __restrict__ table, int tiles, int mode,
                                                                     uint2* __restrict__ to, char* __restrict__ clear, int64_t clear_bytes) {
@@ -327,14 +332,14 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_scatter_kernel(const ID* __
     __shared__ unsigned s_count[SORT_WAVES][SORT_DIGITS];
     __shared__ unsigned s_to[SORT_DIGITS];   // what a rank in the sorted tile lacks to its place in the output, per digit
     __shared__ unsigned s_wave[SORT_WAVES];
-    __shared__ uint2 s_pair[SORT_TILE];
+    __shared__ uint2 s_pair[(SORT_THREADS * ITEMS)];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, digits = 1 << bits;
-    const int64_t tile = (int64_t)blockIdx.x * SORT_TILE;
-    unsigned key[SORT_ITEMS], val[SORT_ITEMS], rank[SORT_ITEMS];
-    bool on[SORT_ITEMS];
+    const int64_t tile = (int64_t)blockIdx.x * (SORT_THREADS * ITEMS);
+    unsigned key[ITEMS], val[ITEMS], rank[ITEMS];
+    bool on[ITEMS];
 #pragma unroll
-    for (int r = 0; r < SORT_ITEMS; ++r) {
-        const int64_t i = tile + (wave * SORT_ITEMS + r) * 64 + lane;
+    for (int r = 0; r < ITEMS; ++r) {
+        const int64_t i = tile + (wave * ITEMS + r) * 64 + lane;
         on[r] = i < n;
         key[r] = val[r] = 0u;
         if (on[r]) {
@@ -349,7 +354,7 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_scatter_kernel(const ID* __
         }
     }
     unsigned total, front;
-    digit_counts(mode, table, tiles, digits, shift, s_to, s_count[0], [&](int64_t i) { return i >= n ? NO_KEY : FIRST ? sort_key(ids[i], V, padding) : from[i].x; }, total, front);
+    digit_counts<ITEMS>(mode, table, tiles, digits, shift, s_to, s_count[0], [&](int64_t i) { return i >= n ? NO_KEY : FIRST ? sort_key(ids[i], V, padding) : from[i].x; }, total, front);
     __syncthreads();
     clear_counts(s_count, digits);
     __syncthreads();
@@ -361,11 +366,11 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_scatter_kernel(const ID* __
     if ((int)threadIdx.x < digits) s_to[threadIdx.x] = first + front - start;
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < SORT_ITEMS; ++r)
+    for (int r = 0; r < ITEMS; ++r)
         if (on[r]) s_pair[s_count[wave][(key[r] >> shift) & (unsigned)(digits - 1)] + rank[r]] = uint2{key[r], val[r]};
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < SORT_ITEMS; ++r) {
+    for (int r = 0; r < ITEMS; ++r) {
         const int i = r * SORT_THREADS + (int)threadIdx.x;
         if (tile + i < n) {
             const uint2 pair = s_pair[i];
@@ -607,7 +612,7 @@ __device__ __forceinline__ float row_value(const unsigned* w, int k) {
     else return (float)__builtin_bit_cast(T, (unsigned short)(w[k / 2] >> (k & 1) * 16));
 }
 
-template <class T, int VEC, class ID>
+template <class T, int VEC, class ID, int ITEMS>
 __global__ __launch_bounds__(SORT_THREADS) void bucket_scatter_kernel(const ID* __restrict__ ids, int64_t n, int64_t V, int64_t padding, int low,
                                                                       unsigned* __restrict__ table, int tiles, int mode, const T* __restrict__ d_out,
                                                                       unsigned* __restrict__ to) {
@@ -615,16 +620,16 @@ __global__ __launch_bounds__(SORT_THREADS) void bucket_scatter_kernel(const ID* 
     __shared__ unsigned s_count[SORT_WAVES][BUCKETS];
     __shared__ unsigned s_to[BUCKETS];   // as in sort_scatter_kernel
     __shared__ unsigned s_wave[SORT_WAVES];
-    __shared__ unsigned s_item[SORT_TILE * ITEM];
+    __shared__ unsigned s_item[(SORT_THREADS * ITEMS) * ITEM];
     __shared__ int s_held;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t tile = (int64_t)blockIdx.x * SORT_TILE;
-    unsigned key[SORT_ITEMS], rank[SORT_ITEMS], row[SORT_ITEMS][W];
-    bool on[SORT_ITEMS];
+    const int64_t tile = (int64_t)blockIdx.x * (SORT_THREADS * ITEMS);
+    unsigned key[ITEMS], rank[ITEMS], row[ITEMS][W];
+    bool on[ITEMS];
     if (threadIdx.x == 0) s_held = 0;
 #pragma unroll
-    for (int r = 0; r < SORT_ITEMS; ++r) {
-        const int64_t i = tile + (wave * SORT_ITEMS + r) * 64 + lane;
+    for (int r = 0; r < ITEMS; ++r) {
+        const int64_t i = tile + (wave * ITEMS + r) * 64 + lane;
         key[r] = i < n ? sort_key(ids[i], V, padding) : (unsigned)V;
         on[r] = key[r] < (unsigned)V;
 #pragma unroll
@@ -636,14 +641,14 @@ __global__ __launch_bounds__(SORT_THREADS) void bucket_scatter_kernel(const ID* 
         const unsigned k = i < n ? sort_key(ids[i], V, padding) : (unsigned)V;
         return k < (unsigned)V ? k : NO_KEY;
     };
-    digit_counts(mode, table, tiles, BUCKETS, low, s_to, s_count[0], key_at, total, front);
+    digit_counts<ITEMS>(mode, table, tiles, BUCKETS, low, s_to, s_count[0], key_at, total, front);
     if (mode != SORT_SUMMED && blockIdx.x == 0) table[(int64_t)tiles * BUCKETS + threadIdx.x] = total;   // for the sums
     __syncthreads();
     clear_counts(s_count, BUCKETS);
     __syncthreads();
     rank_in_wave(key, on, low, BUCKET_BITS, s_count, rank);
 #pragma unroll
-    for (int r = 0; r < SORT_ITEMS; ++r) {
+    for (int r = 0; r < ITEMS; ++r) {
         const int held = __popcll(__ballot(on[r]));
         if (lane == 0) atomicAdd(&s_held, held);
     }
@@ -654,7 +659,7 @@ __global__ __launch_bounds__(SORT_THREADS) void bucket_scatter_kernel(const ID* 
     s_to[threadIdx.x] = first + front - start;
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < SORT_ITEMS; ++r) {
+    for (int r = 0; r < ITEMS; ++r) {
         if (on[r]) {
             unsigned* const at = s_item + (s_count[wave][key[r] >> low] + rank[r]) * ITEM;
             at[0] = key[r];
@@ -664,7 +669,7 @@ __global__ __launch_bounds__(SORT_THREADS) void bucket_scatter_kernel(const ID* 
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < SORT_ITEMS; ++r) {
+    for (int r = 0; r < ITEMS; ++r) {
         const int i = r * SORT_THREADS + (int)threadIdx.x;
         if (i < s_held) {
             const unsigned* const from = s_item + i * ITEM;
@@ -896,7 +901,7 @@ static EmbWork embedding_work(int64_t N, int64_t V, int D) {
     const bool small = N <= SORT_TILE;
     w.passes = (int)ceil_div(bits, SORT_BITS);
     w.bits = (int)ceil_div(bits, w.passes);
-    w.tiles = small ? 1 : ceil_div(N, SORT_TILE);
+    w.tiles = small ? 1 : ceil_div(N, SORT_THREADS * sort_items(N));
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t from = at;
@@ -912,8 +917,9 @@ static EmbWork embedding_work(int64_t N, int64_t V, int D) {
     return w;
 }
 
-// Narrow rows: one vector each, more ids than one workgroup sorts, more rows than one pass sorts by, few enough for the buckets.
-static bool embedding_narrow(int64_t N, int64_t V, int D, int size) { return N > SORT_TILE && V >= SORT_DIGITS && V <= 1ll << BUCKET_MOST_BITS && vector_of(D, size) == D; }
+// Narrow rows: one vector each, more ids than one tile, more rows than one pass sorts by, few enough for the buckets.  (2048 ids
+// of 2^19 rows of two floats: 18 us, sorted by one workgroup 22.)
+static bool embedding_narrow(int64_t N, int64_t V, int D, int size) { return N > SORT_THREADS && V >= SORT_DIGITS && V <= 1ll << BUCKET_MOST_BITS && vector_of(D, size) == D; }
 
 struct NarrowWork {
     int low, buckets;
@@ -925,7 +931,7 @@ static NarrowWork narrow_work(int64_t N, int64_t V, int D) {   // for elements o
     w.low = BUCKET_LOW;
     while (BUCKETS << w.low < V) ++w.low;
     w.buckets = (int)ceil_div(V, 1 << w.low);
-    w.tiles = ceil_div(N, SORT_TILE);
+    w.tiles = ceil_div(N, SORT_THREADS * sort_items(N));
     w.segments = w.buckets + N / BUCKET_SEG;
     w.table = 0;
     w.items = 4ull * (w.tiles + 1) * BUCKETS;
@@ -959,13 +965,20 @@ static int embedding_fwd_typed(const T* table, int64_t V, int D, const ID* ids, 
 
 static int sort_mode(int64_t tiles) { return tiles > SORT_FEW_TILES ? SORT_SUMMED : tiles > SORT_OWN_TILES ? SORT_COUNTED : SORT_UNCOUNTED; }
 
+// f(integral_constant ITEMS)
+template <class F>
+static void with_items(int64_t N, F&& f) {
+    if (sort_items(N) == 1) f(std::integral_constant<int, 1>{});
+    else f(std::integral_constant<int, SORT_ITEMS>{});
+}
+
 template <class ID>
 static int embedding_sort(const ID* ids, int64_t N, int64_t V, int64_t padding, const EmbWork& w, char* work, char* clear, int64_t clear_bytes,
                           const uint2** sorted, hipStream_t stream) {
     // workgroups that clear: 16 KB each while that leaves them one to a compute unit or fewer, then more
     const auto clearing = [](int64_t bytes) { return (unsigned)std::min<int64_t>(1024, ceil_div(bytes, 16384)); };
     uint2* pairs[2] = {reinterpret_cast<uint2*>(work + w.pairs[0]), reinterpret_cast<uint2*>(work + w.pairs[1])};
-    if (w.tiles <= 1) {
+    if (N <= SORT_TILE) {   // one workgroup
         const auto launch = [&](auto items) {
             hipLaunchKernelGGL((sort_small_kernel<ID, decltype(items)::value>), dim3(1 + clearing(clear_bytes)), dim3(SORT_THREADS), 0, stream, ids, (int)N, V, padding, w.passes,
                                w.bits, pairs[0], clear, clear_bytes);
@@ -991,22 +1004,25 @@ static int embedding_sort(const ID* ids, int64_t N, int64_t V, int64_t padding, 
     for (int p = 0; p < w.passes; ++p) {
         const int to = p == 0 ? 0 : 1 - from, shift = p * w.bits;
         const dim3 block(SORT_THREADS);
-        const auto pass = [&](auto first) {
+        const auto pass = [&](auto first, auto items) {
             constexpr bool FIRST = decltype(first)::value;
+            constexpr int ITEMS = decltype(items)::value;
             char* at = clear + cleared;
             int64_t bytes = mode == SORT_UNCOUNTED ? 0 : share(1);
             if (mode != SORT_UNCOUNTED)
-                hipLaunchKernelGGL((sort_count_kernel<ID, FIRST>), dim3((unsigned)w.tiles + clearing(bytes)), block, 0, stream, ids, (const uint2*)pairs[from], N, V, padding,
+                hipLaunchKernelGGL((sort_count_kernel<ID, FIRST, ITEMS>), dim3((unsigned)w.tiles + clearing(bytes)), block, 0, stream, ids, (const uint2*)pairs[from], N, V, padding,
                                    shift, w.bits, NO_KEY, (int)w.tiles, table, at, bytes);
             if (mode == SORT_SUMMED)
                 hipLaunchKernelGGL(sort_prefix_kernel, dim3((unsigned)ceil_div(1 << w.bits, 64)), block, 0, stream, table, (int)w.tiles, 1 << w.bits);
             at = clear + cleared;
             bytes = share(2);
-            hipLaunchKernelGGL((sort_scatter_kernel<ID, FIRST>), dim3((unsigned)w.tiles + clearing(bytes)), block, 0, stream, ids, (const uint2*)pairs[from], N, V, padding,
+            hipLaunchKernelGGL((sort_scatter_kernel<ID, FIRST, ITEMS>), dim3((unsigned)w.tiles + clearing(bytes)), block, 0, stream, ids, (const uint2*)pairs[from], N, V, padding,
                                shift, w.bits, table, (int)w.tiles, mode, pairs[to], at, bytes);
         };
-        if (p == 0) pass(std::true_type{});
-        else pass(std::false_type{});
+        with_items(N, [&](auto items) {
+            if (p == 0) pass(std::true_type{}, items);
+            else pass(std::false_type{}, items);
+        });
         if (int rc = check_launch("nerf_embedding_bwd(sort)")) return rc;
         from = to;
     }
@@ -1045,16 +1061,19 @@ static int embedding_narrow_bwd(const T* d_out, const ID* ids, int64_t N, int64_
         constexpr int VEC = decltype(vec)::value;
         const NarrowWork w = narrow_work(N, V, D);
         unsigned* const table = reinterpret_cast<unsigned*>(work + w.table);
-        unsigned* const items = reinterpret_cast<unsigned*>(work + w.items);
-        const BucketSums p{table + w.tiles * BUCKETS, items, reinterpret_cast<float*>(work + w.part), V, w.low, w.buckets, scale};
+        unsigned* const at = reinterpret_cast<unsigned*>(work + w.items);
+        const BucketSums p{table + w.tiles * BUCKETS, at, reinterpret_cast<float*>(work + w.part), V, w.low, w.buckets, scale};
         const dim3 tiles((unsigned)w.tiles), block(SORT_THREADS);
         const int mode = sort_mode(w.tiles);
-        if (mode != SORT_UNCOUNTED)
-            hipLaunchKernelGGL((sort_count_kernel<ID, true>), tiles, block, 0, stream, ids, (const uint2*)nullptr, N, V, padding, w.low, BUCKET_BITS, (unsigned)V, (int)w.tiles,
-                               table, (char*)nullptr, int64_t(0));
-        if (mode == SORT_SUMMED)
-            hipLaunchKernelGGL(sort_prefix_kernel, dim3(BUCKETS / 64), block, 0, stream, table, (int)w.tiles, BUCKETS);
-        hipLaunchKernelGGL((bucket_scatter_kernel<T, VEC, ID>), tiles, block, 0, stream, ids, N, V, padding, w.low, table, (int)w.tiles, mode, d_out, items);
+        with_items(N, [&](auto items) {
+            constexpr int ITEMS = decltype(items)::value;
+            if (mode != SORT_UNCOUNTED)
+                hipLaunchKernelGGL((sort_count_kernel<ID, true, ITEMS>), tiles, block, 0, stream, ids, (const uint2*)nullptr, N, V, padding, w.low, BUCKET_BITS, (unsigned)V, (int)w.tiles,
+                                   table, (char*)nullptr, int64_t(0));
+            if (mode == SORT_SUMMED)
+                hipLaunchKernelGGL(sort_prefix_kernel, dim3(BUCKETS / 64), block, 0, stream, table, (int)w.tiles, BUCKETS);
+            hipLaunchKernelGGL((bucket_scatter_kernel<T, VEC, ID, ITEMS>), tiles, block, 0, stream, ids, N, V, padding, w.low, table, (int)w.tiles, mode, d_out, at);
+        });
         if (int rc = check_launch("nerf_embedding_bwd(buckets)")) return rc;
         hipLaunchKernelGGL((bucket_sums_kernel<T, VEC>), dim3((unsigned)w.segments), dim3(BUCKET_THREADS), 0, stream, p, d_table);
         hipLaunchKernelGGL((bucket_join_kernel<T, VEC>), dim3((unsigned)w.buckets, (unsigned)ceil_div(1 << w.low, JOIN_IDS)), dim3(1024), 0, stream, p, d_table);
