@@ -116,6 +116,14 @@ def test_types(dev, tx, tg, reverse, blend, B, T, C, G):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tx,tg", [(F32, F32), (BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)])
+@pytest.mark.parametrize("B,C,G", [(1, 1, 1), (3, 1, 1), (2, 7, 7), (5, 64, 64), (3, 65, 5), (2, 66, 3), (7, 129, 1), (300, 1023, 1023), (1000, 12, 4), (1, 2050, 2050)])
+@pytest.mark.parametrize("blend,state", [(False, False), (True, True), (True, False)])
+def test_one_step(dev, tx, tg, B, C, G, blend, state):
+    check(dev, B, 1, C, G, tx, tg, reverse=C % 2 == 0, blend=blend, state=state, seed=C)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("B,T,C,G", [(4099, 5, 3, 1), (700, 64, 1, 1), (300, 192, 3, 1), (9, 192, 3, 3), (130, 1, 260, 260), (1, 20000, 4, 4),
                                      (1, 9000, 68, 1), (2, 1500, 520, 2), (1, 4097, 300, 1), (17, 100, 600, 600), (2, 40, 1030, 1),
                                      # tiles in a chain: two, some, several groups of them; every way to lay out the lanes
