@@ -67,8 +67,9 @@ static ScanShape scan_shape(int64_t B, int64_t T, int C, int G, int steps = 0) {
     s.units_per_b = G == C ? 1 : G;
     s.P = C / s.units_per_b;
     // Two or three channels of a gate: a lane takes them all (65536 x 192 x 3 float, one gate a step: 77 us, a lane a channel 112,
-    // backward 111 and 157; x 2 49 and 105).
-    s.vec = s.P % 4 == 0 ? 4 : G != C && s.P <= 3 ? s.P : 1;
+    // backward 111 and 157; x 2 49 and 105).  Of another even number two (x 6 159 and 192; 39475 x 17 x 100 in ten gates 156
+    // and 249; 4096 x 192 x 250 bfloat16 in five 288 and 296, backward 430 and 504).
+    s.vec = s.P % 4 == 0 ? 4 : G != C && s.P <= 3 ? s.P : G != C && s.P % 2 == 0 ? 2 : 1;
     s.steps = steps ? steps : scan_steps(G == C ? s.vec : 1);
     s.lcl = log2_up(std::min<int64_t>(ceil_div(s.P, s.vec), SCAN_COLS / s.vec));
     s.ls = std::min(log2_up(ceil_div(T, s.steps)), 8 - s.lcl);
