@@ -1217,8 +1217,10 @@ static int scan_check(const char* who, int64_t B, int64_t T, int C, int G, int g
     if (B == 0 || T == 0 || C == 0) return NERF_OK;
     NERF_REQUIRE(B <= (1ll << 40) && T <= (1ll << 40) && B * (double)T * C < 9e17, "%s: too large", who);
     const ScanShape s = scan_shape(B, T, C, G);
-    // a launch holds fewer than 2^32 threads
-    NERF_REQUIRE(s.blocks * (scan_chained(s) ? s.tiles : s.segments) < (1ll << 24) && (s.col_tiles == 1 || B * (double)T * G < (double)(1ll << 32)), "%s: too many workgroups", who);
+    // a launch holds fewer than 2^32 threads; one joins the sums of a shared gate's column tiles (more than 64 channels a gate),
+    // a thread each
+    NERF_REQUIRE(s.blocks * (scan_chained(s) ? s.tiles : s.segments) < (1ll << 24) && (G == C || s.col_tiles == 1 || B * (double)T * G < (double)(1ll << 32)),
+                 "%s: too many workgroups", who);
     return NERF_OK;
 }
 

@@ -480,3 +480,42 @@ def test_entry_points_refuse():
     bwd[5], bwd[17] = p, None
     assert lib.nerf_linear_scan_bwd(*bwd) == -22 and b"null workspace" in lib.nerf_last_error()
     assert lib.nerf_linear_scan_workspace_floats(1, 5000, 4, 3, 1) == 0
+
+
+def test_entry_points_take_more_than_two_to_the_32_elements():
+    """A gate for each channel has no sums over column tiles to hold, and the forward pass none at all: nothing about the
+    number of elements is refused.  (Null outputs stop the calls before anything is launched: no GPU needed.)"""
+    from nerf_amd import _lib as L
+    lib = L.lib()
+    p = 4096                                   # never dereferenced
+    for B, T, C, G in ((1, (1 << 22) + 3, 1028, 1028), (2, 1 << 23, 1024, 1024), (16, 1 << 20, 640, 640), (3, 1 << 21, 1030, 1030)):
+        assert B * T * G >= 1 << 32
+        assert lib.nerf_linear_scan_fwd(p, 1, p, 1, None, B, T, C, G, 0, 0, None, None, None, None, None) == -22
+        assert b"null pointer" in lib.nerf_last_error(), lib.nerf_last_error()
+        assert lib.nerf_linear_scan_bwd(p, 1, None, 1, None, p, p, None, B, T, C, G, 0, 0, p, p, None, p, None) == -22
+        assert b"null pointer" in lib.nerf_last_error(), lib.nerf_last_error()
+
+
+@pytest.mark.gpu
+def test_more_than_two_to_the_32_elements(dev):
+    """One sequence with a gate for each channel: the steps behind the last reset, and behind the first of all, in 64 bits."""
+    from nerf_amd import ops
+    T, C, near = (1 << 22) + 3, 1028, 90       # 4.3e9 elements of 2 bytes
+    gen = torch.Generator(device=dev).manual_seed(13)
+    x = torch.empty(1, T, C, device=dev, dtype=BF16).normal_(generator=gen).requires_grad_(True)
+    gate = torch.empty(1, T, C, device=dev, dtype=BF16).uniform_(generator=gen)
+    for cut in (near, T - near):               # nothing passes from one side of it to the other, in either direction
+        gate[:, cut] = 0.0
+    gate.requires_grad_(True)
+    h = ops.linear_scan(gate, x, blend=True)
+    d_gate, d_x = torch.autograd.grad(h, [gate, x], x.detach())
+    for steps in (slice(0, near), slice(T - near, T)):
+        for cols in (slice(0, 8), slice(509, 519), slice(C - 8, C)):
+            g, v = gate.detach()[:, steps, cols].cpu(), x.detach()[:, steps, cols].cpu()
+            want, tol = ref_scan(g, v, None, False, True, v, None), bounds(g, v, None, False, True, v, None)
+            if steps.start:                    # (what multiplies the gate of the cut comes from in front of it)
+                d_first = d_gate[:, steps.start, cols].float()
+                assert bool(torch.isfinite(d_first).all())
+                d_gate[:, steps.start, cols] = want[2][:, 0].to(dev, BF16)
+            for name, got, k in (("h", h, 0), ("d_gate", d_gate, 2), ("d_x", d_x, 3)):
+                assert_close(got[:, steps, cols], want[k], tol[k], (name, steps, cols))
