@@ -50,13 +50,21 @@ OptionalTensor floats(const Tensor& like, size_t n) {
 }
 
 // A leaf's gradient is accumulated on the stream where the first graph over it that is still alive was made.  While a stream
-// is captured that has to be the captured one: another stream would be drawn into the capture, which ends the process.
+// is captured that has to be a captured one (the same, or one that was forked from it): any other would be drawn into the
+// capture, which ends the process.
 void refuse_foreign_graph(const Tensor& t) {
     if (!t.is_leaf() || !t.requires_grad()) return;
-    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
-    if (!accumulator || !accumulator->stream()) return;
     const c10::Stream here = c10::hip::getCurrentHIPStream(t.get_device()).unwrap();
-    if (accumulator->stream()->id() != here.id())
+    const auto foreign = [&](torch::autograd::Node& node) {
+        const auto stream = node.stream();
+        if (!stream || (stream->id() == here.id() && stream->device_index() == here.device_index())) return false;
+        if (stream->id() == 0) return true;   // the default stream can neither be captured nor asked
+        const c10::Stream other(c10::Stream::UNSAFE, c10::Device(here.device_type(), stream->device_index()), stream->id());
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        return hipStreamIsCapturing(c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, other).stream(), &status) != hipSuccess || status != hipStreamCaptureStatusActive;
+    };
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (accumulator && foreign(*accumulator))
         throw EntryError("a graph over this tensor that was made outside the capture is still alive: drop or detach its outputs before capturing");
 }
 bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }

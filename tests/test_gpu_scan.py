@@ -519,3 +519,27 @@ def test_more_than_two_to_the_32_elements(dev):
                 d_gate[:, steps.start, cols] = want[2][:, 0].to(dev, BF16)
             for name, got, k in (("h", h, 0), ("d_gate", d_gate, 2), ("d_x", d_x, 3)):
                 assert_close(got[:, steps, cols], want[k], tol[k], (name, steps, cols))
+
+
+@pytest.mark.gpu
+def test_capture_takes_a_graph_of_a_forked_stream(dev):
+    """Nodes made on a stream that the capture has forked belong to it."""
+    from nerf_amd import ops
+    gate, x, _, _, _ = (t.to(dev) if t is not None else None for t in make(3, 70, 8, 2, F32, F32, False, 3))
+    leaf = x.clone().requires_grad_(True)
+    want = (ops.linear_scan(gate, leaf.detach()), ops.linear_scan(gate, leaf.detach() * 2))
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            first, twice = ops.linear_scan(gate, leaf), leaf * 2
+        torch.cuda.current_stream().wait_stream(side)
+        second = ops.linear_scan(gate, leaf)
+        third = ops.linear_scan(gate, twice)
+    for _ in range(3):
+        for t in (first, second, third):
+            t.detach().zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(first, want[0]) and torch.equal(second, want[0]) and torch.equal(third, want[1])
