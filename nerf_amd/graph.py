@@ -15,7 +15,9 @@ scheduler (src/train_nerf.py:87,204; src/train_nerf_ngp.py:57-62), whose rate re
 
 While the step is captured no autograd graph of an eager call over the same parameters may be alive (a loss that was kept,
 an output that still requires its gradient): the captured backward pass would meet the gradient accumulators that the eager
-graph made on another stream, which ends the process.  Drop or detach such results first.
+graph made on another stream, which ends the process.  Drop or detach such results first.  ``ops.embedding`` and
+``ops.linear_scan`` look for such graphs through everything that their operands were formed from and raise; a step that
+reaches the parameters by other operators alone is not looked at.
 """
 from __future__ import annotations
 

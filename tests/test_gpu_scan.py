@@ -522,6 +522,43 @@ def test_more_than_two_to_the_32_elements(dev):
 
 
 @pytest.mark.gpu
+def test_capture_refuses_a_live_eager_graph_of_what_formed_the_operands(dev):
+    """A leaf reached through other nodes, and a node that was made outside the capture, are refused like a leaf itself."""
+    from nerf_amd import ops
+    from nerf_amd._lib import NerfHipError
+    _, x, s, d_h, _ = (t.to(dev) for t in make(3, 70, 8, 2, F32, F32, True, 3))
+    sigma = torch.rand(3, 70, 2, device=dev, requires_grad=True)
+    table, ids = torch.randn(9, 8, device=dev, requires_grad=True), torch.arange(70, device=dev).expand(3, 70) % 9
+    start = s.clone().requires_grad_(True)
+    calls = {"gate": (sigma, lambda: ops.linear_scan(torch.exp(-sigma * 0.5), x)), "state": (start, lambda: ops.linear_scan(sigma.detach(), x, start * 2)),
+             "table": (table, lambda: ops.embedding(ids, (table * 0.5).reshape(9, 8)))}
+    for name, (leaf, call) in calls.items():
+        kept = call()
+        want = torch.autograd.grad(kept, leaf, d_h, retain_graph=True)[0]
+        torch.cuda.synchronize()
+        with pytest.raises(NerfHipError, match="still alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+        with torch.no_grad(), torch.cuda.graph(torch.cuda.CUDAGraph()):   # without a gradient there is nothing to refuse
+            call()
+        del kept
+        formed = leaf * 1.0                    # this node's graph is alive; the leaf is not an operand by itself
+        with pytest.raises(NerfHipError, match="still alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                ops.embedding(ids, formed) if name == "table" else ops.linear_scan(sigma.detach(), x, formed) if name == "state" else ops.linear_scan(formed, x)
+        del formed
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = torch.autograd.grad(call(), leaf, d_h)[0]
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want), name
+
+
+@pytest.mark.gpu
 def test_capture_takes_a_graph_of_a_forked_stream(dev):
     """Nodes made on a stream that the capture has forked belong to it."""
     from nerf_amd import ops
