@@ -254,6 +254,23 @@ std::optional<Tensors> grad_norm(const Tensors& params, Tensors grads, double ma
     return changed ? std::optional<Tensors>(std::move(grads)) : std::nullopt;
 }
 
+// Step counts as torch's Adam keeps them, a float each in host memory (a state loaded from elsewhere may hold another kind).
+float* host_float(const Tensor& t) { return t.is_cpu() && t.scalar_type() == at::kFloat && t.numel() == 1 ? static_cast<float*>(t.data_ptr()) : nullptr; }
+std::vector<int64_t> steps(const Tensors& list) {
+    std::vector<int64_t> out;
+    for (const Tensor& t : list) {
+        const float* at = host_float(t);
+        out.push_back((int64_t)(at ? *at : t.item<double>()));
+    }
+    return out;
+}
+void count_step(const Tensors& list) {   // in place
+    for (const Tensor& t : list) {
+        if (float* at = host_float(t)) *at += 1.0f;
+        else t.add_(1);
+    }
+}
+
 // One update with the gradients times norm[1]; `state`: of a group whose count and rate are in device memory.
 void adam_step(const Tensors& params, const Tensors& grads, const Tensors& m, const Tensors& v, int64_t step, const OptionalTensor& state, double lr, double beta1,
                double beta2, double eps, double weight_decay, const Tensor& norm) {
@@ -288,6 +305,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("embedding", &embedding, py::call_guard<py::gil_scoped_release>());
     m.def("linear_scan", &linear_scan, py::call_guard<py::gil_scoped_release>());
     m.def("grad_norm", &grad_norm, py::call_guard<py::gil_scoped_release>());
+    m.def("steps", &steps, py::call_guard<py::gil_scoped_release>());
+    m.def("count_step", &count_step, py::call_guard<py::gil_scoped_release>());
     m.def("adam_step", &adam_step, py::call_guard<py::gil_scoped_release>());
     m.attr("entries") = std::vector<std::string>{
 #define X(name) #name,

@@ -97,6 +97,13 @@ class FusedAdam(torch.optim.Optimizer):
         super().__setstate__(state)
         for name, value in (("max_grad_norm", None), ("_norm", None), ("_dev_state", {}), ("_dev_lr", {})):
             self.__dict__.setdefault(name, value)
+        seen = set()   # a step tensor is counted on in place, so each parameter has one of its own
+        for st in self.state.values():
+            step = st.get("step") if isinstance(st, dict) else None
+            if torch.is_tensor(step) and not step.is_cuda:
+                if step.data_ptr() in seen:
+                    st["step"] = step = step.clone()
+                seen.add(step.data_ptr())
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
@@ -138,35 +145,21 @@ class FusedAdam(torch.optim.Optimizer):
             if group.get("capturable", False):
                 dev = self._capturable_state(gi, ps)
                 self.sync_lr()
-                parts = [(0, None, range(len(ps)))]
+                parts = [(0, range(len(ps)))]
             else:
-                dev, parts = None, self._shared_steps(states)
+                dev, steps = None, [st["step"] for st in states]
+                taken = native.steps(steps)
+                if taken.count(taken[0]) == len(taken):
+                    parts = [(taken[0], range(len(ps)))]
+                else:   # states loaded piecemeal, or a parameter without a gradient in some step
+                    parts = [(n, [i for i, k in enumerate(taken) if k == n]) for n in dict.fromkeys(taken)]
             beta1, beta2 = group["betas"]
             ms, vs = [st["exp_avg"] for st in states], [st["exp_avg_sq"] for st in states]
-            for step0, step, part in parts:
+            for step0, part in parts:
                 lists = (ps, grads, ms, vs) if len(part) == len(ps) else tuple([ts[i] for i in part] for ts in (ps, grads, ms, vs))
                 native.adam_step(*lists, step0 + 1, dev, group["lr"], beta1, beta2, group["eps"], group["weight_decay"], self._norm)
-                if step is not None:
-                    step = step + 1   # a new tensor: a parameter without a gradient in this step keeps the old one
-                    for i in part:
-                        states[i]["step"] = step
-
-    @staticmethod
-    def _shared_steps(states):
-        """(steps taken, step tensor, members) of the states that have taken equally many: normally all of them, unless
-        states were loaded piecemeal or a parameter had no gradient in some step.  The members of a part are left with
-        one step tensor between them, which is never written, so that counting a step is one operation and not one per
-        parameter (``state_dict`` hands out a copy for each)."""
-        first = states[0]["step"]
-        if all([st["step"] is first for st in states]):
-            return [(int(first.item()), first, range(len(states)))]
-        by_tensor = {}
-        for i, st in enumerate(states):
-            by_tensor.setdefault(id(st["step"]), []).append(i)
-        by_count = {}
-        for members in by_tensor.values():
-            by_count.setdefault(int(states[members[0]]["step"].item()), []).extend(members)
-        return [(count, states[members[0]]["step"], members) for count, members in by_count.items()]
+                if dev is None:
+                    native.count_step(steps if len(part) == len(ps) else [steps[i] for i in part])
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -219,5 +212,5 @@ class FusedAdam(torch.optim.Optimizer):
                     group["betas"][0], group["betas"][1], group["eps"], group["weight_decay"],
                     L.stream_of(plist[0])), "nerf_adam_step")
                 for p in plist:
-                    self.state[p]["step"] = self.state[p]["step"] + 1   # not in place: clipped steps share the tensor
+                    self.state[p]["step"] += 1
         return loss

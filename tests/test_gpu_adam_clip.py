@@ -303,3 +303,48 @@ def test_entry_points_refuse():
         count, p, ptrs, ptrs, ptrs, n, step, None, 0.1, b1, b2, 1e-8, 0.0, scale, None)
     for k in ({"count": -1}, {"p": None}, {"p": null}, {"step": 0}, {"b1": 1.0}, {"b2": -0.1}, {"scale": None}):
         assert step(**k) == -22 and lib.nerf_last_error(), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("limit", [None, 1e9])
+def test_every_parameter_keeps_its_own_step_tensor(dev, limit):
+    """As with torch's Adam: a step count taken from the state goes on counting, and setting one leaves the others alone."""
+    from nerf_amd.optim import FusedAdam
+    ps, _ = make([(40, 3), (17,), (4097,)], 1.0, 5, dev)
+    a = [torch.nn.Parameter(p.clone().to(dev)) for p in ps]
+    b = [torch.nn.Parameter(p.clone().to(dev)) for p in ps]
+    mine, ref = FusedAdam(a, lr=1e-2, max_grad_norm=limit), torch.optim.Adam(b, lr=1e-2)
+    for step in range(6):
+        gs = make([p.shape for p in ps], 1.0, 70 + step, dev)[1]
+        for p, q, g in zip(a, b, gs):
+            p.grad, q.grad = g.to(dev), g.to(dev)
+        mine.step()
+        ref.step()
+        if step == 1:
+            held = [mine.state[p]["step"] for p in a]
+            assert len({t.data_ptr() for t in held}) == 3
+        elif step == 2:
+            held[1].zero_()
+            ref.state[b[1]]["step"].zero_()
+        for k, (p, q) in enumerate(zip(a, b)):
+            assert float(mine.state[p]["step"]) == float(ref.state[q]["step"]), (step, k)
+            assert step < 1 or mine.state[p]["step"] is held[k], (step, k)
+            assert torch.allclose(p, q, rtol=2e-6, atol=1e-7 * (step + 1)), (step, k)      # the bound the unclipped step is held to
+
+
+def test_shared_step_tensors_are_told_apart_on_loading():
+    """A state whose parameters hold one step tensor between them (no GPU needed)."""
+    import pickle
+    from nerf_amd.optim import FusedAdam
+    params = [torch.nn.Parameter(torch.ones(3)) for _ in range(3)]
+    opt = FusedAdam(params, max_grad_norm=1.0)
+    one = torch.tensor(4.0)
+    for p in params:
+        opt.state[p] = {"step": one, "exp_avg": torch.zeros(3), "exp_avg_sq": torch.zeros(3)}
+    fresh = FusedAdam([torch.nn.Parameter(torch.ones(3)) for _ in range(3)], max_grad_norm=1.0)
+    shared = torch.optim.Optimizer.state_dict(opt)
+    assert len({st["step"].data_ptr() for st in shared["state"].values()}) == 1
+    fresh.load_state_dict(shared)
+    for twin in (fresh, copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        steps = [st["step"] for st in twin.state.values()]
+        assert len(steps) == 3 and all(float(t) == 4.0 for t in steps) and len({t.data_ptr() for t in steps}) == 3
