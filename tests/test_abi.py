@@ -36,3 +36,20 @@ def test_cpu_tensors_are_rejected():
         ops.encode_pe(torch.zeros(4, 3), 4)
     with pytest.raises(NerfHipError):
         ops.composite(torch.zeros(2, 4, 3), torch.zeros(2, 4), torch.zeros(2, 4))
+
+
+def test_the_library_builds_without_torch():
+    """`make` for a user of the C ABI alone: with a Python that finds no torch (-S: no installed packages) the library is still
+    the whole build; with the installed torch the autograd nodes are part of it."""
+    import subprocess
+    csrc = os.path.join(ROOT, "nerf_amd", "csrc")
+
+    def commands(*args):   # printed, not run
+        r = subprocess.run(["make", "-C", csrc, "-n", "-B", *args], capture_output=True, text=True)
+        assert r.returncode == 0, r.stderr
+        return r.stdout
+
+    alone = commands("PYTHON=python3 -S -E")
+    assert "libnerf_hip.so" in alone and "scan.hip" in alone and "autograd.cpp" not in alone
+    whole = commands()
+    assert "libnerf_hip.so" in whole and "autograd.cpp" in whole
