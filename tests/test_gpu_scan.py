@@ -580,3 +580,63 @@ def test_capture_takes_a_graph_of_a_forked_stream(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(first, want[0]) and torch.equal(second, want[0]) and torch.equal(third, want[1])
+
+
+# (type of x, of the gate, reverse, blend)
+KINDS = [(F32, F32, False, False), (F32, F32, False, True), (BF16, BF16, False, False), (BF16, BF16, True, True), (BF16, F32, False, True), (BF16, F32, True, False),
+         (F16, F16, True, False), (F16, F32, False, False)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tx,tg,reverse,blend", KINDS)
+@pytest.mark.parametrize("B,T,C,G", [
+    # tiles in a chain, by columns a lane: four with a gate each (backward alone; both; sixteen steps a thread where all is of 16
+    # bits), four, one and two of a shared gate, one with a gate each (sixteen steps a thread wherever x is of 16 bits)
+    (3, 300, 132, 132), (3, 600, 132, 132), (3, 1100, 132, 132), (2, 1500, 520, 2), (4, 1100, 130, 2), (4, 600, 100, 2), (2, 1200, 252, 2), (4, 1021, 65, 65)])
+def test_chains_by_type(dev, tx, tg, reverse, blend, B, T, C, G):
+    check(dev, B, T, C, G, tx, tg, reverse, blend, state=not reverse, seed=T)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tx,tg,reverse,blend", [(BF16, BF16, False, False), (F16, F32, True, True)])
+@pytest.mark.parametrize("B,T,C,G", [(8, 4500, 6, 1), (8, 9000, 8, 1), (8, 17000, 12, 4), (8, 16500, 1, 1), (2, 17000, 520, 2), (2, 9000, 520, 520)])
+def test_long_chains_by_type(dev, tx, tg, reverse, blend, B, T, C, G):
+    """Few lanes side by side, so that a tile is thousands of steps; several groups of tiles."""
+    check(dev, B, T, C, G, tx, tg, reverse, blend, state=True, seed=C)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tx,tg", [(F32, F32), (BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)])
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("blend", [False, True])
+@pytest.mark.parametrize("B,T", [(300, 192), (37, 196), (37, 197)])
+@pytest.mark.parametrize("C", [1, 2, 3, 4])
+def test_rays_of_few_channels(dev, tx, tg, reverse, blend, B, T, C):
+    """One gate for one to four channels, whose steps are moved in whole pieces of 16 bytes: all of them whole, the last one
+    partial, and none where a sequence does not start on a piece."""
+    check(dev, B, T, C, 1, tx, tg, reverse, blend, state=C % 2 == 1, seed=C)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tx,tg,reverse,blend", KINDS[2:])
+@pytest.mark.parametrize("C", [2, 3, 4])
+def test_rays_of_few_channels_in_segments(dev, tx, tg, reverse, blend, C):
+    check(dev, 2, 2056, C, 1, tx, tg, reverse, blend, state=True, seed=C)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [3, 40])
+def test_gate_gradient_of_most_channels(dev, T):
+    """One gate for 131072 channels: the sum over all of them, in 2048 column tiles.  A term passes the additions of its lane
+    (3) and of 16 lanes (4) and up to 2048 over the tiles, in the place of the P that bounds() allows; all terms are positive, so
+    that a tile left out or taken twice, 1/2048 of the sum, is beyond the bound (below 1/7000)."""
+    from nerf_amd import ops
+    B, C = 2, 131072
+    gen = torch.Generator().manual_seed(T)
+    gate, x, d_h = torch.rand(B, T, 1, generator=gen), torch.rand(B, T, C, generator=gen) + 0.5, torch.rand(B, T, C, generator=gen) + 0.5
+    leaf = gate.to(dev).requires_grad_(True)
+    (got,) = torch.autograd.grad(ops.linear_scan(leaf, x.to(dev), reverse=True), leaf, d_h.to(dev))
+    want = ref_scan(gate, x, None, True, False, d_h)[2]
+    tol = bounds(gate, x, None, True, False, d_h, None)[2] * ((4 * T + 2055 + 128) / (4 * T + C + 128))
+    assert float(tol.max() / want.max()) < 1 / 7000
+    assert_close(got, want, tol, T)
