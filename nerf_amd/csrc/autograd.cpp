@@ -52,28 +52,20 @@ OptionalTensor floats(const Tensor& like, size_t n) {
 }
 
 // A node's backward runs on the stream that was current when it was made, and a leaf's gradient is accumulated on the stream
-// where the first graph over it that is still alive was made.  While a stream is captured those have to be captured ones (the
-// same, or one that was forked from it): any other would be drawn into the capture, which ends the process.  So everything that
-// the operand was formed from is looked at, down to the leaves.
-void refuse_foreign_graph(const Tensor& t) {
+// where the first graph over it that is still alive was made.  A captured backward pass draws such a stream into the capture
+// and joins it again, but the default stream cannot be captured: that ends the process.  So everything that the operand was
+// formed from is looked at, down to the leaves.
+void refuse_eager_graph(const Tensor& t) {
     if (!t.requires_grad()) return;
-    const c10::Stream here = c10::hip::getCurrentHIPStream(t.get_device()).unwrap();
-    const auto foreign = [&](torch::autograd::Node& node) {
-        const auto stream = node.stream();
-        if (!stream || (stream->id() == here.id() && stream->device_index() == here.device_index())) return false;
-        if (stream->id() == 0) return true;   // the default stream can neither be captured nor asked
-        const c10::Stream other(c10::Stream::UNSAFE, c10::Device(here.device_type(), stream->device_index()), stream->id());
-        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-        return hipStreamIsCapturing(c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, other).stream(), &status) != hipSuccess || status != hipStreamCaptureStatusActive;
-    };
     std::vector<std::shared_ptr<torch::autograd::Node>> next{t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn()};
     std::unordered_set<torch::autograd::Node*> seen;
     while (!next.empty()) {
         const auto node = std::move(next.back());
         next.pop_back();
         if (!node || !seen.insert(node.get()).second) continue;
-        if (foreign(*node))
-            throw EntryError("a graph over this tensor that was made outside the capture is still alive: drop or detach its outputs before capturing");
+        const auto stream = node->stream();
+        if (stream && stream->id() == 0)   // the default one
+            throw EntryError("a graph over this tensor that was made outside the capture, on the default stream, is still alive: drop or detach its outputs before capturing");
         for (const auto& edge : node->next_edges()) next.push_back(edge.function);
     }
 }
@@ -132,7 +124,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
 Tensor embedding(const Tensor& ids, const Tensor& table, double scale, int64_t padding) {
     c10::DeviceGuard guard(table.device());
     if (at::GradMode::is_enabled() && table.requires_grad()) {
-        if (capturing()) refuse_foreign_graph(table);
+        if (capturing()) refuse_eager_graph(table);
         return Embedding::apply(table, ids, scale, padding);
     }
     return embedding_fwd(dense(table), ids, scale);
@@ -204,9 +196,9 @@ std::pair<Tensor, OptionalTensor> linear_scan(const Tensor& gate, const Tensor& 
     c10::DeviceGuard guard(x.device());
     if (at::GradMode::is_enabled() && (gate.requires_grad() || x.requires_grad() || (state && state->requires_grad()))) {
         if (capturing()) {
-            refuse_foreign_graph(gate);
-            refuse_foreign_graph(x);
-            if (state) refuse_foreign_graph(*state);
+            refuse_eager_graph(gate);
+            refuse_eager_graph(x);
+            if (state) refuse_eager_graph(*state);
         }
         auto out = LinearScan::apply(gate, x, state, reverse, blend, want_last);
         return {out[0], want_last ? OptionalTensor(out[1]) : std::nullopt};

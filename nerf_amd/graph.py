@@ -13,11 +13,12 @@ step count and the learning rate on the device (``FusedAdam(capturable=True)``).
 (its loops are eager PyTorch); a captured step computes what the eager step computes -- including under a learning-rate
 scheduler (src/train_nerf.py:87,204; src/train_nerf_ngp.py:57-62), whose rate reaches the device in front of each replay.
 
-While the step is captured no autograd graph of an eager call over the same parameters may be alive (a loss that was kept,
-an output that still requires its gradient): the captured backward pass would meet the gradient accumulators that the eager
-graph made on another stream, which ends the process.  Drop or detach such results first.  ``ops.embedding`` and
-``ops.linear_scan`` look for such graphs through everything that their operands were formed from and raise; a step that
-reaches the parameters by other operators alone is not looked at.
+While the step is captured no autograd graph over the same parameters may be alive that an eager call made on the default
+stream (a loss that was kept, an output that still requires its gradient): the captured backward pass would meet gradient
+accumulators of that stream, which cannot be captured, and that ends the process.  Drop or detach such results first.  (Graphs
+of other streams, those of the warm-up among them, become part of the capture.)  ``ops.embedding`` and ``ops.linear_scan``
+look for such graphs through everything that their operands were formed from and raise; a step that reaches the parameters by
+other operators alone is not looked at.
 """
 from __future__ import annotations
 

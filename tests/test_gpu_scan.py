@@ -582,6 +582,41 @@ def test_capture_takes_a_graph_of_a_forked_stream(dev):
         assert torch.equal(first, want[0]) and torch.equal(second, want[0]) and torch.equal(third, want[1])
 
 
+@pytest.mark.gpu
+def test_capture_takes_a_live_graph_of_another_stream(dev):
+    """A graph that is alive on a stream other than the default one does not stand in the way: its accumulators' stream
+    becomes part of the capture.  (What a warm-up on a side stream leaves behind.)"""
+    from nerf_amd import ops
+    gate, x, s, d_h, _ = (t.to(dev) for t in make(3, 70, 8, 2, F32, F32, True, 3))
+    sigma, start = torch.rand(3, 70, 2, device=dev, requires_grad=True), s.clone().requires_grad_(True)
+    table, ids = torch.randn(9, 8, device=dev, requires_grad=True), torch.arange(70, device=dev).expand(3, 70) % 9
+    calls = {"gate": (sigma, lambda: ops.linear_scan(torch.exp(-sigma * 0.5), x)), "state": (start, lambda: ops.linear_scan(gate, x, start)),
+             "table": (table, lambda: ops.embedding(ids, table))}
+    side = torch.cuda.Stream()
+    for name, (leaf, call) in calls.items():
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            kept = call()
+            want = torch.autograd.grad(kept, leaf, d_h, retain_graph=True)[0]
+        torch.cuda.synchronize()
+        for whole in (False, True):            # the gradient handed back, and accumulated in the leaf
+            leaf.grad = None
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                if whole:
+                    call().backward(d_h)
+                    got = leaf.grad
+                else:
+                    got = torch.autograd.grad(call(), leaf, d_h)[0]
+            for _ in range(3):
+                got.zero_()
+                graph.replay()
+                torch.cuda.synchronize()
+                assert torch.equal(got, want), (name, whole)
+        leaf.grad = None
+        del kept
+
+
 # (type of x, of the gate, reverse, blend)
 KINDS = [(F32, F32, False, False), (F32, F32, False, True), (BF16, BF16, False, False), (BF16, BF16, True, True), (BF16, F32, False, True), (BF16, F32, True, False),
          (F16, F16, True, False), (F16, F32, False, False)]
