@@ -229,6 +229,10 @@ int nerf_gather_kept_by_slot(const float* d_rgb, const float* d_sigma, const int
  * Made for |gate| <= 1; larger gates are right as long as float32 holds their products over
  * stretches of the sequence.  A state that has become infinite or NaN stays one or the other (an
  * infinity may turn into a NaN; no gate takes it back), and leaves other channels alone.  C <= 131072.
+ * Workgroups along a long sequence hand the state on to each other.  Each waits for what runs already, and for at most
+ * 2^20 reads, over a second: should a word not come by then, which no input brings about, the steps
+ * behind it are NaN, with NERF_OK returned long before.  last is composed, not replayed: it and the last
+ * step of h agree to float32 rounding, not in every bit.
  * carry: nerf_linear_scan_carry_floats(B,T,C,G) floats that the backward pass needs (NULL: not
  * kept).  workspace: nerf_linear_scan_workspace_floats(B,T,C,G,backward) floats, NULL where that is
  * 0.  T >= 1; B = 0 or C = 0 is nothing to do (no output is written).  Every pointer 16-byte aligned.

@@ -1,5 +1,5 @@
 // What of the package's host side is in C++: the two operators that enter autograd's graph from here, ops.embedding and
-// ops.linear_scan, and the pointer lists of the clipped optimiser step.  A backward pass written in
+// ops.linear_scan, and the pointer lists and step counts of the clipped optimiser step.  A backward pass written in
 // Python costs a small call more than its kernels -- autograd's thread has to take the interpreter's lock and run cold
 // code -- so allocation, launch and graph node are here; ops.py checks the arguments.  Host code only: every kernel is
 // reached through the C ABI, whose functions ops.py's binding hands over (bind), so that both use one library.

@@ -43,9 +43,9 @@ constexpr unsigned NO_KEY = 0xffffffffu;
 
 // ---- forward ---------------------------------------------------------------------------------------------------
 // A group of lanes per row, 16 bytes a lane where the row divides into them.  Bound by the reads of the rows and the writes
-// where those are long (65536 rows of 1024 bfloat16: 39 us, 6.8 TB/s, the rate of a fill, since rows come from the caches
-// again), by the lines that a row of a few bytes touches where they are short (2^20 rows of two floats out of 2^19: 9.8 us
-// for 24 MB of ids, rows and outputs).  Four rows a group at a time were no faster (1 % on either side of it).
+// where those are long (65536 rows of 1024 bfloat16 out of 50021: 44 us, 6.1 TB/s, above a copy's rate, since some rows come
+// from the caches again), by the lines that a row of a few bytes touches where they are short (2^20 rows of two floats out of
+// 2^19: 11.6 us for 21 MB of ids, rows and outputs).  Four rows a group at a time were no faster (1 % on either side of it).
 template <class T, int VEC, class ID>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(const T* __restrict__ table, int64_t V, int D, const ID* __restrict__ ids, int64_t N,
                                                             float scale, int l_lanes, T* __restrict__ out) {
@@ -395,7 +395,7 @@ struct EmbSums {
 // A wave holds 64 / lanes sorted positions at a time, one per group of lanes, and adds them up by a scan that stops where
 // the id changes; what the last group holds is carried into the next round.  The rows of ROUNDS rounds are under way at
 // once.  WHOLE: all 64 lanes on one row -- the id is the wave's, and nothing changes lanes.  Bound by the reads of the rows,
-// and by their latency where there are few: 131072 rows of 32 float 6 us (17 MB), 16384 of 1024 bfloat16 14 us (34 MB).
+// and by their latency where there are few: 65536 rows of 32 float 6.8 us (8 MB), 16384 of 1024 bfloat16 15 us (34 MB).
 template <class T, int VEC, bool WHOLE>
 __global__ __launch_bounds__(256) void embedding_sums_kernel(EmbSums p, const T* __restrict__ d_out, T* __restrict__ d_table) {
     constexpr int ROUNDS = 8;
@@ -487,7 +487,7 @@ __global__ __launch_bounds__(256) void embedding_sums_kernel(EmbSums p, const T*
 
 // The runs that cross chunks: a run belongs to the chunk that it starts in.  Those over a few chunks are joined by a
 // group of lanes each, longer ones by the whole workgroup.  A few dependent reads long whatever there is to join: 7 us where
-// there is little, 13 for 40 runs over a hundred chunks each.
+// there is little, 13 for 40 runs over some fifty chunks each.
 template <class T, int VEC>
 __global__ __launch_bounds__(JOIN_THREADS) void embedding_join_kernel(EmbSums p, T* __restrict__ d_table) {
     constexpr int FEW = 16;   // against 8: runs over 8 to 15 chunks 39 us and 52 (262144 ids of 1000 rows), shorter ones 0.7 us more

@@ -23,7 +23,7 @@
 // batch entry; G < C: one unit of P columns per (batch entry, gate).  A workgroup of 256 threads is cut into groups of
 // CL x S threads: CL lanes side by side on the columns of a unit (VEC each), S slices of K steps.  Both passes are
 // bound by memory: the forward pass moves gate + x + h once, the backward pass gate, x, dh in and d_gate, d_x out.  16384 rays
-// x 192 x 32 float, one gate a step: 141 us for 818 MB and 233 for 1.23 GB, 5.8 and 5.3 TB/s, against 5.1 for a large copy.
+// x 192 x 32 float, one gate a step: 141 us for 818 MB and 240 for 1.23 GB, 5.8 and 5.1 TB/s, against 5.1 for a large copy.
 #include <algorithm>
 
 #include "typed.h"
@@ -66,8 +66,8 @@ static ScanShape scan_shape(int64_t B, int64_t T, int C, int G, int steps = 0) {
     s.B = B; s.T = T; s.C = C; s.G = G;
     s.units_per_b = G == C ? 1 : G;
     s.P = C / s.units_per_b;
-    // Two or three channels of a gate: a lane takes them all (65536 x 192 x 3 float, one gate a step: 77 us, a lane a channel 112,
-    // backward 111 and 157; x 2 49 and 105).  Of another even number two (x 6 159 and 192; 39475 x 17 x 100 in ten gates 156
+    // Two or three channels of a gate: a lane takes them all (65536 x 192 x 3 float, one gate a step: 78 us, a lane a channel 112,
+    // backward 115 and 157; x 2 55 and 105), in dense pieces where it can (see scan_fwd_kernel).  Of another even number two (x 6 159 and 192; 39475 x 17 x 100 in ten gates 156
     // and 249; 4096 x 192 x 250 bfloat16 in five 288 and 296, backward 430 and 504).
     s.vec = s.P % 4 == 0 ? 4 : G != C && s.P <= 3 ? s.P : G != C && s.P % 2 == 0 ? 2 : 1;
     s.steps = steps ? steps : scan_steps(G == C ? s.vec : 1);
@@ -750,8 +750,8 @@ template <int VEC, bool DENSE>
 constexpr bool scan_buffers() { return VEC == 4 && !DENSE; }
 
 // DENSE: a lane has all channels of a sequence and its steps are one piece of memory (few channels, the rays of a picture):
-// they move 16 bytes at a time.  65536 rays x 192 x 3 float: 107 us step by step, 82 so; x 1: 69 and 27.  (Backward 139 and
-// 120, 106 and 43.)
+// they move 16 bytes at a time.  65536 rays x 192 x 3 float: 78 us, step by step (193 samples) 103; x 2 55 and 93, x 1 26 and
+// 70.  (Backward 115 and 179, 80 and 144, 47 and 122.)
 template <class GT, class XT, int VEC, int GV, int K, bool CHAIN, bool DENSE>
 __global__ __launch_bounds__(SCAN_THREADS, CHAIN ? 4 : 1) void scan_fwd_kernel(ScanArgs p) {
     __shared__ float s_a[2][4][SCAN_COLS], s_x[2][4][SCAN_COLS], s_part[CHAIN ? CHAIN_GROUP : 1][2][SCAN_COLS];

@@ -441,7 +441,8 @@ def linear_scan(gate: torch.Tensor, x: torch.Tensor, state: Optional[torch.Tenso
     and h rounded once to the type of ``x``.  A gate of zero starts a new sequence.  Gates are meant to lie in [-1, 1];
     larger ones are right while float32 holds their products.  At most 131072 channels.
     ``return_state``: ``(h, last)``, ``last`` [..., C] float32 the state after the last step, unrounded: what the next call
-    takes as ``state`` (a long sequence in parts, or one step at a time with T = 1).
+    takes as ``state`` (a long sequence in parts, or one step at a time with T = 1); it is composed of stretches, so that it and
+    the last step of h agree to float32 rounding, not in every bit.
     Differentiable once in ``gate``, ``x`` and ``state``."""
     # (the texts of these checks are only put together where one fails: a call may take a few microseconds in all)
     shape, gates = tuple(x.shape), tuple(gate.shape)

@@ -10,7 +10,8 @@ not implemented and raise.  ``clip_grad_norm_`` (src/train_nerf.py:165) lives in
 ``max_grad_norm`` does the same clipping inside ``step()``: the 2-norm of the gradients of all groups together, and
 Adam on the gradients times min(1, max_grad_norm / (norm + 1e-6)), formed as they are read -- the gradients themselves
 are left as they are.  ``grad_norm`` is then the norm of the last step, a 0-d tensor on the device (the same tensor for
-every step, also under a captured graph), NaN or infinite where a gradient is, as with ``clip_grad_norm_``.
+every step, also under a captured graph), NaN or infinite where a gradient is, as with ``clip_grad_norm_``.  A captured
+step keeps the ``max_grad_norm`` that it was captured with.
 
 ``capturable=True`` (torch's name for it) keeps the step count AND the learning rate in device memory, so that a
 whole training step -- this optimiser's launch included -- can be captured into a HIP graph and replayed
