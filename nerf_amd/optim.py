@@ -63,6 +63,15 @@ class FusedAdam(torch.optim.Optimizer):
                 self.state[p]["step"] = view
         return dev
 
+    def _leave_capturable(self, gi: int) -> None:
+        """A group that is no longer capturable: every parameter counts for itself again, on the host."""
+        view = self._dev_state.pop(gi)[1]
+        self._dev_lr.pop(gi, None)
+        for p in self.param_groups[gi]["params"]:
+            st = self.state.get(p)
+            if st and st["step"] is view:
+                st["step"] = view.detach().cpu()
+
     def sync_lr(self) -> None:
         """Send every capturable group's ``lr`` to its device state if it differs from what the device holds (one
         one-thread launch per changed group on the current stream, nothing when unchanged).  Under stream capture
@@ -101,7 +110,7 @@ class FusedAdam(torch.optim.Optimizer):
         seen = set()   # a step tensor is counted on in place, so each parameter has one of its own
         for st in self.state.values():
             step = st.get("step") if isinstance(st, dict) else None
-            if torch.is_tensor(step) and not step.is_cuda:
+            if torch.is_tensor(step):
                 if step.data_ptr() in seen:
                     st["step"] = step = step.clone()
                 seen.add(step.data_ptr())
@@ -148,6 +157,8 @@ class FusedAdam(torch.optim.Optimizer):
                 self.sync_lr()
                 parts = [(0, range(len(ps)))]
             else:
+                if gi in self._dev_state:
+                    self._leave_capturable(gi)
                 dev, steps = None, [st["step"] for st in states]
                 taken = native.steps(steps)
                 if taken.count(taken[0]) == len(taken):
@@ -199,6 +210,8 @@ class FusedAdam(torch.optim.Optimizer):
                     group["betas"][0], group["betas"][1], group["eps"], group["weight_decay"],
                     L.stream_of(ps[0])), "nerf_adam_step_capturable")
                 continue
+            if gi in self._dev_state:
+                self._leave_capturable(gi)
             # parameters of one group share the step count unless states were loaded piecemeal
             by_step = {}
             for p in ps:

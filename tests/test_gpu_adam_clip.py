@@ -348,3 +348,30 @@ def test_shared_step_tensors_are_told_apart_on_loading():
     for twin in (fresh, copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
         steps = [st["step"] for st in twin.state.values()]
         assert len(steps) == 3 and all(float(t) == 4.0 for t in steps) and len({t.data_ptr() for t in steps}) == 3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("limit", [None, 1e9])
+@pytest.mark.parametrize("copied", [False, True])
+def test_a_group_that_is_capturable_for_a_while(dev, limit, copied):
+    """The parameters of a capturable group share their step count in device memory; before and after they count for themselves."""
+    from nerf_amd.optim import FusedAdam
+    ps, _ = make([(40, 3), (17,), (4097,)], 1.0, 6, dev)
+    a = [torch.nn.Parameter(p.clone().to(dev)) for p in ps]
+    b = [torch.nn.Parameter(p.clone().to(dev)) for p in ps]
+    mine, ref = FusedAdam(a, lr=1e-2, max_grad_norm=limit), torch.optim.Adam(b, lr=1e-2)
+    for step in range(8):
+        gs = make([p.shape for p in ps], 1.0, 90 + step, dev)[1]
+        if step == 4 and copied:
+            a, mine = copy.deepcopy((a, mine))
+        mine.param_groups[0]["capturable"] = step in (2, 3, 7)
+        for k, (p, q, g) in enumerate(zip(a, b, gs)):
+            p.grad, q.grad = (None, None) if (step, k) == (5, 1) else (g.to(dev), g.to(dev))
+        if step == 7:                          # one count for the group again
+            mine.state[a[1]]["step"] += 1
+            ref.state[b[1]]["step"] += 1
+        mine.step()
+        ref.step()
+        for k, (p, q) in enumerate(zip(a, b)):
+            assert float(mine.state[p]["step"]) == float(ref.state[q]["step"]), (step, k)
+            assert torch.allclose(p, q, rtol=2e-6, atol=1e-7 * (step + 1)), (step, k)
